@@ -281,6 +281,153 @@ typedef struct {
 int kk_plan_get_info(const kk_plan* plan, kk_plan_info* info);
 void kk_plan_free(kk_plan* plan);
 
+/* ------------------------------------------------------------------ operators over an 8-bit cache
+ * For the language models that stand before the synthesis in a program that talks (they write the text
+ * or the phonemes that kk_forward_batch reads), on the same context and device: the norms and position
+ * rotation of queries and keys, a paged cache of keys and values in 8 bits, and attention over it.  No
+ * counterpart in the reference.  Like kk_snake_block_noalloc they work on the caller's device memory,
+ * and they allocate nothing, keep nothing between calls and never synchronize:
+ *  - `stream` is a hipStream_t of the context's device (NULL: its null stream).  A call checks its
+ *    arguments, enqueues its kernels there and returns; the calls can be captured into a HIP graph, which
+ *    reads the device arrays again at each replay.  The caller's current device is left as it was.
+ *  - All arrays are device memory of the context's device, the structs host memory read during the call.
+ *  - Calls on one context may overlap with each other and with every other entry; two calls that write
+ *    the same memory are ordered by the caller's streams.  A workspace belongs to one call at a time: calls
+ *    (and graphs) that may run at the same time take a workspace each.
+ *  - KK_ERR_INVALID and a message for arguments that are out of range, before anything is enqueued.
+ *    What only the device knows (row_start, len, table) is checked by the kernels: see kk_kv_batch. */
+#define KK_BF16 1
+#define KK_F16 2
+#define KK_F32 3
+
+/* RMS norm of each head of q and k and the rotation by its row's position, in one pass:
+ *   y = x / sqrt(mean(x^2) + eps) * weight          (norm = 0: y = x; weight NULL: 1)
+ *   (y_a, y_b) of pair i -> (y_a cos t - y_b sin t, y_b cos t + y_a sin t),  t = pos * f_i
+ * for the pairs i < rot / 2: values (i, i + rot / 2) of a head, or (2 i, 2 i + 1) with `interleaved`; values
+ * from `rot` on are not rotated.  f_i = freq[i] (radians a position), or theta^(-2 i / rot) where freq is
+ * NULL.  Everything is computed in 32 bits, the angle in 64, and rounded once.
+ * Strides are in values: row r, head h of q lies at q + r * q_row + h * q_head, its `dim` values next to
+ * each other.  An output may be its input (same strides), and must not overlap it otherwise.  The wide
+ * path takes pointers and strides that are multiples of 16 bytes, rot / 2 and dim - rot that are multiples
+ * of 8 (of 4 for f32; with `interleaved` also rot of twice that); the others are right and slower. */
+typedef struct {
+    int32_t type;              /* KK_BF16, KK_F16, KK_F32: q, k and the outputs */
+    int32_t dim;               /* values a head: even, 2..512 */
+    int32_t rows;              /* >= 0 */
+    int32_t q_heads, k_heads;  /* >= 0 each: 0 leaves that side out */
+    const void* q;
+    int64_t q_row, q_head;
+    const void* k;
+    int64_t k_row, k_head;
+    void* q_out;
+    int64_t q_out_row, q_out_head;
+    void* k_out;
+    int64_t k_out_row, k_out_head;
+    int32_t norm;              /* 1: RMS norm, 0: rotation only */
+    float eps;                 /* >= 0 */
+    const float* q_weight;     /* [dim], or NULL */
+    const float* k_weight;
+    const int32_t* pos;        /* [rows] */
+    int32_t rot;               /* even, 0..dim */
+    int32_t interleaved;
+    double theta;              /* > 0 */
+    const double* freq;        /* [rot / 2], or NULL */
+} kk_norm_rope;
+int kk_qk_norm_rope(kk_ctx* ctx, const kk_norm_rope* args, void* stream, char* err, size_t errlen);
+
+/* A cache of keys and values: pages of KK_KV_PAGE tokens of every head, 8 bits a value, and one scale for
+ * each (page, head) of K and one of V; a value is its stored number times its scale.  V is stored with a
+ * value's tokens next to each other, which is how the matrix cores read it.  Scales are at least 2^-90, or
+ * 0 for a page that holds only zeros. */
+#define KK_KV_PAGE 64
+#define KK_KV_INT8 1 /* -127..127 */
+#define KK_KV_E4M3 2 /* 8-bit floating point, 4 bits of exponent and 3 of mantissa, up to 448 */
+typedef struct {
+    int32_t type;   /* KK_KV_* */
+    int32_t heads;  /* >= 1 */
+    int32_t dim;    /* 64, 96, 128, 192 or 256 */
+    int32_t pages;  /* >= 1 */
+    void* k;        /* [pages][heads][KK_KV_PAGE][dim] bytes, 16-byte aligned */
+    void* v;        /* [pages][heads][dim][KK_KV_PAGE] bytes, 16-byte aligned */
+    float* k_scale; /* [pages][heads] */
+    float* v_scale; /* [pages][heads] */
+    int32_t* fault; /* one word, or NULL: where a kernel meets a bad batch it sets KK_KV_BAD_* bits */
+} kk_kv_cache;
+
+/* A ragged batch of sequences over a cache.  Rows [row_start[b], row_start[b + 1]) of a call's tensors are
+ * the last tokens of sequence b, whose len[b] tokens (these included) lie in pages table[b][0..]: token t
+ * in page table[b][t / 64], slot t % 64.  max_new and max_len bound the rows and the tokens of any sequence;
+ * they size the launch.  Rows outside all sequences are neither read nor written.
+ * Checked on the device: a sequence whose rows leave [0, rows), exceed max_new, or whose len leaves [0, max_len]
+ * is left out (KK_KV_BAD_BATCH; the table is not read); a page number outside [0, pages) is not accessed: nothing
+ * is written there, and what is read there is NaN (KK_KV_BAD_PAGE). */
+#define KK_KV_BAD_BATCH 1
+#define KK_KV_BAD_PAGE 2
+typedef struct {
+    int32_t n;                /* sequences, >= 0 */
+    int32_t rows;             /* rows of the call's tensors, >= 0 */
+    int32_t max_new;          /* >= 0 */
+    int32_t max_len;          /* 0..64 table_width */
+    const int32_t* row_start; /* [n + 1], not falling */
+    const int32_t* len;       /* [n] */
+    const int32_t* table;     /* [n] rows of table_width page numbers */
+    int32_t table_width;
+    int64_t table_stride;     /* from a sequence's row to the next, in page numbers */
+} kk_kv_batch;
+
+/* Keys and values of a batch's rows: row r, head h of k lies at k + r * k_row + h * k_head (in values). */
+typedef struct {
+    int32_t type; /* KK_BF16, KK_F16, KK_F32 */
+    void* k;
+    int64_t k_row, k_head;
+    void* v;
+    int64_t v_row, v_head;
+} kk_kv_rows;
+
+/* Stores the batch's rows (read from `rows`) as the last tokens of their sequences (len counts them: it must be
+ * at least the sequence's rows, else KK_KV_BAD_BATCH).  In each page and head written, for K and for V:
+ *  - scale' = max(|x|) / 127 (e4m3: / 448) over the finite new values, at least 2^-90; 0 if they are all 0;
+ *  - a page written from slot 0 on takes it; a page that holds earlier tokens keeps its scale where that is as
+ *    large, and grows to scale' where not: its earlier tokens are stored again, round(stored * scale / scale').
+ *    Each growth costs those tokens up to another half step of the new scale;
+ *  - stored = x / scale (as x times the reciprocal) rounded to nearest even; infinities become the largest
+ *    stored number, NaN 0.
+ * Slots behind a sequence's last token stay as they are.  A page that is written belongs to one sequence of the
+ * batch (pages shared by several are for reading: kk_kv_read, kk_kv_attention). */
+int kk_kv_write(kk_ctx* ctx, const kk_kv_cache* cache, const kk_kv_batch* batch, const kk_kv_rows* rows, void* stream,
+                char* err, size_t errlen);
+/* The batch's rows back into `rows`: the last row_start[b + 1] - row_start[b] tokens of each sequence, stored number
+ * times scale, rounded once to the type (len as for kk_kv_write). */
+int kk_kv_read(kk_ctx* ctx, const kk_kv_cache* cache, const kk_kv_batch* batch, const kk_kv_rows* rows, void* stream,
+               char* err, size_t errlen);
+
+/* Attention of the batch's rows over their sequences' tokens: out = sum_t p_t v_t, p = softmax over the tokens t that
+ * a row sees of scale * q . k_t.  Query head h reads cache head h / (heads / cache->heads).  Row i of a sequence's m
+ * rows stands at position len - m + i; with `causal` it sees the tokens up to its own position, with `window` > 0 (then
+ * causal is needed) the last `window` of those; without, all len tokens.  A row that sees nothing (len 0, a position below 0)
+ * gives zeros.  Scores, softmax and sums are f32; the stored numbers enter the matrix products exactly, the
+ * queries to 2^-24 of a row's largest value, probabilities with 11 bits (scales of V that differ by over 2^100 within what a
+ * row sees are out of f32's range).  The result does not depend on what else
+ * is in the batch, except that the axis is split by max_len and the batch's size (the order of f32 sums). */
+typedef struct {
+    int32_t type;  /* KK_BF16 or KK_F16: q and out */
+    int32_t heads; /* query heads, a multiple of cache->heads */
+    const void* q;
+    int64_t q_row, q_head; /* in values */
+    void* out;             /* not q */
+    int64_t out_row, out_head;
+    float scale; /* > 0 */
+    int32_t causal, window;
+    void* workspace;       /* 16-byte aligned, kk_kv_attention_workspace bytes or more; need not be cleared */
+    size_t workspace_bytes;
+} kk_kv_attention_args;
+/* The workspace that kk_kv_attention needs for these arguments (0: none), or negative KK_ERR_* for arguments that it would
+ * refuse.  It depends on n, rows, max_new, max_len, heads, dim and window alone. */
+int64_t kk_kv_attention_workspace(kk_ctx* ctx, const kk_kv_cache* cache, const kk_kv_batch* batch,
+                                  const kk_kv_attention_args* args, char* err, size_t errlen);
+int kk_kv_attention(kk_ctx* ctx, const kk_kv_cache* cache, const kk_kv_batch* batch, const kk_kv_attention_args* args,
+                    void* stream, char* err, size_t errlen);
+
 /* ------------------------------------------------------------------ output formats (src/wav.rs)
  * PCM_16 encoding of the last run's audio on the device (wav::encode, src/wav.rs:63-80): per
  * sample v = round_ties_even(s * 32767) in f32; values outside [-32768, 32767] (NaN and the

@@ -24,6 +24,7 @@
 #include "kk_common.h"
 #include "kk_host.h"
 #include "kk_kernels.h"
+#include "kk_kv.h"
 #include "kokoro_hip.h"
 
 namespace kk {
@@ -274,6 +275,9 @@ struct kk_ctx {
 };
 
 namespace kk {
+
+int ctx_device(const kk_ctx* ctx) { return ctx->device; }
+int ctx_cus(const kk_ctx* ctx) { return ctx->n_cu; }
 
 static int round_up(int v, int m) { return (v + m - 1) / m * m; }
 

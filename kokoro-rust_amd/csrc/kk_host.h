@@ -18,4 +18,11 @@ constexpr int kGapT = 2;  // GAP_T (src/gpu_batch.rs:29): gap token rows after e
 // predicted frames later.
 std::string ids_item_error(const kk_item& it, int b);
 
+// The refusals of the operators over an 8-bit cache, or "": what the host can see of their arguments (sizes, types, null
+// pointers, alignment, and sizes that a launch could not hold).
+std::string norm_rope_error(const kk_norm_rope* a);
+std::string kv_batch_error(const kk_kv_cache* c, const kk_kv_batch* b);
+std::string kv_rows_error(const kk_kv_rows* r);
+std::string kv_attention_error(const kk_kv_cache* c, const kk_kv_batch* b, const kk_kv_attention_args* a);
+
 }  // namespace kk

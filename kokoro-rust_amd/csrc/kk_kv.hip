@@ -1,0 +1,273 @@
+// kk_kv.hip -- writing tokens into the 8-bit cache, and reading them back.
+//
+// Bound by memory: a value is read in 16 bits and written in 8 (and the other way round).  One block per (page of a
+// sequence, head, K or V) holds the page's new tokens in registers, so their largest value, the page's scale and the
+// stored bytes come from one pass; nothing of a page is shared between blocks.  V goes through LDS once more, because the
+// cache holds a value's tokens next to each other: bytes are written [token][dim] and taken out as 4 x 4 byte blocks.
+#include "kk_kv.h"
+
+namespace kk {
+namespace {
+
+// The page that a block works on; its number in the cache, or -1 for one that does not exist.
+template <int THREADS>
+__device__ __forceinline__ bool kv_page(const KvCacheDev& c, const KvBatchDev& B, int per_seq, bool report, KvPage& p,
+                                        int& page, int* found) {
+    KvSeq s;
+    int i;
+    if (per_seq) {
+        const int b = blockIdx.x / per_seq;
+        i = blockIdx.x - b * per_seq;
+        if (!kv_seq(B, b, s)) {
+            if (report && threadIdx.x == 0) kv_fault(c, KK_KV_BAD_BATCH);
+            return false;
+        }
+    } else {
+        i = kv_find<THREADS>(c, B, blockIdx.x, 1, kPage, 2, report && blockIdx.x == 0, s, found);
+        if (i < 0) return false;
+    }
+    if (!kv_page_rows(s, i, p)) {
+        if (report && threadIdx.x == 0 && s.m > s.len) kv_fault(c, KK_KV_BAD_BATCH);
+        return false;
+    }
+    page = B.table[s.b * B.stride + p.at];
+    if (page < 0 || page >= c.pages) {
+        if (report && threadIdx.x == 0) kv_fault(c, KK_KV_BAD_PAGE);
+        page = -1;
+    }
+    return true;
+}
+
+// 4 x 4 bytes transposed: o[i] byte j = w[j] byte i.
+__device__ __forceinline__ void transpose4(const uint32_t w[4], uint32_t o[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);
+    const uint32_t c = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+    o[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+    o[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+    o[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+    o[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
+
+__device__ __forceinline__ uint32_t byte_mask(int first, int lo, int hi) {  // bytes first..first+3 that lie in [lo, hi)
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (first + i >= lo && first + i < hi) m |= 0xffu << (8 * i);
+    return m;
+}
+
+constexpr int kKvThreads = 256;
+
+template <int T, int CT, int D>
+__global__ void __launch_bounds__(kKvThreads) kv_write_kernel(KvCacheDev c, KvBatchDev B, KvRowsDev R, int per_seq) {
+    constexpr int kChunks = D / 8, kMine = kPage * kChunks / kKvThreads;  // 8-value chunks of a token, of a thread
+    constexpr int kLd = D + 4;                                           // bytes of a token's row in LDS
+    __shared__ int found[2];
+    __shared__ float wave_top[kKvThreads / 64];
+    __shared__ uint32_t lds[kPage * kLd / 4];
+    const int head = blockIdx.y >> 1, is_v = blockIdx.y & 1, tid = threadIdx.x;
+    KvPage p;
+    int id;
+    if (!kv_page<kKvThreads>(c, B, per_seq, blockIdx.y == 0, p, id, found) || id < 0) return;
+    float* scale_at = (is_v ? c.vs : c.ks) + (int64_t)id * c.heads + head;
+    const float scale_was = p.lo ? *scale_at : 0.0f;
+    const void* src = is_v ? R.v : R.k;
+    const int64_t row_step = is_v ? R.v_row : R.k_row, head_step = is_v ? R.v_head : R.k_head;
+    const bool vec = is_v ? R.v_vec : R.k_vec;
+    uint8_t* page = (is_v ? c.v : c.k) + ((int64_t)id * c.heads + head) * (kPage * D);
+
+    float x[kMine][8];
+    float top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kMine; j++) {
+        const int slot = (tid + j * kKvThreads) / kChunks, ch = (tid + j * kKvThreads) % kChunks;
+        if (slot >= p.lo && slot < p.hi) {
+            load_values<T, 8>(src, (p.row0 + slot - p.lo) * row_step + head * head_step + ch * 8, vec, x[j]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[j][i] = 0.0f;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < kMine; j++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float m = fabsf(x[j][i]);
+            top = fmaxf(top, m <= 3.402823466e38f ? m : 0.0f);  // NaN and infinities do not count
+        }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
+    if ((tid & 63) == 0) wave_top[tid >> 6] = top;
+    __syncthreads();
+    top = wave_top[0];
+#pragma unroll
+    for (int i = 1; i < kKvThreads / 64; i++) top = fmaxf(top, wave_top[i]);
+
+    const float want = top > 0.0f ? fmaxf(top * (CT == KK_KV_E4M3 ? 1.0f / 448.0f : 1.0f / 127.0f), kScaleLeast) : 0.0f;
+    const float scale = fmaxf(scale_was, want);
+    const bool grown = p.lo > 0 && scale > scale_was;
+    const float ratio = grown ? scale_was / scale : 1.0f;
+    const float inv = scale > 0.0f ? 1.0f / scale : 0.0f;
+    if (tid == 0) *scale_at = scale;
+#pragma unroll
+    for (int j = 0; j < kMine; j++) {
+        const int slot = (tid + j * kKvThreads) / kChunks, ch = (tid + j * kKvThreads) % kChunks;
+        uint2 w;
+        w.x = pack4<CT>(f32x4{x[j][0] * inv, x[j][1] * inv, x[j][2] * inv, x[j][3] * inv});
+        w.y = pack4<CT>(f32x4{x[j][4] * inv, x[j][5] * inv, x[j][6] * inv, x[j][7] * inv});
+        if (is_v) {
+            lds[slot * (kLd / 4) + ch * 2] = w.x;
+            lds[slot * (kLd / 4) + ch * 2 + 1] = w.y;
+            continue;
+        }
+        uint2* at = (uint2*)(page + slot * D + ch * 8);
+        if (slot >= p.lo && slot < p.hi) {
+            *at = w;
+        } else if (grown && slot < p.lo) {
+            uint2 o = *at;
+            o.x = pack4<CT>(unpack4f<CT>(o.x) * ratio);
+            o.y = pack4<CT>(unpack4f<CT>(o.y) * ratio);
+            *at = o;
+        }
+    }
+    if (!is_v) return;
+    __syncthreads();
+    // 16 tokens of 4 values a thread
+    for (int t = tid; t < D; t += kKvThreads) {
+        const int first = (t & 3) * 16, d = (t >> 2) * 4;
+        if (first >= p.hi || (first + 16 <= p.lo && !grown)) continue;
+        uint32_t o[4][4];
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            uint32_t w[4], y[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = lds[(first + 4 * g + i) * (kLd / 4) + d / 4];
+            transpose4(w, y);
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[i][g] = y[i];
+        }
+        const bool whole = first >= p.lo && first + 16 <= p.hi;
+        if (!whole && !grown) {  // a few tokens: their bytes alone
+            const int a = max(p.lo - first, 0), b = min(p.hi - first, 16);
+#pragma unroll
+            for (int k = 0; k < 16; k++)
+                if (k >= a && k < b)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        page[(d + i) * kPage + first + k] = (uint8_t)(o[i][k >> 2] >> (8 * (k & 3)));
+            continue;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            uint4* at = (uint4*)(page + (d + i) * kPage + first);
+            uint32_t old[4] = {0, 0, 0, 0};
+            if (!whole) __builtin_memcpy(old, at, 16);
+            uint4 w;
+            uint32_t* wp = (uint32_t*)&w;
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const uint32_t now = byte_mask(first + 4 * g, p.lo, p.hi), was = byte_mask(first + 4 * g, 0, p.lo);
+                const uint32_t again = was ? pack4<CT>(unpack4f<CT>(old[g]) * ratio) : 0;
+                wp[g] = (o[i][g] & now) | (again & was) | (old[g] & ~(now | was));
+            }
+            *at = w;
+        }
+    }
+}
+
+template <int T, int CT, int D>
+__global__ void __launch_bounds__(kKvThreads) kv_read_kernel(KvCacheDev c, KvBatchDev B, KvRowsDev R, int per_seq) {
+    constexpr int kChunks = D / 8, kMine = kPage * kChunks / kKvThreads;
+    constexpr int kLd = D + 4;
+    __shared__ int found[2];
+    __shared__ uint32_t lds[kPage * kLd / 4];
+    const int head = blockIdx.y >> 1, is_v = blockIdx.y & 1, tid = threadIdx.x;
+    KvPage p;
+    int id;
+    if (!kv_page<kKvThreads>(c, B, per_seq, blockIdx.y == 0, p, id, found)) return;
+    const bool bad = id < 0;
+    const int64_t at = (int64_t)(bad ? 0 : id) * c.heads + head;
+    const float scale = bad ? __uint_as_float(0x7fc00000u) : (is_v ? c.vs : c.ks)[at];
+    const uint8_t* page = (is_v ? c.v : c.k) + at * (kPage * D);
+    void* dst = is_v ? R.v : R.k;
+    const int64_t row_step = is_v ? R.v_row : R.k_row, head_step = is_v ? R.v_head : R.k_head;
+    const bool vec = is_v ? R.v_vec : R.k_vec;
+    if (is_v) {
+        for (int t = tid; t < D; t += kKvThreads) {
+            const int first = (t & 3) * 16, d = (t >> 2) * 4;
+            uint32_t w[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) __builtin_memcpy(w[i], page + (d + i) * kPage + first, 16);
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const uint32_t v[4] = {w[0][g], w[1][g], w[2][g], w[3][g]};
+                uint32_t y[4];
+                transpose4(v, y);
+#pragma unroll
+                for (int i = 0; i < 4; i++) lds[(first + 4 * g + i) * (kLd / 4) + d / 4] = y[i];
+            }
+        }
+        __syncthreads();
+    }
+    uint2 w[kMine];
+#pragma unroll
+    for (int j = 0; j < kMine; j++) {
+        const int slot = (tid + j * kKvThreads) / kChunks, ch = (tid + j * kKvThreads) % kChunks;
+        w[j] = is_v ? uint2{lds[slot * (kLd / 4) + ch * 2], lds[slot * (kLd / 4) + ch * 2 + 1]}
+                    : *(const uint2*)(page + slot * D + ch * 8);
+    }
+#pragma unroll
+    for (int j = 0; j < kMine; j++) {
+        const int slot = (tid + j * kKvThreads) / kChunks, ch = (tid + j * kKvThreads) % kChunks;
+        if (slot < p.lo || slot >= p.hi) continue;
+        const f32x4 a = unpack4f<CT>(w[j].x) * scale, b = unpack4f<CT>(w[j].y) * scale;
+        const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        store_values<T, 8>(dst, (p.row0 + slot - p.lo) * row_step + head * head_step + ch * 8, vec, x);
+    }
+}
+
+typedef void (*KvKernel)(KvCacheDev, KvBatchDev, KvRowsDev, int);
+
+template <bool WRITE, int T, int CT>
+KvKernel kv_kernel_of(int dim) {
+#define KK_KV_CASE(D) \
+    case D: return WRITE ? kv_write_kernel<T, CT, D> : kv_read_kernel<T, CT, D>;
+    switch (dim) {
+        KK_KV_CASE(64)
+        KK_KV_CASE(96)
+        KK_KV_CASE(128)
+        KK_KV_CASE(192)
+        KK_KV_CASE(256)
+    }
+#undef KK_KV_CASE
+    return nullptr;
+}
+template <bool WRITE, int T>
+KvKernel kv_kernel_of(int cache, int dim) {
+    return cache == KK_KV_INT8 ? kv_kernel_of<WRITE, T, KK_KV_INT8>(dim) : kv_kernel_of<WRITE, T, KK_KV_E4M3>(dim);
+}
+
+template <bool WRITE>
+hipError_t kv_launch(const kk_kv_cache& c, const kk_kv_batch& b, const kk_kv_rows& r, hipStream_t s) {
+    const int e = r.type == KK_F32 ? 4 : 2;
+    auto whole = [&](const void* p, int64_t row, int64_t head) {
+        return (uintptr_t)p % 16 == 0 && row * e % 16 == 0 && head * e % 16 == 0;
+    };
+    const KvRowsDev d{r.k, r.v, r.k_row, r.k_head, r.v_row, r.v_head, whole(r.k, r.k_row, r.k_head), whole(r.v, r.v_row, r.v_head)};
+    const KvKernel k = r.type == KK_BF16  ? kv_kernel_of<WRITE, KK_BF16>(c.type, c.dim)
+                       : r.type == KK_F16 ? kv_kernel_of<WRITE, KK_F16>(c.type, c.dim)
+                                          : kv_kernel_of<WRITE, KK_F32>(c.type, c.dim);
+    const KvTiles t = kv_tiles(b);
+    return launch(k, dim3((unsigned)t.tiles, 2 * (unsigned)c.heads), dim3(kKvThreads), 0, s, kv_dev(c), kv_dev(b), d, t.per_seq);
+}
+
+}  // namespace
+
+hipError_t launch_kv_write(const kk_kv_cache& c, const kk_kv_batch& b, const kk_kv_rows& r, hipStream_t s) {
+    return kv_launch<true>(c, b, r, s);
+}
+hipError_t launch_kv_read(const kk_kv_cache& c, const kk_kv_batch& b, const kk_kv_rows& r, hipStream_t s) {
+    return kv_launch<false>(c, b, r, s);
+}
+
+}  // namespace kk

@@ -1,0 +1,686 @@
+// kk_kv_attn.hip -- attention over the 8-bit cache.
+//
+// Mathematics.  With page scales a (K) and b (V), stored numbers k, v and a row's scale c = scale log2(e):
+//   s_t = c a (q . k_t),  out = sum_t 2^{s_t} b v_t / sum_t 2^{s_t}
+// in one pass over the pages, keeping per row M, the largest s_t + log2 b seen, and m, the largest s_t (or up to kSlack below them),
+//   P_t = 2^{s_t + log2 b - M + kLift},  O = sum P_t v_t = 2^{kLift - M} sum 2^{s_t} b v_t,
+//   l = sum_t 2^{s_t - m}: a page's sum of P_t times 2^{M - kLift - log2 b - m},  out = 2^{M - kLift - m} O / l.
+// Folding log2 b into the exponent costs nothing (it goes into the constant of the fused multiply-add) and leaves the
+// stored numbers themselves as operands: int8 and e4m3 are exact in f16, so K and V enter the matrix cores without a
+// rounding, Q as f16 scaled per row to [2^14, 2^15) (a bf16 value keeps its 8 bits down to 2^-28 of the row's largest), and
+// P as f16: 11 bits, and 2^-24 is 2^-35 of the largest P or less (kLift = 11; M lags by kSlack = 4 bits at most, so P <= 2^15).
+// f16 rather than bf16 for P because a row that sees one token would otherwise be rounded to 8 bits twice.
+// M and m are apart so that scales of V far from 1 stay in range; a page of zeros (b = 0) adds to l alone, its P relative to
+// its own largest s.  O and l are rescaled only when M or m move by more than kSlack.
+//
+// Layout.  Everything is transposed, S^T = K Q^T and O^T = V^T P^T, so that a query row stays on one lane column: its M, m and l are
+// one value a lane, a rescale multiplies a lane's own O, and the lanes that compute S hold exactly the P that the second
+// product wants, once the 64 tokens of a page are taken in the right order (a sum over tokens may run in any).
+#include "kk_kv.h"
+
+namespace kk {
+namespace {
+
+constexpr float kSlack = 4.0f, kLift = 11.0f;
+
+struct AttnDev {
+    const void* q;
+    void* out;
+    int64_t q_row, q_head, out_row, out_head;
+    float* acc;   // [rows][heads][parts][dim]
+    float2* ml;   // [rows][heads][parts]: m and l
+    float c;      // scale log2(e)
+    int heads, group, type, causal, window, q_vec, out_vec;
+    int chunk, parts, tile_rows;
+};
+
+__device__ __forceinline__ float other_half(float x, bool maximum) {  // with the lane 32 away
+    const uint32_t u = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const float a = __uint_as_float(r[0]), b = __uint_as_float(r[1]);
+    return maximum ? fmaxf(a, b) : a + b;
+}
+__device__ __forceinline__ float other_row(float x, bool maximum) {  // with the lane 16 away
+    const uint32_t u = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const float a = __uint_as_float(r[0]), b = __uint_as_float(r[1]);
+    return maximum ? fmaxf(a, b) : a + b;
+}
+
+// N query values to f16 in units of 2^(e - 14), e the exponent of the row's largest, which `top` holds for the whole row.
+__device__ __forceinline__ void q_units(float top, float& down, float& up) {
+    int e = (int)(__float_as_uint(top) >> 23) & 255;
+    e = min(max(e, 27), 254);
+    down = __uint_as_float((uint32_t)(268 - e) << 23);
+    up = __uint_as_float((uint32_t)(e - 14) << 23);
+}
+
+template <int N>
+__device__ __forceinline__ void load_query(const AttnDev& a, int64_t at, float* x) {
+    if (a.type == KK_BF16)
+        load_values<KK_BF16, N>(a.q, at, a.q_vec, x);
+    else
+        load_values<KK_F16, N>(a.q, at, a.q_vec, x);
+}
+
+// Four values of a row, next to each other, behind a division by l (or as a part's).
+__device__ __forceinline__ void store_out4(const AttnDev& a, int64_t at, const float* x) {
+    uint16_t e[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) e[i] = a.type == KK_BF16 ? f32_to_bf16_bits(x[i]) : ElemOf<KK_F16>::store(x[i]);
+    uint16_t* p = (uint16_t*)a.out + at;
+    if (a.out_vec) {
+        uint2 w;
+        __builtin_memcpy(&w, e, 8);
+        *(uint2*)p = w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) p[i] = e[i];
+    }
+}
+
+// A page's number and scales; one that does not exist is page 0 with a NaN scale.
+struct PageIn {
+    int64_t at;
+    float k_scale, v_scale;
+    int live;  // slots that hold tokens of the sequence: the bytes of V behind them, which may be the NaN code, are masked
+};
+__device__ __forceinline__ PageIn page_in(const KvCacheDev& c, const KvBatchDev& B, const KvSeq& s, int page, int head,
+                                          bool report) {
+    int id = __builtin_amdgcn_readfirstlane(B.table[s.b * B.stride + page]);
+    const bool bad = id < 0 || id >= c.pages;
+    if (bad) {
+        if (report) kv_fault(c, KK_KV_BAD_PAGE);
+        id = 0;
+    }
+    PageIn p;
+    p.at = (int64_t)id * c.heads + head;
+    p.live = bad ? 0 : s.len - page * kPage;
+    p.k_scale = bad ? __uint_as_float(0x7fc00000u) : c.ks[p.at];
+    p.v_scale = bad ? 0.0f : c.vs[p.at];  // the scores are NaN: rows that do not see the page stay clean
+    return p;
+}
+
+// A row's maxima and sum; `page` brings in a page with V's scale b, in which the row's largest s is `top`.  Returns whether any
+// row of the wave moved (then O is to be multiplied by f); P = 2^{s + off}, and the sum of P counts w in l.
+struct RowSum {
+    float M = -INFINITY, m = -INFINITY, l = 0.0f;
+    __device__ __forceinline__ bool page(float b, float top, float& f, float& off, float& w) {
+        const bool zero = b == 0.0f;
+        const float b_log = zero ? 0.0f : __builtin_amdgcn_logf(b);
+        const bool up_M = !zero && top + b_log > M + kSlack, up_m = top > m + kSlack;
+        const bool moves = __ballot(up_M || up_m) != 0;
+        if (moves) {
+            const float to_M = up_M ? top + b_log : M, to_m = up_m ? top : m;
+            f = up_M ? __builtin_amdgcn_exp2f(M - to_M) : 1.0f;
+            if (up_m) l *= __builtin_amdgcn_exp2f(m - to_m);
+            M = to_M, m = to_m;
+        }
+        const float r = zero ? top : M - b_log, ref = r == -INFINITY ? 0.0f : r;
+        off = kLift - ref;
+        w = __builtin_amdgcn_exp2f(fminf(ref - kLift - (m == -INFINITY ? 0.0f : m), 126.0f));
+        return moves;
+    }
+    // what brings O to units of 2^-m, as l is
+    __device__ __forceinline__ float last() const {
+        return __builtin_amdgcn_exp2f(M - kLift - (m == -INFINITY ? 0.0f : m));
+    }
+};
+
+// ------------------------------------------------------------------ few rows: single tokens, drafts
+
+// At most 16 NT rows of a (sequence, cache head).  Bound by reading the cache once.  Each of a block's four waves takes every
+// fourth page of the part straight into registers, in 16-byte loads that are the MFMA operands (v_mfma_f32_16x16x32_f16)
+// once unpacked; nothing of the cache goes through LDS.  Row i of K's token tile t is token 16 (i / 4) + 4 t + i % 4: then
+// lane group g's scores are those of tokens 16 g .. 16 g + 15 in order, the 16 bytes that it loads of each row of V.
+// K of the next page is loaded while this one's softmax and second product run, V while its first product runs.
+template <int D, int CT, int NT>
+__global__ void __launch_bounds__(256, D <= 192 && D * NT <= 256 ? 2 : 1) attend_few_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
+    constexpr bool kWide = D % 64 == 0;            // 16 bytes of a K row a lane, else 8
+    constexpr int kLoads = kWide ? D / 64 : D / 32;  // of each token tile
+    constexpr int kSteps = D / 32, kDim = D / 16;
+    constexpr int kLd = D + 4;
+    __shared__ float lds_ml[4][NT * 16][2];
+    __shared__ float lds_o[2][NT * 16][kLd];
+    const int head = blockIdx.x % c.heads, rest = blockIdx.x / c.heads;
+    const int part = rest % a.parts, b = rest / a.parts;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, g = lane >> 4;
+    KvSeq s;
+    if (!kv_seq(B, b, s)) {
+        if (threadIdx.x == 0 && head == 0 && part == 0) kv_fault(c, KK_KV_BAD_BATCH);
+        return;
+    }
+    if (s.m == 0) return;
+    const Span sp = span_of(s, a.causal, a.window, a.chunk, 0, s.m - 1);
+    if (part >= sp.parts) return;
+    const int page0 = sp.lo + part * a.chunk, page1 = min(page0 + a.chunk, sp.hi);
+
+    // the rows of this lane's columns: queries and the tokens [lo, hi) that they see
+    f16x8 q[NT][kSteps];
+    float qs[NT];
+    int lo[NT], hi[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const int r = n * 16 + col, i = r / a.group;
+        const bool on = i < s.m;
+        float x[D / 4];
+#pragma unroll
+        for (int j = 0; j < D / 4; j++) x[j] = 0.0f;
+        if (on) {
+            const int64_t at = (int64_t)(s.r0 + i) * a.q_row + (head * a.group + r % a.group) * a.q_head;
+#pragma unroll
+            for (int j = 0; j < kLoads; j++) {
+                if constexpr (kWide)
+                    load_query<16>(a, at + j * 64 + g * 16, x + 16 * j);
+                else
+                    load_query<8>(a, at + j * 32 + g * 8, x + 8 * j);
+            }
+        }
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < D / 4; j++) top = fmaxf(top, fabsf(x[j]));
+        top = other_half(other_row(top, true), true);
+        float down;
+        q_units(top, down, qs[n]);
+        qs[n] *= a.c;
+#pragma unroll
+        for (int j = 0; j < kSteps; j++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) q[n][j][k] = (_Float16)(x[8 * j + k] * down);
+        const int pos = s.len - s.m + i;
+        hi[n] = on ? (a.causal ? max(0, min(s.len, pos + 1)) : s.len) : 0;
+        lo[n] = a.window ? max(0, pos - a.window + 1) : 0;
+    }
+    // tokens that every row sees
+    const int all_lo = a.window ? s.len - a.window : 0, all_hi = a.causal ? s.len - s.m + 1 : s.len;
+
+    f32x4 o[NT][kDim];
+    RowSum rs[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+#pragma unroll
+        for (int d = 0; d < kDim; d++) o[n][d] = f32x4{0, 0, 0, 0};
+    }
+
+    uint4 kr[4][kLoads];
+    auto load_k = [&](const PageIn& p) {
+        const uint8_t* base = c.k + p.at * (kPage * D);
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const uint8_t* row = base + ((col >> 2) * 16 + t * 4 + (col & 3)) * D;
+#pragma unroll
+            for (int j = 0; j < kLoads; j++) {
+                if constexpr (kWide) {
+                    kr[t][j] = *(const uint4*)(row + j * 64 + g * 16);
+                } else {
+                    const uint2 w = *(const uint2*)(row + j * 32 + g * 8);
+                    kr[t][j].x = w.x, kr[t][j].y = w.y;
+                }
+            }
+        }
+    };
+    const bool report = lane == 0;
+    int page = page0 + wave;
+    PageIn now;
+    if (page < page1) {
+        now = page_in(c, B, s, page, head, report);
+        load_k(now);
+    }
+    while (page < page1) {
+        uint4 vr[kDim];
+        {
+            const uint8_t* base = c.v + now.at * (kPage * D) + g * 16;
+#pragma unroll
+            for (int d = 0; d < kDim; d++) vr[d] = *(const uint4*)(base + (d * 16 + col) * kPage);
+        }
+        f32x4 sc[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) sc[n][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < kLoads; j++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const f16x8 k0 = unpack8<CT>(kr[t][j].x, kr[t][j].y);
+                constexpr int W = kWide ? 2 : 1;
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+                    sc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[n][j * W], sc[n][t], 0, 0, 0);
+                if constexpr (kWide) {
+                    const f16x8 k1 = unpack8<CT>(kr[t][j].z, kr[t][j].w);
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+                        sc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q[n][2 * j + 1], sc[n][t], 0, 0, 0);
+                }
+            }
+        const int t0 = page * kPage;
+        const PageIn p = now;
+        page += 4;
+        if (page < page1) {
+            now = page_in(c, B, s, page, head, report);
+            load_k(now);
+        }
+        const bool whole = t0 >= all_lo && t0 + kPage <= all_hi;
+        f16x8 pr[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            float c1 = qs[n] * p.k_scale;
+            if (!whole) {
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int tok = t0 + g * 16 + t * 4 + r;
+                        sc[n][t][r] = tok >= lo[n] && tok < hi[n] ? sc[n][t][r] * c1 : -INFINITY;
+                    }
+                c1 = 1.0f;
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) mx = fmaxf(mx, sc[n][t][r]);
+            mx = other_half(other_row(mx, true), true) * c1;
+            float f, off, w;
+            if (rs[n].page(p.v_scale, mx, f, off, w))
+#pragma unroll
+                for (int d = 0; d < kDim; d++) o[n][d] *= f;
+            float sum = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float e = __builtin_amdgcn_exp2f(fmaf(sc[n][t][r], c1, off));
+                    sum += e;
+                    pr[n][t >> 1][(t & 1) * 4 + r] = (_Float16)e;
+                }
+            rs[n].l = fmaf(sum, w, rs[n].l);
+        }
+        if (CT == KK_KV_E4M3 && p.live < kPage) {
+#pragma unroll
+            for (int d = 0; d < kDim; d++) {
+                uint32_t* w = (uint32_t*)&vr[d];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int left = p.live - (g * 16 + 4 * i);
+                    w[i] = left >= 4 ? w[i] : left <= 0 ? 0u : w[i] & (0xffffffffu >> (32 - 8 * left));
+                }
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < kDim; d++) {
+            const f16x8 v0 = unpack8<CT>(vr[d].x, vr[d].y), v1 = unpack8<CT>(vr[d].z, vr[d].w);
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pr[n][0], o[n][d], 0, 0, 0);
+                o[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pr[n][1], o[n][d], 0, 0, 0);
+            }
+        }
+    }
+
+    // the four waves' results joined: m and l through LDS, then O in two steps
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        rs[n].l = other_half(other_row(rs[n].l, false), false);
+        if (g == 0) lds_ml[wave][n * 16 + col][0] = rs[n].m, lds_ml[wave][n * 16 + col][1] = rs[n].l;
+    }
+    __syncthreads();
+    float m[NT], l[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        m[n] = -INFINITY, l[n] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; w++) m[n] = fmaxf(m[n], lds_ml[w][n * 16 + col][0]);
+        const float ref = m[n] == -INFINITY ? 0.0f : m[n];
+#pragma unroll
+        for (int w = 0; w < 4; w++)
+            l[n] += lds_ml[w][n * 16 + col][1] * __builtin_amdgcn_exp2f(lds_ml[w][n * 16 + col][0] - ref);
+        const float f = rs[n].last() * __builtin_amdgcn_exp2f(rs[n].m - ref);
+#pragma unroll
+        for (int d = 0; d < kDim; d++) o[n][d] *= f;
+    }
+    auto put = [&](int to) {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int d = 0; d < kDim; d++) *(f32x4*)&lds_o[to][n * 16 + col][d * 16 + g * 4] = o[n][d];
+    };
+    auto add = [&](int from) {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int d = 0; d < kDim; d++) o[n][d] += *(const f32x4*)&lds_o[from][n * 16 + col][d * 16 + g * 4];
+    };
+    if (wave >= 2) put(wave - 2);
+    __syncthreads();
+    if (wave < 2) add(wave);
+    __syncthreads();
+    if (wave == 1) put(1);
+    __syncthreads();
+    if (wave != 0) return;
+    add(1);
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const int r = n * 16 + col, i = r / a.group;
+        if (i >= s.m) continue;
+        const int hq = head * a.group + r % a.group;
+        const int64_t row = s.r0 + i;
+        if (sp.parts == 1) {
+            const float inv = l[n] == 0.0f ? 0.0f : 1.0f / l[n];
+#pragma unroll
+            for (int d = 0; d < kDim; d++) {
+                float x[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) x[k] = l[n] == 0.0f ? 0.0f : o[n][d][k] * inv;
+                store_out4(a, row * a.out_row + hq * a.out_head + d * 16 + g * 4, x);
+            }
+        } else {
+            const int64_t at = (row * a.heads + hq) * a.parts + part;
+            if (g == 0) a.ml[at] = make_float2(m[n], l[n]);
+#pragma unroll
+            for (int d = 0; d < kDim; d++) *(f32x4*)(a.acc + at * D + d * 16 + g * 4) = o[n][d];
+        }
+    }
+}
+
+// ------------------------------------------------------------------ many rows: prompts
+
+// 128 rows of a (sequence, cache head), 32 a wave (v_mfma_f32_32x32x16_f16).  Bound by the matrix cores, the exponentials
+// beside them, and the unpacking, which a block does once for all its rows: a page's bytes are loaded while the page before is
+// computed, unpacked and stored to the other of two LDS buffers, K by token ([token][dim]), V by value ([dim][token]),
+// rows padded by 16 bytes (16-byte reads of 8 lanes then cover all banks).  Within 32 tokens K's rows are stored so
+// that a lane's 8 scores of one step are 8 tokens in order, as its 16 bytes of V hold them.
+template <int D, int CT>
+__global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_many_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
+    constexpr int kK = D + 8, kV = kPage + 8;  // halves of a row in LDS
+    constexpr int kBuf = kPage * kK + D * kV;
+    constexpr int kLoads = (4 * D + 255) / 256;  // 16-byte pieces of K, and of V, a thread
+    constexpr int kSteps = D / 16, kDim = D / 32;
+    __shared__ __align__(16) _Float16 lds[2 * kBuf];
+    __shared__ int found[2];
+    const int head = blockIdx.x % c.heads, rest = blockIdx.x / c.heads;
+    const int part = rest % a.parts;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, h = lane >> 5;
+    KvSeq s;
+    int tile = kv_find<256>(c, B, rest / a.parts, a.group, kManyRows, 1, blockIdx.x == 0, s, found);
+    const int64_t all_rows = tile < 0 ? 0 : (int64_t)s.m * a.group;
+    const int tiles = (int)((all_rows + kManyRows - 1) / kManyRows);
+    if (tile < 0 || tile >= tiles) return;
+    tile = tiles - 1 - tile;  // the rows that see most first
+    const int64_t r_first = (int64_t)tile * kManyRows;
+    const Span sp = span_of(s, a.causal, a.window, a.chunk, (int)(r_first / a.group), (int)min((int64_t)s.m - 1, (r_first + kManyRows - 1) / a.group));
+    if (part >= sp.parts) return;
+    const int page0 = sp.lo + part * a.chunk, page1 = min(page0 + a.chunk, sp.hi);
+
+    const int64_t r = r_first + wave * 32 + col;
+    const int i = (int)(r / a.group), hq = head * a.group + (int)(r % a.group);
+    const bool on = i < s.m;
+    f16x8 q[kSteps];
+    float qs;
+    {
+        float x[D / 2];
+#pragma unroll
+        for (int j = 0; j < D / 2; j++) x[j] = 0.0f;
+        if (on)
+#pragma unroll
+            for (int j = 0; j < kSteps; j++)
+                load_query<8>(a, (int64_t)(s.r0 + i) * a.q_row + hq * a.q_head + j * 16 + h * 8, x + 8 * j);
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < D / 2; j++) top = fmaxf(top, fabsf(x[j]));
+        top = other_half(top, true);
+        float down;
+        q_units(top, down, qs);
+        qs *= a.c;
+#pragma unroll
+        for (int j = 0; j < kSteps; j++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) q[j][k] = (_Float16)(x[8 * j + k] * down);
+    }
+    const int pos = s.len - s.m + i;
+    const int hi = on ? (a.causal ? max(0, min(s.len, pos + 1)) : s.len) : 0;
+    const int lo = a.window ? max(0, pos - a.window + 1) : 0;
+    // what the wave's first and last row see
+    const int i0 = (int)((r_first + wave * 32) / a.group), i1 = (int)min((int64_t)s.m - 1, (r_first + wave * 32 + 31) / a.group);
+    const int off = s.len - s.m;
+    const int all_lo = a.window ? off + i1 - a.window + 1 : 0, all_hi = a.causal ? min(s.len, off + i0 + 1) : s.len;
+    const int any_lo = a.window ? max(0, off + i0 - a.window + 1) : 0;
+    const int any_hi = i0 >= s.m ? 0 : a.causal ? max(0, min(s.len, off + i1 + 1)) : s.len;
+
+    f32x16 o[kDim];
+#pragma unroll
+    for (int d = 0; d < kDim; d++)
+#pragma unroll
+        for (int k = 0; k < 16; k++) o[d][k] = 0.0f;
+    RowSum rs;
+
+    uint4 kr[kLoads], vr[kLoads];
+    auto load = [&](const PageIn& p) {
+        const uint4 *kb = (const uint4*)(c.k + p.at * (kPage * D)), *vb = (const uint4*)(c.v + p.at * (kPage * D));
+#pragma unroll
+        for (int j = 0; j < kLoads; j++) {
+            const int w = tid + j * 256;
+            if (4 * D % 256 == 0 || w < 4 * D) kr[j] = kb[w], vr[j] = vb[w];
+        }
+    };
+    auto store = [&](int live, int buf) {
+        _Float16 *kb = lds + buf * kBuf, *vb = kb + kPage * kK;
+#pragma unroll
+        for (int j = 0; j < kLoads; j++) {
+            const int w = tid + j * 256;
+            if (4 * D % 256 != 0 && w >= 4 * D) continue;
+            const int tok = w / (D / 16), d = (w % (D / 16)) * 16;
+            // token 16 s + 8 h + j of 32 (j = 4 u + k) is the row that lane half h holds as score 8 s + j
+            const int row = (tok & 32) | ((tok & 16) | ((tok & 4) << 1) | ((tok & 8) >> 1) | (tok & 3));
+            *(f16x8*)(kb + row * kK + d) = unpack8<CT>(kr[j].x, kr[j].y);
+            *(f16x8*)(kb + row * kK + d + 8) = unpack8<CT>(kr[j].z, kr[j].w);
+            const int dv = w / 4, t = (w % 4) * 16;
+            if (CT == KK_KV_E4M3 && live < kPage) {
+                uint32_t* v = (uint32_t*)&vr[j];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int left = live - (t + 4 * k);
+                    v[k] = left >= 4 ? v[k] : left <= 0 ? 0u : v[k] & (0xffffffffu >> (32 - 8 * left));
+                }
+            }
+            *(f16x8*)(vb + dv * kV + t) = unpack8<CT>(vr[j].x, vr[j].y);
+            *(f16x8*)(vb + dv * kV + t + 8) = unpack8<CT>(vr[j].z, vr[j].w);
+        }
+    };
+
+    PageIn now, next;
+    if (page0 < page1) {
+        now = page_in(c, B, s, page0, head, tid == 0);
+        load(now);
+        store(now.live, 0);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int page = page0; page < page1; page++, buf ^= 1) {
+        const bool more = page + 1 < page1;
+        if (more) {
+            next = page_in(c, B, s, page + 1, head, tid == 0);
+            load(next);
+        }
+        const int t0 = page * kPage;
+        if (t0 < any_hi && t0 + kPage > any_lo) {
+            const _Float16 *kb = lds + buf * kBuf, *vb = kb + kPage * kK;
+            f32x16 sc[2];
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int k = 0; k < 16; k++) sc[t][k] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kSteps; j++)
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    const f16x8 k = *(const f16x8*)(kb + (t * 32 + col) * kK + j * 16 + h * 8);
+                    sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[j], sc[t], 0, 0, 0);
+                }
+            float c1 = qs * now.k_scale;
+            if (!(t0 >= all_lo && t0 + kPage <= all_hi)) {
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        const int tok = t0 + t * 32 + (k >> 3) * 16 + h * 8 + (k & 7);
+                        sc[t][k] = tok >= lo && tok < hi ? sc[t][k] * c1 : -INFINITY;
+                    }
+                c1 = 1.0f;
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int k = 0; k < 16; k++) mx = fmaxf(mx, sc[t][k]);
+            mx = other_half(mx, true) * c1;
+            float f, add, w;
+            if (rs.page(now.v_scale, mx, f, add, w))
+#pragma unroll
+                for (int d = 0; d < kDim; d++) o[d] *= f;
+            f16x8 pr[4];
+            float sum = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    const float e = __builtin_amdgcn_exp2f(fmaf(sc[t][k], c1, add));
+                    sum += e;
+                    pr[t * 2 + (k >> 3)][k & 7] = (_Float16)e;
+                }
+            rs.l = fmaf(sum, w, rs.l);
+#pragma unroll
+            for (int d = 0; d < kDim; d++)
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const f16x8 v = *(const f16x8*)(vb + (d * 32 + col) * kV + u * 16 + h * 8);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pr[u], o[d], 0, 0, 0);
+                }
+        }
+        if (more) {
+            store(next.live, buf ^ 1);
+            now = next;
+        }
+        __syncthreads();
+    }
+    const float l = other_half(rs.l, false), last = rs.last();
+    if (!on) return;
+    const int64_t row = s.r0 + i;
+    if (sp.parts == 1) {
+        const float inv = l == 0.0f ? 0.0f : last / l;
+#pragma unroll
+        for (int d = 0; d < kDim; d++)
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                float x[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) x[k] = l == 0.0f ? 0.0f : o[d][u * 4 + k] * inv;
+                store_out4(a, row * a.out_row + hq * a.out_head + d * 32 + u * 8 + h * 4, x);
+            }
+    } else {
+        const int64_t at = (row * a.heads + hq) * a.parts + part;
+        if (h == 0) a.ml[at] = make_float2(rs.m, l);
+#pragma unroll
+        for (int d = 0; d < kDim; d++)
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                *(f32x4*)(a.acc + at * D + d * 32 + u * 8 + h * 4) =
+                    f32x4{o[d][u * 4], o[d][u * 4 + 1], o[d][u * 4 + 2], o[d][u * 4 + 3]} * last;
+    }
+}
+
+// ------------------------------------------------------------------ the parts joined
+
+// One wave for each (row, head): out = sum_p 2^{m_p - m} O_p / sum_p 2^{m_p - m} l_p, the parts in order.
+template <int D>
+__global__ void __launch_bounds__(256) attend_join_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
+    const int lane = threadIdx.x & 63;
+    const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int row = (int)(w / a.heads), hq = (int)(w % a.heads);
+    if (row >= B.rows) return;
+    KvSeq s;
+    bool have = false;
+    for (int b0 = 0; b0 < B.n && !have; b0 += 64) {
+        KvSeq t;
+        const bool mine = b0 + lane < B.n && kv_seq(B, b0 + lane, t) && row >= t.r0 && row < t.r0 + t.m;
+        const uint64_t vote = __ballot(mine);
+        if (vote) have = kv_seq(B, b0 + __builtin_ctzll(vote), s);
+    }
+    if (!have) return;
+    const int64_t r = (int64_t)(row - s.r0) * a.group + hq % a.group, first = r / a.tile_rows * a.tile_rows;
+    const Span sp = span_of(s, a.causal, a.window, a.chunk, (int)(first / a.group), (int)min((int64_t)s.m - 1, (first + a.tile_rows - 1) / a.group));
+    if (sp.parts == 1) return;
+    const int64_t at = ((int64_t)row * a.heads + hq) * a.parts;
+    float m = -INFINITY;
+    for (int p = lane; p < sp.parts; p += 64) m = fmaxf(m, a.ml[at + p].x);
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
+    const float ref = m == -INFINITY ? 0.0f : m;
+    constexpr int N = (D + 63) / 64;
+    float x[N], l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < N; k++) x[k] = 0.0f;
+#pragma unroll 8
+    for (int p = 0; p < sp.parts; p++) {
+        const float2 ml = a.ml[at + p];
+        const float f = __builtin_amdgcn_exp2f(ml.x - ref);
+        l = fmaf(ml.y, f, l);
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            if (D % 64 == 0 || lane + 64 * k < D) x[k] = fmaf(a.acc[(at + p) * D + lane + 64 * k], f, x[k]);
+    }
+    const float inv = 1.0f / l;
+    uint16_t* out = (uint16_t*)a.out + row * a.out_row + hq * a.out_head;
+#pragma unroll
+    for (int k = 0; k < N; k++)
+        if (D % 64 == 0 || lane + 64 * k < D) {
+            const float y = l == 0.0f ? 0.0f : x[k] * inv;
+            out[lane + 64 * k] = a.type == KK_BF16 ? f32_to_bf16_bits(y) : ElemOf<KK_F16>::store(y);
+        }
+}
+
+template <int D, int CT>
+hipError_t run(const kk_kv_cache& c, const kk_kv_batch& b, const AttnPlan& p, const AttnDev& a, hipStream_t s) {
+    const KvCacheDev cd = kv_dev(c);
+    const KvBatchDev bd = kv_dev(b);
+    const dim3 grid((unsigned)(p.tiles * c.heads * p.parts)), block(256);
+    hipError_t rc;
+    if (p.few) {
+        rc = launch(p.row_tiles == 1 ? attend_few_kernel<D, CT, 1> : attend_few_kernel<D, CT, 2>, grid, block, 0, s, cd, bd, a);
+    } else {
+        rc = launch(attend_many_kernel<D, CT>, grid, block, 0, s, cd, bd, a);
+    }
+    if (rc != hipSuccess || p.parts == 1) return rc;
+    return launch(attend_join_kernel<D>, dim3((unsigned)ceil_div((int64_t)b.rows * a.heads, 4)), block, 0, s, cd, bd, a);
+}
+
+}  // namespace
+
+hipError_t launch_kv_attention(const kk_kv_cache& c, const kk_kv_batch& b, const kk_kv_attention_args& a,
+                               const AttnPlan& p, hipStream_t s) {
+    AttnDev d{};
+    d.q = a.q, d.out = a.out, d.q_row = a.q_row, d.q_head = a.q_head, d.out_row = a.out_row, d.out_head = a.out_head;
+    d.acc = (float*)a.workspace;
+    if (p.parts > 1) d.ml = (float2*)(d.acc + (int64_t)b.rows * a.heads * p.parts * c.dim);
+    d.c = a.scale * 1.44269504f;
+    d.heads = a.heads, d.group = a.heads / c.heads, d.type = a.type, d.causal = a.causal, d.window = a.window;
+    d.q_vec = (uintptr_t)a.q % 16 == 0 && a.q_row % 8 == 0 && a.q_head % 8 == 0;
+    d.out_vec = (uintptr_t)a.out % 8 == 0 && a.out_row % 4 == 0 && a.out_head % 4 == 0;
+    d.chunk = p.chunk, d.parts = p.parts, d.tile_rows = p.few ? 16 * p.row_tiles : kManyRows;
+#define KK_ATTN_CASE(D) \
+    case D: return c.type == KK_KV_INT8 ? run<D, KK_KV_INT8>(c, b, p, d, s) : run<D, KK_KV_E4M3>(c, b, p, d, s);
+    switch (c.dim) {
+        KK_ATTN_CASE(64)
+        KK_ATTN_CASE(96)
+        KK_ATTN_CASE(128)
+        KK_ATTN_CASE(192)
+        KK_ATTN_CASE(256)
+    }
+#undef KK_ATTN_CASE
+    return hipErrorInvalidValue;
+}
+
+}  // namespace kk

@@ -1,0 +1,136 @@
+// kk_kv_index.h -- which rows, pages and parts the blocks of the cache operators work on: plain index arithmetic, the
+// same functions on the host (tests/kv_index_check.hip walks every block of random batches with them) and in the kernels.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "kokoro_hip.h"
+
+namespace kk {
+
+constexpr int kPage = KK_KV_PAGE;
+constexpr int kFewRows = 32;     // rows of a (sequence, cache head) up to which attention reads the cache into registers
+constexpr int kManyRows = 128;   // rows of a block of the attention kernel for prompts
+constexpr int kMostParts = 256;  // of the token axis
+
+struct KvBatchDev {
+    const int32_t *row_start, *len, *table;
+    int64_t stride;
+    int n, rows, max_new, max_len;
+};
+inline KvBatchDev kv_dev(const kk_kv_batch& b) {
+    return {b.row_start, b.len, b.table, b.table_stride, b.n, b.rows, b.max_new, b.max_len};
+}
+
+struct KvSeq {
+    int b, r0, m, len;
+};
+
+// Sequence b of the batch; false where its rows or its length leave the bounds the launch was sized by.
+__host__ __device__ inline bool kv_seq(const KvBatchDev& B, int b, KvSeq& s) {
+    s.b = b;
+    s.r0 = B.row_start[b];
+    const int64_t m = (int64_t)B.row_start[b + 1] - s.r0;
+    s.len = B.len[b];
+    s.m = (int)m;
+    return s.r0 >= 0 && m >= 0 && m <= B.max_new && s.r0 + m <= B.rows && s.len >= 0 && s.len <= B.max_len;
+}
+
+// A sequence with m rows has at most m G / M + E tiles of M (E = 1 for tiles of its own rows, 2 for pages, where the first
+// and the last may be partial), so the tile numbers from floor(r0 G / M) + E b on are its own, without a sum over the
+// sequences before it.
+__host__ __device__ inline int64_t kv_tile_base(int64_t row, int b, int64_t G, int M, int E) { return row * G / M + (int64_t)E * b; }
+__host__ __device__ inline bool kv_tile_in(const KvSeq& s, int64_t tile, int64_t G, int M, int E, int& i) {
+    const int64_t base = kv_tile_base(s.r0, s.b, G, M, E);
+    i = (int)(tile - base);
+    return tile >= base && tile < kv_tile_base((int64_t)s.r0 + s.m, s.b + 1, G, M, E);
+}
+
+// ------------------------------------------------------------------ writing and reading back: pages
+
+// `per_seq` > 0: that many block rows for each sequence; 0: tile numbers as above.
+struct KvTiles {
+    int per_seq;
+    int64_t tiles;
+};
+inline KvTiles kv_tiles(const kk_kv_batch& b) {
+    const int64_t per = b.max_new < 2 ? 1 : (b.max_new - 2) / kPage + 2;  // pages that max_new rows can touch
+    const int64_t flat = b.rows / kPage + 2 * (int64_t)b.n;
+    // A ragged batch of few long and many short sequences would start mostly empty blocks for the longest one's pages; an even
+    // one needs no search.
+    if (per * b.n <= 2 * flat) return {(int)per, per * b.n};
+    return {0, flat};
+}
+
+// Page i of those that a sequence's rows touch: the sequence's page `at`, whose slots [lo, hi) are rows row0...
+struct KvPage {
+    int at, lo, hi;
+    int64_t row0;
+};
+__host__ __device__ inline bool kv_page_rows(const KvSeq& s, int i, KvPage& p) {
+    if (s.m == 0 || s.m > s.len) return false;
+    const int first = s.len - s.m;
+    p.at = first / kPage + i;
+    if (p.at > (s.len - 1) / kPage) return false;
+    p.lo = first > p.at * kPage ? first - p.at * kPage : 0;
+    p.hi = s.len - p.at * kPage < kPage ? s.len - p.at * kPage : kPage;
+    p.row0 = (int64_t)s.r0 + (p.at * kPage + p.lo - first);
+    return true;
+}
+
+// ------------------------------------------------------------------ attention: parts of the token axis
+
+// What the rows [first, last] (numbers in their sequence) of a block see: pages [lo, hi), in parts of `chunk` pages.
+struct Span {
+    int lo, hi, parts;
+};
+__host__ __device__ inline Span span_of(const KvSeq& s, bool causal, int window, int chunk, int first, int last) {
+    const int p0 = s.len - s.m + first, p1 = s.len - s.m + last;
+    int t_hi = s.len;
+    if (causal && p1 + 1 < t_hi) t_hi = p1 + 1 > 0 ? p1 + 1 : 0;
+    const int t_lo = window && p0 - window + 1 > 0 ? p0 - window + 1 : 0;
+    Span r;
+    r.lo = t_lo / kPage;
+    r.hi = (t_hi + kPage - 1) / kPage;
+    if (r.hi < r.lo) r.hi = r.lo;
+    r.parts = r.hi == r.lo ? 1 : (r.hi - r.lo + chunk - 1) / chunk;
+    return r;
+}
+
+// How kk_kv_attention is launched.
+struct AttnPlan {
+    bool few;         // at most kFewRows rows of a (sequence, cache head)
+    int row_tiles;    // few: 16-row tiles of a block (1 or 2)
+    int64_t tiles;    // blocks along the rows
+    int chunk, parts; // pages of a part, parts of the axis
+    int64_t ws_bytes; // partial results, 0 for one part
+};
+inline AttnPlan attention_plan(const kk_kv_cache& c, const kk_kv_batch& b, const kk_kv_attention_args& a, int n_cu) {
+    AttnPlan p{};
+    const int64_t group = a.heads / c.heads, rows = b.max_new * group;
+    p.few = rows <= kFewRows;
+    p.row_tiles = rows <= 16 ? 1 : 2;
+    p.tiles = p.few ? b.n : b.rows * group / kManyRows + b.n;
+    int64_t pages = ((int64_t)b.max_len + kPage - 1) / kPage;
+    if (a.window) {  // a block's rows stand at most that many tokens apart, and N tokens touch at most N / 64 + 2 pages
+        const int64_t seen = (int64_t)a.window + (p.few ? b.max_new : kManyRows / group + 1);
+        pages = std::min(pages, seen / kPage + 2);
+    }
+    pages = std::max<int64_t>(pages, 1);
+    const int64_t blocks = p.tiles * c.heads;
+    int64_t chunk = pages;
+    if (p.few)
+        chunk = std::min<int64_t>(std::max<int64_t>(pages * blocks / (4 * n_cu), 8), 16);
+    else if (blocks < 2 * n_cu)
+        chunk = std::max<int64_t>(pages * blocks / (2 * n_cu), 8);
+    chunk = std::max(chunk, (pages + kMostParts - 1) / kMostParts);
+    p.parts = (int)((pages + chunk - 1) / chunk);
+    p.chunk = (int)((pages + p.parts - 1) / p.parts);
+    p.parts = (int)((pages + p.chunk - 1) / p.chunk);
+    if (p.parts > 1) p.ws_bytes = (int64_t)b.rows * a.heads * p.parts * (c.dim * (int64_t)sizeof(float) + 2 * (int64_t)sizeof(float));
+    return p;
+}
+
+}  // namespace kk

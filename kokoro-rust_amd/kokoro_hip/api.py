@@ -28,8 +28,11 @@ EXPORTS = [
     "kk_plan_item_samples", "kk_plan_fetch_pcm16_async", "kk_plan_fetch_wait", "kk_snake_block_noalloc", "kk_profile_launches", "kk_checkpoint_open", "kk_checkpoint_count",
     "kk_checkpoint_entry", "kk_checkpoint_free", "kk_upload_checkpoint", "kk_weight_norm", "kk_voice_load",
     "kk_voice_free", "kk_voice_ref_s", "kk_forward_batch", "kk_result_free", "kk_plan_create_full",
-    "kk_plan_durations",
+    "kk_plan_durations", "kk_qk_norm_rope", "kk_kv_write", "kk_kv_read", "kk_kv_attention", "kk_kv_attention_workspace",
 ]
+BF16, F16, F32 = 1, 2, 3
+KV_PAGE, KV_INT8, KV_E4M3 = 64, 1, 2
+KV_BAD_BATCH, KV_BAD_PAGE = 1, 2
 NOALLOC_MAX_ROWS = 65536
 NOALLOC_MAX_ITEMS = 64
 
@@ -76,6 +79,42 @@ class PlanInfo(C.Structure):
     _fields_ = [("n_items", C.c_int64), ("ln", C.c_int64), ("frames", C.c_int64), ("samples", C.c_int64),
                 ("conv_flop", C.c_double), ("snake_flop", C.c_double), ("device_bytes", C.c_int64),
                 ("launches", C.c_int64)]
+
+
+class NormRope(C.Structure):
+    """kk_norm_rope: device pointers as integers."""
+    _fields_ = [("type", C.c_int32), ("dim", C.c_int32), ("rows", C.c_int32), ("q_heads", C.c_int32), ("k_heads", C.c_int32),
+                ("q", C.c_void_p), ("q_row", C.c_int64), ("q_head", C.c_int64), ("k", C.c_void_p), ("k_row", C.c_int64),
+                ("k_head", C.c_int64), ("q_out", C.c_void_p), ("q_out_row", C.c_int64), ("q_out_head", C.c_int64),
+                ("k_out", C.c_void_p), ("k_out_row", C.c_int64), ("k_out_head", C.c_int64), ("norm", C.c_int32),
+                ("eps", C.c_float), ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("pos", C.c_void_p),
+                ("rot", C.c_int32), ("interleaved", C.c_int32), ("theta", C.c_double), ("freq", C.c_void_p)]
+
+
+class KvCache(C.Structure):
+    """kk_kv_cache: pages of 64 tokens in 8 bits, device pointers as integers."""
+    _fields_ = [("type", C.c_int32), ("heads", C.c_int32), ("dim", C.c_int32), ("pages", C.c_int32), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("fault", C.c_void_p)]
+
+
+class KvBatch(C.Structure):
+    """kk_kv_batch: a ragged batch of sequences over a cache."""
+    _fields_ = [("n", C.c_int32), ("rows", C.c_int32), ("max_new", C.c_int32), ("max_len", C.c_int32),
+                ("row_start", C.c_void_p), ("len", C.c_void_p), ("table", C.c_void_p), ("table_width", C.c_int32),
+                ("table_stride", C.c_int64)]
+
+
+class KvRows(C.Structure):
+    """kk_kv_rows: keys and values of a batch's rows."""
+    _fields_ = [("type", C.c_int32), ("k", C.c_void_p), ("k_row", C.c_int64), ("k_head", C.c_int64), ("v", C.c_void_p),
+                ("v_row", C.c_int64), ("v_head", C.c_int64)]
+
+
+class KvAttention(C.Structure):
+    """kk_kv_attention_args."""
+    _fields_ = [("type", C.c_int32), ("heads", C.c_int32), ("q", C.c_void_p), ("q_row", C.c_int64), ("q_head", C.c_int64),
+                ("out", C.c_void_p), ("out_row", C.c_int64), ("out_head", C.c_int64), ("scale", C.c_float),
+                ("causal", C.c_int32), ("window", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
 class LaunchRecord(C.Structure):
@@ -154,6 +193,12 @@ def lib():
         L.kk_layout_frames.restype = i64
         L.kk_layout_col_item.argtypes = [i64, vp, vp, i32, vp]
         L.kk_layout_src_row.argtypes = [C.POINTER(vp), vp, i32, vp, vp, i64, vp]
+        L.kk_qk_norm_rope.argtypes = [vp, C.POINTER(NormRope), vp, cp, sz]
+        L.kk_kv_write.argtypes = [vp, C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(KvRows), vp, cp, sz]
+        L.kk_kv_read.argtypes = L.kk_kv_write.argtypes
+        L.kk_kv_attention.argtypes = [vp, C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(KvAttention), vp, cp, sz]
+        L.kk_kv_attention_workspace.argtypes = [vp, C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(KvAttention), cp, sz]
+        L.kk_kv_attention_workspace.restype = i64
         _lib = L
     return _lib
 
@@ -397,6 +442,37 @@ class Context:
         err = _err()
         _check(lib().kk_snake_block_noalloc(self.h, prefix.encode(), C.c_void_p(x_ptr), int(rows), _p(starts),
                                             _p(lens), len(lens), rp, err, len(err)), err)
+
+    # -------------------------------------------------------------- operators over an 8-bit cache
+    # Device memory in and out, by pointer, on the caller's stream (an integer hipStream_t; 0 is the null stream); the
+    # structs can be kept and used again.  A call returns once its kernels are enqueued.
+    def qk_norm_rope(self, args, stream=0):
+        """kk_qk_norm_rope of a NormRope."""
+        err = _err()
+        _check(lib().kk_qk_norm_rope(self.h, C.byref(args), stream, err, len(err)), err)
+
+    def kv_write(self, cache, batch, rows, stream=0):
+        """kk_kv_write: the KvRows into the KvCache as the last tokens of the KvBatch's sequences."""
+        err = _err()
+        _check(lib().kk_kv_write(self.h, C.byref(cache), C.byref(batch), C.byref(rows), stream, err, len(err)), err)
+
+    def kv_read(self, cache, batch, rows, stream=0):
+        """kk_kv_read: those tokens back into the KvRows."""
+        err = _err()
+        _check(lib().kk_kv_read(self.h, C.byref(cache), C.byref(batch), C.byref(rows), stream, err, len(err)), err)
+
+    def kv_attention(self, cache, batch, args, stream=0):
+        """kk_kv_attention of a KvAttention, whose workspace holds kv_attention_workspace bytes."""
+        err = _err()
+        _check(lib().kk_kv_attention(self.h, C.byref(cache), C.byref(batch), C.byref(args), stream, err, len(err)), err)
+
+    def kv_attention_workspace(self, cache, batch, args):
+        """kk_kv_attention_workspace: bytes (0: none needed)."""
+        err = _err()
+        n = lib().kk_kv_attention_workspace(self.h, C.byref(cache), C.byref(batch), C.byref(args), err, len(err))
+        if n < 0:
+            raise KKError(int(n), err.value.decode(errors="replace"))
+        return n
 
     def prepare(self, items):
         """The items marshalled once into the ABI's structs, for repeated calls (timing)."""
