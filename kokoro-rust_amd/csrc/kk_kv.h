@@ -114,7 +114,7 @@ template <>
 struct ElemOf<KK_BF16> {
     typedef uint16_t type;
     static __device__ __forceinline__ float load(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
-    static __device__ __forceinline__ uint16_t store(float f) { return f32_to_bf16_bits(f); }
+    static __device__ __forceinline__ uint16_t store(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
 };
 template <>
 struct ElemOf<KK_F16> {

@@ -67,7 +67,7 @@ __device__ __forceinline__ void load_query(const AttnDev& a, int64_t at, float* 
 __device__ __forceinline__ void store_out4(const AttnDev& a, int64_t at, const float* x) {
     uint16_t e[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) e[i] = a.type == KK_BF16 ? f32_to_bf16_bits(x[i]) : ElemOf<KK_F16>::store(x[i]);
+    for (int i = 0; i < 4; i++) e[i] = a.type == KK_BF16 ? ElemOf<KK_BF16>::store(x[i]) : ElemOf<KK_F16>::store(x[i]);
     uint16_t* p = (uint16_t*)a.out + at;
     if (a.out_vec) {
         uint2 w;
@@ -638,7 +638,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(KvCacheDev c, KvBatchD
     for (int k = 0; k < N; k++)
         if (D % 64 == 0 || lane + 64 * k < D) {
             const float y = l == 0.0f ? 0.0f : x[k] * inv;
-            out[lane + 64 * k] = a.type == KK_BF16 ? f32_to_bf16_bits(y) : ElemOf<KK_F16>::store(y);
+            out[lane + 64 * k] = a.type == KK_BF16 ? ElemOf<KK_BF16>::store(y) : ElemOf<KK_F16>::store(y);
         }
 }
 

@@ -4,16 +4,20 @@
 //
 // Bound by memory: every value is read and written once (2 x 2 bytes a value in 16 bits).  A head is held by
 // L = 2^j lanes; each holds both sides of its pairs (neox: V values at c V and V at rot / 2 + c V), so the rotation
-// exchanges nothing between lanes and only the sum of squares is a reduction.  The lanes of a wave hold 64 / L heads
-// of one row at once (8 for heads of 128 values in 16 bits) and walk over units (row, 64 / L heads) in order, so a
-// row's sines are computed once for its heads.  Angles: pos * f_i / 2 pi in f64, its fraction to f32 and sincospi
-// there, which keeps 2^-24 of a turn at any position; a lane's f_i are one f64 exp2 and products, once per wave.
+// exchanges nothing between lanes and only the sum of squares is a reduction.  A unit is 64 / L heads of a row (8 heads of
+// 128 values in 16 bits); a wave works through a row's units, or some of them where there are few rows, and loads kAhead units
+// before it works on the first, which hides the loads' latency without many waves.  The row's angles are computed once: lane i
+// takes pair i, pos * f_i / 2 pi in f64, its fraction to f32 and sincospi there (2^-24 of a turn at any position), and
+// the wave's lanes read theirs from LDS.
+#include <algorithm>
 #include <cmath>
 
 #include "kk_kv.h"
 
 namespace kk {
 namespace {
+
+constexpr int kMostPairs = 256;  // of a head: dim <= 512
 
 struct NormRopeDev {
     const void *q, *k;
@@ -22,107 +26,146 @@ struct NormRopeDev {
     const float *q_weight, *k_weight;
     const int32_t* pos;
     const double* freq;
-    double log2_step, step;  // log2(f_1 / f_0) and f_1 / f_0 without a table
+    double log2_step;  // log2(f_1 / f_0) without a table
     float eps;
     int rows, dim, q_heads, heads, rot, norm;
-    int lanes, log2_lanes;   // of a head
-    int groups;              // units of a row
-    int64_t units, per_wave;
+    int lanes, log2_lanes;  // of a head
+    int units, split;       // of a row: units, and waves that share them
+    int waves;
 };
 
-// V values a chunk (16 bytes, or 1), K chunk pairs a lane.
-template <int T, int V, int K, bool INTER>
+template <int T, int V>
+struct Chunk {  // V values next to each other as they lie in memory
+    typename ElemOf<T>::type e[V];
+    __device__ __forceinline__ void load(const typename ElemOf<T>::type* p) {
+        if constexpr (V > 1) {
+            const uint4 q = *(const uint4*)p;
+            __builtin_memcpy(e, &q, 16);
+        } else {
+            e[0] = *p;
+        }
+    }
+};
+
+// V values a chunk (16 bytes, or 1), K chunk pairs a lane, kAhead units in flight.
+template <int T, int V, int K, int kAhead, bool INTER>
 __global__ void __launch_bounds__(256) norm_rope_kernel(NormRopeDev a) {
     typedef typename ElemOf<T>::type E;
-    const int lane = threadIdx.x & 63;
-    const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int64_t u0 = wave * a.per_wave, u1 = u0 + a.per_wave < a.units ? u0 + a.per_wave : a.units;
-    const int sub = lane & (a.lanes - 1), in_wave = lane >> a.log2_lanes, wide = 64 >> a.log2_lanes;
+    __shared__ __align__(16) float lds[4][2][kMostPairs];
+    __shared__ __align__(16) float weight[2][2 * kMostPairs];
+    const int lane = threadIdx.x & 63, in_block = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = blockIdx.x * 4 + in_block;
+    if (a.norm) {
+        for (int i = threadIdx.x; i < a.dim; i += 256) {
+            weight[0][i] = a.q_weight ? a.q_weight[i] : 1.0f;
+            weight[1][i] = a.k_weight ? a.k_weight[i] : 1.0f;
+        }
+        __syncthreads();
+    }
+    if (wave >= a.waves) return;
+    float *cos_at = lds[in_block][0], *sin_at = lds[in_block][1];
+    const int sub = lane & (a.lanes - 1), slot = lane >> a.log2_lanes, wide = 64 >> a.log2_lanes;
     const int turning = a.rot / (2 * V), pairs = a.dim / (2 * V);  // chunk pairs of a head
     int at[K][2];                                                  // a chunk pair's two places in the head
-    double f[K][V];                                                // turns a position of its pairs
+    bool mine[K];
 #pragma unroll
     for (int j = 0; j < K; j++) {
-        const int c = sub + j * a.lanes;
-        if (INTER || c >= turning)  // behind `rot` a pair is 2 V values next to each other
+        mine[j] = sub + j * a.lanes < pairs;
+        const int c = mine[j] ? sub + j * a.lanes : pairs - 1;  // lanes without one load the last
+        if (INTER || c >= turning)                             // behind `rot` a pair is 2 V values next to each other
             at[j][0] = 2 * V * c, at[j][1] = at[j][0] + V;
         else
             at[j][0] = V * c, at[j][1] = a.rot / 2 + V * c;
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-            if (c >= turning)
-                f[j][i] = 0.0;
-            else if (a.freq)
-                f[j][i] = a.freq[c * V + i] * (0.5 / M_PI);
-            else
-                f[j][i] = i ? f[j][i - 1] * a.step : exp2(a.log2_step * (double)(c * V)) * (0.5 / M_PI);
-        }
     }
-    int64_t row_now = -1;
-    float cs[K][V], sn[K][V];
-    for (int64_t u = u0; u < u1; u++) {
-        const int64_t row = u / a.groups;
-        const int h = (int)(u - row * a.groups) * wide + in_wave;
-        const bool live = h < a.heads, is_q = h < a.q_heads;
-        const int hh = is_q ? h : h - a.q_heads;
-        const E* x = (const E*)(is_q ? a.q : a.k) + row * (is_q ? a.q_row : a.k_row) + hh * (is_q ? a.q_head : a.k_head);
-        float v[K][2 * V];
-        float sum = 0.0f;
+    const int step = a.waves / a.split, part = wave % a.split;
+    const int u0 = a.units * part / a.split, u1 = a.units * (part + 1) / a.split;
+    double f[kMostPairs / 64];  // turns a position of the pairs whose angles this lane computes
+    bool first = true;
+    for (int row = wave / a.split; row < a.rows; row += step) {
+        const double pos = (double)a.pos[row];
+        float cs[K][V], sn[K][V];
+        for (int ub = u0; ub < u1; ub += kAhead) {
+            Chunk<T, V> raw[kAhead][K][2];
 #pragma unroll
-        for (int j = 0; j < K; j++) {
-            const bool on = live && sub + j * a.lanes < pairs;
+            for (int n = 0; n < kAhead; n++) {
+                const int h = min(min(ub + n, u1 - 1) * wide + slot, a.heads - 1);
+                const bool is_q = h < a.q_heads;
+                const E* x = is_q ? (const E*)a.q + row * a.q_row + h * a.q_head
+                                  : (const E*)a.k + row * a.k_row + (h - a.q_heads) * a.k_head;
 #pragma unroll
-            for (int i = 0; i < 2 * V; i++) v[j][i] = 0.0f;
-            if (on) {
-                load_values<T, V>(x, at[j][0], V > 1, v[j]);
-                load_values<T, V>(x, at[j][1], V > 1, v[j] + V);
+                for (int j = 0; j < K; j++) raw[n][j][0].load(x + at[j][0]), raw[n][j][1].load(x + at[j][1]);
             }
-        }
-        if (row != row_now) {
-            row_now = row;
-            const double pos = (double)a.pos[row];
+            if (first) {  // behind the first loads
+                first = false;
 #pragma unroll
-            for (int j = 0; j < K; j++)
-#pragma unroll
-                for (int i = 0; i < V; i++) {
-                    double t = pos * f[j][i];
-                    t -= rint(t);
-                    sincospif(2.0f * (float)t, &sn[j][i], &cs[j][i]);
+                for (int j = 0; j < kMostPairs / 64; j++) {
+                    const int i = lane + 64 * j;
+                    if (64 * j < a.rot / 2) f[j] = (a.freq ? a.freq[min(i, a.rot / 2 - 1)] : exp2(a.log2_step * (double)i)) * (0.5 / M_PI);
                 }
-        }
-        if (a.norm) {
-#pragma unroll
-            for (int j = 0; j < K; j++)
-#pragma unroll
-                for (int i = 0; i < 2 * V; i++) sum = fmaf(v[j][i], v[j][i], sum);
-            for (int m = 1; m < a.lanes; m <<= 1) sum += __shfl_xor(sum, m);
-            const float r = 1.0f / sqrtf(sum / (float)a.dim + a.eps);
-            const float* w = is_q ? a.q_weight : a.k_weight;
-#pragma unroll
-            for (int j = 0; j < K; j++) {
-                const bool on = w && live && sub + j * a.lanes < pairs;
-#pragma unroll
-                for (int i = 0; i < 2 * V; i++)
-                    v[j][i] *= on ? r * w[at[j][i / V] + i % V] : r;
             }
-        }
-        E* y = (E*)(is_q ? a.q_out : a.k_out) + row * (is_q ? a.q_out_row : a.k_out_row) +
-               hh * (is_q ? a.q_out_head : a.k_out_head);
+            if (ub == u0) {
 #pragma unroll
-        for (int j = 0; j < K; j++) {
-            if (!(live && sub + j * a.lanes < pairs)) continue;
-            float o[2 * V];
+                for (int j = 0; j < kMostPairs / 64; j++) {
+                    if (64 * j >= a.rot / 2) break;
+                    double t = pos * f[j];
+                    t -= rint(t);
+                    float s, c;
+                    sincospif(2.0f * (float)t, &s, &c);
+                    cos_at[lane + 64 * j] = c, sin_at[lane + 64 * j] = s;
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                const int p = INTER && V > 1 ? 2 * i : i, q = INTER && V > 1 ? 2 * i + 1 : V + i;
-                o[p] = v[j][p] * cs[j][i] - v[j][q] * sn[j][i];
-                o[q] = v[j][q] * cs[j][i] + v[j][p] * sn[j][i];
+                for (int j = 0; j < K; j++) {
+                    const int c = min(sub + j * a.lanes, kMostPairs / V - 1);
+#pragma unroll
+                    for (int i = 0; i < V; i++) cs[j][i] = cos_at[c * V + i], sn[j][i] = sin_at[c * V + i];
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
             }
-            if (sub + j * a.lanes >= turning)  // sine 0 and cosine 1, but for infinities
 #pragma unroll
-                for (int i = 0; i < 2 * V; i++) o[i] = v[j][i];
-            store_values<T, V>(y, at[j][0], V > 1, o);
-            store_values<T, V>(y, at[j][1], V > 1, o + V);
+            for (int n = 0; n < kAhead; n++) {
+                if (ub + n >= u1) break;
+                const int h = (ub + n) * wide + slot;
+                const bool is_q = h < a.q_heads, live = h < a.heads;
+                float v[K][2 * V];
+                float sum = 0.0f;
+#pragma unroll
+                for (int j = 0; j < K; j++)
+#pragma unroll
+                    for (int i = 0; i < 2 * V; i++) {
+                        v[j][i] = ElemOf<T>::load(raw[n][j][i / V].e[i % V]);
+                        sum = fmaf(v[j][i], mine[j] ? v[j][i] : 0.0f, sum);
+                    }
+                if (a.norm) {
+                    for (int m = 1; m < a.lanes; m <<= 1) sum += __shfl_xor(sum, m);
+                    const float r = 1.0f / sqrtf(sum / (float)a.dim + a.eps);
+                    const float* w = weight[is_q ? 0 : 1];
+#pragma unroll
+                    for (int j = 0; j < K; j++)
+#pragma unroll
+                        for (int i = 0; i < 2 * V; i++) v[j][i] *= r * w[at[j][i / V] + i % V];
+                }
+                E* y = is_q ? (E*)a.q_out + row * a.q_out_row + h * a.q_out_head
+                            : (E*)a.k_out + row * a.k_out_row + (h - a.q_heads) * a.k_out_head;
+#pragma unroll
+                for (int j = 0; j < K; j++) {
+                    if (!(live && mine[j])) continue;
+                    float* x = v[j];
+                    if (sub + j * a.lanes < turning) {
+#pragma unroll
+                        for (int i = 0; i < V; i++) {
+                            const int p = INTER && V > 1 ? 2 * i : i, q = INTER && V > 1 ? 2 * i + 1 : V + i;
+                            const float xp = x[p], xq = x[q];
+                            x[p] = xp * cs[j][i] - xq * sn[j][i];
+                            x[q] = xq * cs[j][i] + xp * sn[j][i];
+                        }
+                    }
+                    store_values<T, V>(y, at[j][0], V > 1, x);
+                    store_values<T, V>(y, at[j][1], V > 1, x + V);
+                }
+            }
         }
     }
 }
@@ -132,14 +175,15 @@ hipError_t run(NormRopeDev d, bool wide, bool inter, int n_cu, hipStream_t s) {
     constexpr int V = T == KK_F32 ? 4 : 8;
     const int pairs = d.dim / (wide ? 2 * V : 2);
     while (d.lanes < 64 && d.lanes < pairs) d.lanes *= 2, d.log2_lanes++;
-    d.groups = (int)ceil_div(d.heads, 64 / d.lanes);
-    d.units = (int64_t)d.rows * d.groups;
-    // enough waves for every slot (32 a CU), each over several units once there are more
-    d.per_wave = ceil_div(d.units, (int64_t)n_cu * 32);
-    const dim3 grid((unsigned)ceil_div(ceil_div(d.units, d.per_wave), 4)), block(256);
-    // heads have at most 512 values: 64 lanes hold one with 8 or 4 values a chunk, or 4 pairs a lane
-    if (wide) return launch(inter ? norm_rope_kernel<T, V, 1, true> : norm_rope_kernel<T, V, 1, false>, grid, block, 0, s, d);
-    return launch(inter ? norm_rope_kernel<T, 1, 4, true> : norm_rope_kernel<T, 1, 4, false>, grid, block, 0, s, d);
+    d.units = (int)ceil_div(d.heads, 64 / d.lanes);
+    // 16 waves a CU, which with kAhead units each cover the memory's latency; rows that are fewer are shared
+    const int64_t most = (int64_t)n_cu * 16;
+    d.split = (int)std::min<int64_t>(d.units, std::max<int64_t>(1, most / d.rows));
+    d.waves = (int)(std::min<int64_t>(d.rows, most / d.split) * d.split);
+    const dim3 grid((unsigned)ceil_div(d.waves, 4)), block(256);
+    // heads have at most 512 values: 64 lanes hold one with 8 or 4 values a chunk, or with 4 pairs a lane
+    if (wide) return launch(inter ? norm_rope_kernel<T, V, 1, 4, true> : norm_rope_kernel<T, V, 1, 4, false>, grid, block, 0, s, d);
+    return launch(inter ? norm_rope_kernel<T, 1, 4, 2, true> : norm_rope_kernel<T, 1, 4, 2, false>, grid, block, 0, s, d);
 }
 
 }  // namespace
@@ -152,10 +196,7 @@ hipError_t launch_norm_rope(const kk_norm_rope& a, int n_cu, hipStream_t s) {
     d.q_weight = a.q_weight, d.k_weight = a.k_weight, d.pos = a.pos, d.freq = a.freq;
     d.eps = a.eps, d.rows = a.rows, d.dim = a.dim, d.q_heads = a.q_heads, d.heads = a.q_heads + a.k_heads;
     d.rot = a.rot, d.norm = a.norm, d.lanes = 1, d.log2_lanes = 0;
-    if (a.rot && !a.freq) {
-        d.log2_step = -2.0 / a.rot * std::log2(a.theta);
-        d.step = std::exp2(d.log2_step);
-    }
+    if (a.rot && !a.freq) d.log2_step = -2.0 / a.rot * std::log2(a.theta);
     const int e = a.type == KK_F32 ? 4 : 2, V = 16 / e;
     auto whole = [&](int heads, const void* p, int64_t row, int64_t head) {
         return heads == 0 || ((uintptr_t)p % 16 == 0 && row * e % 16 == 0 && head * e % 16 == 0);
