@@ -129,6 +129,18 @@ struct ElemOf<KK_F32> {
     static __device__ __forceinline__ float store(float f) { return f; }
 };
 
+// A load of data that is read once: it does not displace what the caches hold for others.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint4 stream_load(const uint4* p) {
+    const u32x4 v = __builtin_nontemporal_load((const u32x4*)p);
+    return uint4{v[0], v[1], v[2], v[3]};
+}
+__device__ __forceinline__ uint2 stream_load(const uint2* p) {
+    const u32x2 v = __builtin_nontemporal_load((const u32x2*)p);
+    return uint2{v[0], v[1]};
+}
+
 // N values next to each other, as 16-byte accesses where `vec` says that they lie on such a boundary.
 template <int T, int N>
 __device__ __forceinline__ void load_values(const void* base, int64_t at, bool vec, float* x) {

@@ -129,19 +129,21 @@ struct RowSum {
 
 // ------------------------------------------------------------------ few rows: single tokens, drafts
 
-// At most 16 NT rows of a (sequence, cache head).  Bound by reading the cache once.  Each of a block's four waves takes every
-// fourth page of the part straight into registers, in 16-byte loads that are the MFMA operands (v_mfma_f32_16x16x32_f16)
+// At most 16 NT rows of a (sequence, cache head).  Bound by reading the cache once.  Each of a block's W waves takes every
+// W-th page of the part straight into registers, in 16-byte loads that are the MFMA operands (v_mfma_f32_16x16x32_f16)
 // once unpacked; nothing of the cache goes through LDS.  Row i of K's token tile t is token 16 (i / 4) + 4 t + i % 4: then
 // lane group g's scores are those of tokens 16 g .. 16 g + 15 in order, the 16 bytes that it loads of each row of V.
-// K of the next page is loaded while this one's softmax and second product run, V while its first product runs.
-template <int D, int CT, int NT>
-__global__ void __launch_bounds__(256, D <= 192 && D * NT <= 256 ? 2 : 1) attend_few_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
+// K of the next page is loaded while this one's softmax and second product run, V while its first product runs.  The waves
+// leave their O, m and l in LDS, and after one barrier the block's threads join them.
+template <int D, int CT, int NT, int W>
+__global__ void __launch_bounds__(64 * W, D <= 192 && D * NT <= 256 ? 2 : 1)
+attend_few_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
     constexpr bool kWide = D % 64 == 0;            // 16 bytes of a K row a lane, else 8
     constexpr int kLoads = kWide ? D / 64 : D / 32;  // of each token tile
     constexpr int kSteps = D / 32, kDim = D / 16;
     constexpr int kLd = D + 4;
-    __shared__ float lds_ml[4][NT * 16][2];
-    __shared__ float lds_o[2][NT * 16][kLd];
+    __shared__ float lds_ml[W][NT * 16][2];
+    __shared__ __align__(16) float lds_o[W][NT * 16][kLd];
     const int head = blockIdx.x % c.heads, rest = blockIdx.x / c.heads;
     const int part = rest % a.parts, b = rest / a.parts;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -155,6 +157,31 @@ __global__ void __launch_bounds__(256, D <= 192 && D * NT <= 256 ? 2 : 1) attend
     const Span sp = span_of(s, a.causal, a.window, a.chunk, 0, s.m - 1);
     if (part >= sp.parts) return;
     const int page0 = sp.lo + part * a.chunk, page1 = min(page0 + a.chunk, sp.hi);
+
+    uint4 kr[4][kLoads];
+    auto load_k = [&](const PageIn& p) {
+        const uint8_t* base = c.k + p.at * (kPage * D);
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const uint8_t* row = base + ((col >> 2) * 16 + t * 4 + (col & 3)) * D;
+#pragma unroll
+            for (int j = 0; j < kLoads; j++) {
+                if constexpr (kWide) {
+                    kr[t][j] = stream_load((const uint4*)(row + j * 64 + g * 16));
+                } else {
+                    const uint2 w = stream_load((const uint2*)(row + j * 32 + g * 8));
+                    kr[t][j].x = w.x, kr[t][j].y = w.y;
+                }
+            }
+        }
+    };
+    const bool report = lane == 0;
+    int page = page0 + wave;
+    PageIn now;
+    if (page < page1) {
+        now = page_in(c, B, s, page, head, report);
+        load_k(now);
+    }
 
     // the rows of this lane's columns: queries and the tokens [lo, hi) that they see
     f16x8 q[NT][kSteps];
@@ -203,36 +230,12 @@ __global__ void __launch_bounds__(256, D <= 192 && D * NT <= 256 ? 2 : 1) attend
         for (int d = 0; d < kDim; d++) o[n][d] = f32x4{0, 0, 0, 0};
     }
 
-    uint4 kr[4][kLoads];
-    auto load_k = [&](const PageIn& p) {
-        const uint8_t* base = c.k + p.at * (kPage * D);
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const uint8_t* row = base + ((col >> 2) * 16 + t * 4 + (col & 3)) * D;
-#pragma unroll
-            for (int j = 0; j < kLoads; j++) {
-                if constexpr (kWide) {
-                    kr[t][j] = *(const uint4*)(row + j * 64 + g * 16);
-                } else {
-                    const uint2 w = *(const uint2*)(row + j * 32 + g * 8);
-                    kr[t][j].x = w.x, kr[t][j].y = w.y;
-                }
-            }
-        }
-    };
-    const bool report = lane == 0;
-    int page = page0 + wave;
-    PageIn now;
-    if (page < page1) {
-        now = page_in(c, B, s, page, head, report);
-        load_k(now);
-    }
     while (page < page1) {
         uint4 vr[kDim];
         {
             const uint8_t* base = c.v + now.at * (kPage * D) + g * 16;
 #pragma unroll
-            for (int d = 0; d < kDim; d++) vr[d] = *(const uint4*)(base + (d * 16 + col) * kPage);
+            for (int d = 0; d < kDim; d++) vr[d] = stream_load((const uint4*)(base + (d * 16 + col) * kPage));
         }
         f32x4 sc[NT][4];
 #pragma unroll
@@ -244,10 +247,10 @@ __global__ void __launch_bounds__(256, D <= 192 && D * NT <= 256 ? 2 : 1) attend
 #pragma unroll
             for (int t = 0; t < 4; t++) {
                 const f16x8 k0 = unpack8<CT>(kr[t][j].x, kr[t][j].y);
-                constexpr int W = kWide ? 2 : 1;
+                constexpr int kStep = kWide ? 2 : 1;
 #pragma unroll
                 for (int n = 0; n < NT; n++)
-                    sc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[n][j * W], sc[n][t], 0, 0, 0);
+                    sc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[n][j * kStep], sc[n][t], 0, 0, 0);
                 if constexpr (kWide) {
                     const f16x8 k1 = unpack8<CT>(kr[t][j].z, kr[t][j].w);
 #pragma unroll
@@ -257,7 +260,7 @@ __global__ void __launch_bounds__(256, D <= 192 && D * NT <= 256 ? 2 : 1) attend
             }
         const int t0 = page * kPage;
         const PageIn p = now;
-        page += 4;
+        page += W;
         if (page < page1) {
             now = page_in(c, B, s, page, head, report);
             load_k(now);
@@ -320,67 +323,42 @@ __global__ void __launch_bounds__(256, D <= 192 && D * NT <= 256 ? 2 : 1) attend
         }
     }
 
-    // the four waves' results joined: m and l through LDS, then O in two steps
+    const int rows = s.m * a.group;
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-        rs[n].l = other_half(other_row(rs[n].l, false), false);
-        if (g == 0) lds_ml[wave][n * 16 + col][0] = rs[n].m, lds_ml[wave][n * 16 + col][1] = rs[n].l;
+        const int r = n * 16 + col;
+        const float l = other_half(other_row(rs[n].l, false), false), f = rs[n].last();
+        if (r >= rows) continue;
+        if (g == 0) lds_ml[wave][r][0] = rs[n].m, lds_ml[wave][r][1] = l;
+#pragma unroll
+        for (int d = 0; d < kDim; d++) *(f32x4*)&lds_o[wave][r][d * 16 + g * 4] = o[n][d] * f;
     }
     __syncthreads();
-    float m[NT], l[NT];
+    for (int t = threadIdx.x; t < rows * (D / 4); t += 64 * W) {
+        const int r = t / (D / 4), d = t % (D / 4) * 4;
+        float m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        m[n] = -INFINITY, l[n] = 0.0f;
+        for (int w = 0; w < W; w++) m = fmaxf(m, lds_ml[w][r][0]);
+        const float ref = m == -INFINITY ? 0.0f : m;
+        f32x4 x = {0, 0, 0, 0};
 #pragma unroll
-        for (int w = 0; w < 4; w++) m[n] = fmaxf(m[n], lds_ml[w][n * 16 + col][0]);
-        const float ref = m[n] == -INFINITY ? 0.0f : m[n];
-#pragma unroll
-        for (int w = 0; w < 4; w++)
-            l[n] += lds_ml[w][n * 16 + col][1] * __builtin_amdgcn_exp2f(lds_ml[w][n * 16 + col][0] - ref);
-        const float f = rs[n].last() * __builtin_amdgcn_exp2f(rs[n].m - ref);
-#pragma unroll
-        for (int d = 0; d < kDim; d++) o[n][d] *= f;
-    }
-    auto put = [&](int to) {
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int d = 0; d < kDim; d++) *(f32x4*)&lds_o[to][n * 16 + col][d * 16 + g * 4] = o[n][d];
-    };
-    auto add = [&](int from) {
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int d = 0; d < kDim; d++) o[n][d] += *(const f32x4*)&lds_o[from][n * 16 + col][d * 16 + g * 4];
-    };
-    if (wave >= 2) put(wave - 2);
-    __syncthreads();
-    if (wave < 2) add(wave);
-    __syncthreads();
-    if (wave == 1) put(1);
-    __syncthreads();
-    if (wave != 0) return;
-    add(1);
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-        const int r = n * 16 + col, i = r / a.group;
-        if (i >= s.m) continue;
+        for (int w = 0; w < W; w++) {
+            const float f = __builtin_amdgcn_exp2f(lds_ml[w][r][0] - ref);
+            l = fmaf(lds_ml[w][r][1], f, l);
+            x += *(const f32x4*)&lds_o[w][r][d] * f;
+        }
+        const int64_t row = s.r0 + r / a.group;
         const int hq = head * a.group + r % a.group;
-        const int64_t row = s.r0 + i;
         if (sp.parts == 1) {
-            const float inv = l[n] == 0.0f ? 0.0f : 1.0f / l[n];
+            const float inv = 1.0f / l;
+            float y[4];
 #pragma unroll
-            for (int d = 0; d < kDim; d++) {
-                float x[4];
-#pragma unroll
-                for (int k = 0; k < 4; k++) x[k] = l[n] == 0.0f ? 0.0f : o[n][d][k] * inv;
-                store_out4(a, row * a.out_row + hq * a.out_head + d * 16 + g * 4, x);
-            }
+            for (int k = 0; k < 4; k++) y[k] = l == 0.0f ? 0.0f : x[k] * inv;
+            store_out4(a, row * a.out_row + hq * a.out_head + d, y);
         } else {
             const int64_t at = (row * a.heads + hq) * a.parts + part;
-            if (g == 0) a.ml[at] = make_float2(m[n], l[n]);
-#pragma unroll
-            for (int d = 0; d < kDim; d++) *(f32x4*)(a.acc + at * D + d * 16 + g * 4) = o[n][d];
+            if (d == 0) a.ml[at] = make_float2(m, l);
+            *(f32x4*)(a.acc + at * D + d) = x;
         }
     }
 }
@@ -594,43 +572,65 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_many_kernel(KvCa
 
 // ------------------------------------------------------------------ the parts joined
 
-// One wave for each (row, head): out = sum_p 2^{m_p - m} O_p / sum_p 2^{m_p - m} l_p, the parts in order.
-template <int D>
-__global__ void __launch_bounds__(256) attend_join_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int row = (int)(w / a.heads), hq = (int)(w % a.heads);
+// out = sum_p 2^{m_p - m} O_p / sum_p 2^{m_p - m} l_p for each (row, head), by J waves that take every J-th part: one where there
+// are few parts, four where there are many.  Bound by the latency of three dependent loads (the sequence, m, O).
+template <int D, int J>
+__global__ void __launch_bounds__(256) attend_join_kernel(KvBatchDev B, AttnDev a) {
+    constexpr int N = (D + 63) / 64;
+    __shared__ float lds[J][64 * N + 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t w = J == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+    const int row = (int)(w / a.heads), hq = (int)(w % a.heads), p0 = J == 1 ? 0 : wave;
     if (row >= B.rows) return;
     KvSeq s;
     bool have = false;
     for (int b0 = 0; b0 < B.n && !have; b0 += 64) {
-        KvSeq t;
+        KvSeq t{};
         const bool mine = b0 + lane < B.n && kv_seq(B, b0 + lane, t) && row >= t.r0 && row < t.r0 + t.m;
         const uint64_t vote = __ballot(mine);
-        if (vote) have = kv_seq(B, b0 + __builtin_ctzll(vote), s);
+        if (vote) {
+            const int from = __builtin_ctzll(vote);
+            have = true;
+            s.b = b0 + from, s.r0 = __builtin_amdgcn_readlane(t.r0, from);
+            s.m = __builtin_amdgcn_readlane(t.m, from), s.len = __builtin_amdgcn_readlane(t.len, from);
+        }
     }
     if (!have) return;
     const int64_t r = (int64_t)(row - s.r0) * a.group + hq % a.group, first = r / a.tile_rows * a.tile_rows;
-    const Span sp = span_of(s, a.causal, a.window, a.chunk, (int)(first / a.group), (int)min((int64_t)s.m - 1, (first + a.tile_rows - 1) / a.group));
+    const Span sp = span_of(s, a.causal, a.window, a.chunk, (int)(first / a.group),
+                            (int)min((int64_t)s.m - 1, (first + a.tile_rows - 1) / a.group));
     if (sp.parts == 1) return;
     const int64_t at = ((int64_t)row * a.heads + hq) * a.parts;
     float m = -INFINITY;
     for (int p = lane; p < sp.parts; p += 64) m = fmaxf(m, a.ml[at + p].x);
+    m = other_half(other_row(m, true), true);
 #pragma unroll
-    for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
+    for (int k = 1; k < 16; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
     const float ref = m == -INFINITY ? 0.0f : m;
-    constexpr int N = (D + 63) / 64;
     float x[N], l = 0.0f;
 #pragma unroll
     for (int k = 0; k < N; k++) x[k] = 0.0f;
+    const int dim = min(lane, D - 1 - 64 * (N - 1));  // of the last 64 values
 #pragma unroll 8
-    for (int p = 0; p < sp.parts; p++) {
+    for (int p = p0; p < sp.parts; p += J) {
         const float2 ml = a.ml[at + p];
         const float f = __builtin_amdgcn_exp2f(ml.x - ref);
         l = fmaf(ml.y, f, l);
 #pragma unroll
-        for (int k = 0; k < N; k++)
-            if (D % 64 == 0 || lane + 64 * k < D) x[k] = fmaf(a.acc[(at + p) * D + lane + 64 * k], f, x[k]);
+        for (int k = 0; k < N; k++) x[k] = fmaf(a.acc[(at + p) * D + (k < N - 1 ? lane : dim) + 64 * k], f, x[k]);
+    }
+    if constexpr (J > 1) {
+#pragma unroll
+        for (int k = 0; k < N; k++) lds[wave][lane + 64 * k] = x[k];
+        if (lane == 0) lds[wave][64 * N] = l;
+        __syncthreads();
+        if (wave != 0) return;
+#pragma unroll
+        for (int j = 1; j < J; j++) {
+            l += lds[j][64 * N];
+#pragma unroll
+            for (int k = 0; k < N; k++) x[k] += lds[j][lane + 64 * k];
+        }
     }
     const float inv = 1.0f / l;
     uint16_t* out = (uint16_t*)a.out + row * a.out_row + hq * a.out_head;
@@ -646,15 +646,20 @@ template <int D, int CT>
 hipError_t run(const kk_kv_cache& c, const kk_kv_batch& b, const AttnPlan& p, const AttnDev& a, hipStream_t s) {
     const KvCacheDev cd = kv_dev(c);
     const KvBatchDev bd = kv_dev(b);
-    const dim3 grid((unsigned)(p.tiles * c.heads * p.parts)), block(256);
+    const dim3 grid((unsigned)(p.tiles * c.heads * p.parts));
     hipError_t rc;
-    if (p.few) {
-        rc = launch(p.row_tiles == 1 ? attend_few_kernel<D, CT, 1> : attend_few_kernel<D, CT, 2>, grid, block, 0, s, cd, bd, a);
-    } else {
-        rc = launch(attend_many_kernel<D, CT>, grid, block, 0, s, cd, bd, a);
-    }
+    if (!p.few)
+        rc = launch(attend_many_kernel<D, CT>, grid, dim3(256), 0, s, cd, bd, a);
+    else if (p.row_tiles == 1 && p.waves == 8)
+        rc = launch(attend_few_kernel<D, CT, 1, D <= 192 ? 8 : 4>, grid, dim3(D <= 192 ? 512 : 256), 0, s, cd, bd, a);
+    else if (p.row_tiles == 1)
+        rc = launch(attend_few_kernel<D, CT, 1, 4>, grid, dim3(256), 0, s, cd, bd, a);
+    else
+        rc = launch(attend_few_kernel<D, CT, 2, 4>, grid, dim3(256), 0, s, cd, bd, a);
     if (rc != hipSuccess || p.parts == 1) return rc;
-    return launch(attend_join_kernel<D>, dim3((unsigned)ceil_div((int64_t)b.rows * a.heads, 4)), block, 0, s, cd, bd, a);
+    const int64_t sums = (int64_t)b.rows * a.heads;
+    if (p.parts > 16) return launch(attend_join_kernel<D, 4>, dim3((unsigned)sums), dim3(256), 0, s, bd, a);
+    return launch(attend_join_kernel<D, 1>, dim3((unsigned)ceil_div(sums, 4)), dim3(256), 0, s, bd, a);
 }
 
 }  // namespace

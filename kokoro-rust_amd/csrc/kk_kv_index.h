@@ -103,6 +103,7 @@ __host__ __device__ inline Span span_of(const KvSeq& s, bool causal, int window,
 struct AttnPlan {
     bool few;         // at most kFewRows rows of a (sequence, cache head)
     int row_tiles;    // few: 16-row tiles of a block (1 or 2)
+    int waves;        // few: of a block, 8 while its blocks leave CUs idle, else 4
     int64_t tiles;    // blocks along the rows
     int chunk, parts; // pages of a part, parts of the axis
     int64_t ws_bytes; // partial results, 0 for one part
@@ -123,12 +124,13 @@ inline AttnPlan attention_plan(const kk_kv_cache& c, const kk_kv_batch& b, const
     int64_t chunk = pages;
     if (p.few)
         chunk = std::min<int64_t>(std::max<int64_t>(pages * blocks / (4 * n_cu), 8), 16);
-    else if (blocks < 2 * n_cu)
-        chunk = std::max<int64_t>(pages * blocks / (2 * n_cu), 8);
+    else if (2 * blocks <= n_cu)
+        chunk = std::max<int64_t>(pages * blocks / n_cu, 16);
     chunk = std::max(chunk, (pages + kMostParts - 1) / kMostParts);
     p.parts = (int)((pages + chunk - 1) / chunk);
     p.chunk = (int)((pages + p.parts - 1) / p.parts);
     p.parts = (int)((pages + p.chunk - 1) / p.chunk);
+    p.waves = blocks * p.parts <= n_cu ? 8 : 4;
     if (p.parts > 1) p.ws_bytes = (int64_t)b.rows * a.heads * p.parts * (c.dim * (int64_t)sizeof(float) + 2 * (int64_t)sizeof(float));
     return p;
 }

@@ -61,7 +61,7 @@ auto no_throw(char* err, size_t errlen, F&& f) -> decltype(f()) {
 bool empty(const kk_kv_batch& b) { return b.n == 0 || b.rows == 0 || b.max_new == 0; }
 
 std::string blocks_error(const kk_kv_batch& b, const AttnPlan& p, int heads, int cache_heads) {
-    if (p.tiles * cache_heads > kMostBlocks / p.parts || (p.parts > 1 && (int64_t)b.rows * heads / 4 > kMostBlocks))
+    if (p.tiles * cache_heads > kMostBlocks / p.parts || (p.parts > 1 && (int64_t)b.rows * heads > kMostBlocks))
         return "the batch is too large for one launch";
     return "";
 }

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import threading
 
 import numpy as np
 
@@ -205,6 +206,14 @@ def lib():
 
 def _err():
     return C.create_string_buffer(1024)
+
+
+class _OpsErr(threading.local):
+    def __init__(self):
+        self.err = _err()
+
+
+_ops = _OpsErr()
 
 
 def _check(rc, err):
@@ -445,26 +454,31 @@ class Context:
 
     # -------------------------------------------------------------- operators over an 8-bit cache
     # Device memory in and out, by pointer, on the caller's stream (an integer hipStream_t; 0 is the null stream); the
-    # structs can be kept and used again.  A call returns once its kernels are enqueued.
+    # structs can be kept and used again.  A call returns once its kernels are enqueued; the message buffer is one for each
+    # thread, since making one takes as long as the rest of a call's Python.
     def qk_norm_rope(self, args, stream=0):
         """kk_qk_norm_rope of a NormRope."""
-        err = _err()
-        _check(lib().kk_qk_norm_rope(self.h, C.byref(args), stream, err, len(err)), err)
+        rc = lib().kk_qk_norm_rope(self.h, C.byref(args), stream, _ops.err, 1024)
+        if rc:
+            _check(rc, _ops.err)
 
     def kv_write(self, cache, batch, rows, stream=0):
         """kk_kv_write: the KvRows into the KvCache as the last tokens of the KvBatch's sequences."""
-        err = _err()
-        _check(lib().kk_kv_write(self.h, C.byref(cache), C.byref(batch), C.byref(rows), stream, err, len(err)), err)
+        rc = lib().kk_kv_write(self.h, C.byref(cache), C.byref(batch), C.byref(rows), stream, _ops.err, 1024)
+        if rc:
+            _check(rc, _ops.err)
 
     def kv_read(self, cache, batch, rows, stream=0):
         """kk_kv_read: those tokens back into the KvRows."""
-        err = _err()
-        _check(lib().kk_kv_read(self.h, C.byref(cache), C.byref(batch), C.byref(rows), stream, err, len(err)), err)
+        rc = lib().kk_kv_read(self.h, C.byref(cache), C.byref(batch), C.byref(rows), stream, _ops.err, 1024)
+        if rc:
+            _check(rc, _ops.err)
 
     def kv_attention(self, cache, batch, args, stream=0):
         """kk_kv_attention of a KvAttention, whose workspace holds kv_attention_workspace bytes."""
-        err = _err()
-        _check(lib().kk_kv_attention(self.h, C.byref(cache), C.byref(batch), C.byref(args), stream, err, len(err)), err)
+        rc = lib().kk_kv_attention(self.h, C.byref(cache), C.byref(batch), C.byref(args), stream, _ops.err, 1024)
+        if rc:
+            _check(rc, _ops.err)
 
     def kv_attention_workspace(self, cache, batch, args):
         """kk_kv_attention_workspace: bytes (0: none needed)."""
