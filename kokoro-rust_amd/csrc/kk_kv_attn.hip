@@ -145,7 +145,7 @@ attend_few_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
     __shared__ float lds_ml[W][NT * 16][2];
     __shared__ __align__(16) float lds_o[W][NT * 16][kLd];
     const int head = blockIdx.x % c.heads, rest = blockIdx.x / c.heads;
-    const int part = rest % a.parts, b = rest / a.parts;
+    const int part = rest / B.n, b = rest % B.n;  // parts that only long sequences have come last: few blocks end empty meanwhile
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
     KvSeq s;

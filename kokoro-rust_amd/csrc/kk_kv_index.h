@@ -122,15 +122,20 @@ inline AttnPlan attention_plan(const kk_kv_cache& c, const kk_kv_batch& b, const
     pages = std::max<int64_t>(pages, 1);
     const int64_t blocks = p.tiles * c.heads;
     int64_t chunk = pages;
+    // Few rows: a part for each of two blocks a CU where that leaves at least a page a wave (4), and at most 32 pages (more
+    // parts than the device holds at once even out ragged lengths).  Measured at 8 heads of 128, us by the parts' pages 4, 8, 16,
+    // 32, 64, 128: one sequence of 8,000 tokens 11.2, 12.5, 15.1, 22.2, 34.9, 57.7; of 131,000: 66, 54, 52, 49, 48, 71; 64 of
+    // 200 to 8,191: 123, 104, 97, 99, 107, 119; 64 of 8,191: 250, 210, 189, 177, 173, 164.  Up to 1,000 tokens one block's 8
+    // waves, without a second launch, are as fast (11.5 against 11.8).
     if (p.few)
-        chunk = std::min<int64_t>(std::max<int64_t>(pages * blocks / (4 * n_cu), 8), 16);
+        chunk = pages <= 16 ? pages : std::min<int64_t>(std::max<int64_t>((pages * blocks + 2 * n_cu - 1) / (2 * n_cu), 4), 32);
     else if (2 * blocks <= n_cu)
         chunk = std::max<int64_t>(pages * blocks / n_cu, 16);
     chunk = std::max(chunk, (pages + kMostParts - 1) / kMostParts);
     p.parts = (int)((pages + chunk - 1) / chunk);
     p.chunk = (int)((pages + p.parts - 1) / p.parts);
     p.parts = (int)((pages + p.chunk - 1) / p.chunk);
-    p.waves = blocks * p.parts <= n_cu ? 8 : 4;
+    p.waves = blocks * p.parts <= n_cu && p.chunk > 4 ? 8 : 4;
     if (p.parts > 1) p.ws_bytes = (int64_t)b.rows * a.heads * p.parts * (c.dim * (int64_t)sizeof(float) + 2 * (int64_t)sizeof(float));
     return p;
 }

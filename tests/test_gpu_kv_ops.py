@@ -203,6 +203,25 @@ def test_attention(ctx, case):
     assert torch.equal(out, again)
 
 
+def test_attention_of_many_sequences(ctx):
+    """700 sequences, most of them short, some without rows or tokens, a few long ones: parts that only some sequences have."""
+    rng = np.random.default_rng(11)
+    lens = rng.integers(0, 90, 700)
+    lens[[3, 300, 301, 699]] = [1500, 9000, 64, 4321]
+    new = (rng.random(700) < 0.8).astype(int) * (lens > 0)
+    new[[3, 300, 699, 0]] = [3, 1, 2, 1]
+    lens[0] = 0  # a row that sees nothing
+    cache, tables = _filled(ctx, "int8", 1, 64, lens.tolist(), 12)
+    batch = R.Batch(new.tolist(), lens.tolist(), tables)
+    q = torch.randn(batch.rows, 4, 64, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    out = torch.full_like(q, 9.0)
+    args, space = R.attention_args(ctx, cache, batch, q, out, _code("bf16"), 0.2)
+    assert args.workspace_bytes > 0
+    ctx.kv_attention(cache.args, batch.args, args)
+    R.check_attention(out, q, cache, batch, 0.2, True, 0, "bf16")
+    assert (space[args.workspace_bytes:] == 0xA5).all() and int(cache.fault) == 0
+
+
 @pytest.mark.parametrize("new", [1, 40])
 def test_attention_rows_and_strides(ctx, new):
     """Queries and outputs in wider rows, aligned to 16 bytes and not; the same values as from packed ones."""
@@ -336,15 +355,16 @@ def test_bad_pages(ctx):
 
 @pytest.mark.parametrize("new", [1, 2, 40])
 @pytest.mark.parametrize("wrong", ["long", "rows", "fall", "negative"])
-def test_bad_sequences(ctx, new, wrong):
+@pytest.mark.parametrize("bound", [150, 5000])
+def test_bad_sequences(ctx, new, wrong, bound):
     """A sequence whose length or rows leave the bounds is left out and reported; its neighbours are computed."""
     from kokoro_hip import api
     lens = [100, 150, 80]
     cache, tables = _filled(ctx, "int8", 1, 64, lens, 4)
-    batch = R.Batch([new] * 3, lens, tables, first=3, rows=3 * new + 3)
+    batch = R.Batch([new] * 3, lens, tables, first=3, rows=3 * new + 3, max_len=bound, width=-(-bound // PAGE))
     start, length = batch.dev[0], batch.dev[1]
     if wrong == "long":
-        length[1] = 151
+        length[1] = bound + 1
     elif wrong == "negative":
         length[1] = -1
     elif wrong == "rows":
