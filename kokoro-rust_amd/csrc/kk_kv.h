@@ -53,9 +53,10 @@ __device__ __forceinline__ int kv_find(const KvCacheDev& c, const KvBatchDev& B,
         if (ok && kv_tile_in(t, tile, G, M, E, i)) found[0] = b, found[1] = i;
     }
     __syncthreads();
-    if (found[0] < 0) return -1;
-    kv_seq(B, found[0], s);
-    return found[1];
+    const int b = __builtin_amdgcn_readfirstlane(found[0]);  // scalar from here on
+    if (b < 0) return -1;
+    kv_seq(B, b, s);
+    return __builtin_amdgcn_readfirstlane(found[1]);
 }
 
 // ------------------------------------------------------------------ stored numbers

@@ -55,12 +55,28 @@ __device__ __forceinline__ void q_units(float top, float& down, float& up) {
     up = __uint_as_float((uint32_t)(e - 14) << 23);
 }
 
-template <int N>
-__device__ __forceinline__ void load_query(const AttnDev& a, int64_t at, float* x) {
-    if (a.type == KK_BF16)
-        load_values<KK_BF16, N>(a.q, at, a.q_vec, x);
-    else
-        load_values<KK_F16, N>(a.q, at, a.q_vec, x);
+// P pieces of 8 query values, `step` values apart, to f32: the loads of all of them before the first is used.
+template <int P>
+__device__ __forceinline__ void load_query(const AttnDev& a, int64_t at, int step, float* x) {
+    uint16_t e[P][8];
+    const uint16_t* p = (const uint16_t*)a.q + at;
+    if (a.q_vec) {
+#pragma unroll
+        for (int j = 0; j < P; j++) {
+            const uint4 w = *(const uint4*)(p + j * step);
+            __builtin_memcpy(e[j], &w, 16);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < P; j++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) e[j][k] = p[j * step + k];
+    }
+#pragma unroll
+    for (int j = 0; j < P; j++)
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            x[8 * j + k] = a.type == KK_BF16 ? ElemOf<KK_BF16>::load(e[j][k]) : ElemOf<KK_F16>::load(e[j][k]);
 }
 
 // Four values of a row, next to each other, behind a division by l (or as a part's).
@@ -101,13 +117,14 @@ __device__ __forceinline__ PageIn page_in(const KvCacheDev& c, const KvBatchDev&
     return p;
 }
 
-// A row's maxima and sum; `page` brings in a page with V's scale b, in which the row's largest s is `top`.  Returns whether any
+// A row's maxima and sum; `page` brings in a page with V's scale b (log_b = log2 b, -inf for a page of zeros), in which the
+// row's largest s is `top`.  Returns whether any
 // row of the wave moved (then O is to be multiplied by f); P = 2^{s + off}, and the sum of P counts w in l.
 struct RowSum {
     float M = -INFINITY, m = -INFINITY, l = 0.0f;
-    __device__ __forceinline__ bool page(float b, float top, float& f, float& off, float& w) {
-        const bool zero = b == 0.0f;
-        const float b_log = zero ? 0.0f : __builtin_amdgcn_logf(b);
+    __device__ __forceinline__ bool page(float log_b, float top, float& f, float& off, float& w) {
+        const bool zero = log_b == -INFINITY;
+        const float b_log = zero ? 0.0f : log_b;
         const bool up_M = !zero && top + b_log > M + kSlack, up_m = top > m + kSlack;
         const bool moves = __ballot(up_M || up_m) != 0;
         if (moves) {
@@ -196,12 +213,14 @@ attend_few_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
         for (int j = 0; j < D / 4; j++) x[j] = 0.0f;
         if (on) {
             const int64_t at = (int64_t)(s.r0 + i) * a.q_row + (head * a.group + r % a.group) * a.q_head;
+            if constexpr (kWide) {  // 16 values of each 64 a lane: the two halves of 8 apart
+                float y[2][D / 8];
+                load_query<D / 64>(a, at + g * 16, 64, y[0]);
+                load_query<D / 64>(a, at + g * 16 + 8, 64, y[1]);
 #pragma unroll
-            for (int j = 0; j < kLoads; j++) {
-                if constexpr (kWide)
-                    load_query<16>(a, at + j * 64 + g * 16, x + 16 * j);
-                else
-                    load_query<8>(a, at + j * 32 + g * 8, x + 8 * j);
+                for (int j = 0; j < D / 4; j++) x[j] = y[j / 8 & 1][j / 16 * 8 + j % 8];
+            } else {
+                load_query<D / 32>(a, at + g * 8, 32, x);
             }
         }
         float top = 0.0f;
@@ -287,7 +306,7 @@ attend_few_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
                 for (int r = 0; r < 4; r++) mx = fmaxf(mx, sc[n][t][r]);
             mx = other_half(other_row(mx, true), true) * c1;
             float f, off, w;
-            if (rs[n].page(p.v_scale, mx, f, off, w))
+            if (rs[n].page(__builtin_amdgcn_logf(p.v_scale), mx, f, off, w))
 #pragma unroll
                 for (int d = 0; d < kDim; d++) o[n][d] *= f;
             float sum = 0.0f;
@@ -365,36 +384,111 @@ attend_few_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
 
 // ------------------------------------------------------------------ many rows: prompts
 
-// 128 rows of a (sequence, cache head), 32 a wave (v_mfma_f32_32x32x16_f16).  Bound by the matrix cores, the exponentials
-// beside them, and the unpacking, which a block does once for all its rows: a page's bytes are loaded while the page before is
-// computed, unpacked and stored to the other of two LDS buffers, K by token ([token][dim]), V by value ([dim][token]),
-// rows padded by 16 bytes (16-byte reads of 8 lanes then cover all banks).  Within 32 tokens K's rows are stored so
-// that a lane's 8 scores of one step are 8 tokens in order, as its 16 bytes of V hold them.
-template <int D, int CT>
-__global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_many_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
+// 32 W rows of a (sequence, cache head), 32 a wave (v_mfma_f32_32x32x16_f16).  Bound by the matrix cores and the vector
+// instructions beside them (exponentials, unpacking) in about equal parts, so both must run at once.  While a page's scores become
+// probabilities, the next page's first product runs, and while its second product runs, the pages after are unpacked, one
+// matrix instruction with its share of vector instructions after the other (the order of the source, which sched_barrier
+// keeps; left to itself the compiler puts each kind in a row).
+// With W = 8 a SIMD's two waves are half a page apart (two barriers a page): one takes its maxima and exponentials while the
+// other is in its second product; K and V have three buffers each.  With W = 4, for fewer rows or heads of over 128 values, all waves
+// go together, on two buffers.
+// A page's bytes are loaded a whole page ahead, unpacked once for all the block's rows and stored to LDS, K by token
+// ([token][dim]), V by value ([dim][token]), rows padded by 16 bytes (16-byte reads of 8 lanes then cover all banks).  Within 32
+// tokens K's rows are stored so that a lane's 8 scores of one step are 8 tokens in order, as its 16 bytes of V hold them.
+// Page numbers and scales are read 64 pages at a time, one a lane.
+template <int D, int CT, int W>
+__global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) attend_many_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
+    constexpr int kRows = 32 * W, kThreads = 64 * W;
+    constexpr bool kApart = W == 8;
+    constexpr int kBufs = kApart ? 3 : 2;
     constexpr int kK = D + 8, kV = kPage + 8;  // halves of a row in LDS
-    constexpr int kBuf = kPage * kK + D * kV;
-    constexpr int kLoads = (4 * D + 255) / 256;  // 16-byte pieces of K, and of V, a thread
+    constexpr int kKBuf = kPage * kK, kVBuf = D * kV;
+    constexpr int kLoads = (4 * D + kThreads - 1) / kThreads;  // 16-byte pieces of K, and of V, a thread (the last one's twice where they do not divide)
     constexpr int kSteps = D / 16, kDim = D / 32;
-    __shared__ __align__(16) _Float16 lds[2 * kBuf];
+    constexpr int kFirst = 2 * kSteps, kSecond = 4 * kDim, kAhead = 4;  // products of a page, operands read ahead
+    __shared__ __align__(16) _Float16 lds[kBufs * (kKBuf + kVBuf)];
     __shared__ int found[2];
     const int head = blockIdx.x % c.heads, rest = blockIdx.x / c.heads;
     const int part = rest % a.parts;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, h = lane >> 5;
     KvSeq s;
-    int tile = kv_find<256>(c, B, rest / a.parts, a.group, kManyRows, 1, blockIdx.x == 0, s, found);
+    int tile = kv_find<kThreads>(c, B, rest / a.parts, a.group, kRows, 1, blockIdx.x == 0, s, found);
     const int64_t all_rows = tile < 0 ? 0 : (int64_t)s.m * a.group;
-    const int tiles = (int)((all_rows + kManyRows - 1) / kManyRows);
+    const int tiles = (int)((all_rows + kRows - 1) / kRows);
     if (tile < 0 || tile >= tiles) return;
     tile = tiles - 1 - tile;  // the rows that see most first
-    const int64_t r_first = (int64_t)tile * kManyRows;
-    const Span sp = span_of(s, a.causal, a.window, a.chunk, (int)(r_first / a.group), (int)min((int64_t)s.m - 1, (r_first + kManyRows - 1) / a.group));
+    const int64_t r_first = (int64_t)tile * kRows;
+    const int i_first = (int)(r_first / a.group), over = (int)(r_first % a.group);  // the block's first row: token, head
+    const Span sp = span_of(s, a.causal, a.window, a.chunk, i_first, min(s.m - 1, i_first + (over + kRows - 1) / a.group));
     if (part >= sp.parts) return;
     const int page0 = sp.lo + part * a.chunk, page1 = min(page0 + a.chunk, sp.hi);
 
-    const int64_t r = r_first + wave * 32 + col;
-    const int i = (int)(r / a.group), hq = head * a.group + (int)(r % a.group);
+    // numbers and scales of the pages from `base` on, one a lane; a page that does not exist is page 0 with a NaN scale of K, and its
+    // V is masked: rows that do not see it stay clean
+    int base = page0, ids = 0;
+    float k_scales = 0.0f, v_logs = 0.0f;
+    const int end = page1 - 1;
+    auto look = [&](int from) {
+        base = from;
+        const int id = B.table[s.b * B.stride + min(from + lane, end)];
+        const bool bad = id < 0 || id >= c.pages;
+        if (bad && wave == 0) kv_fault(c, KK_KV_BAD_PAGE);
+        const int64_t at = (int64_t)(bad ? 0 : id) * c.heads + head;
+        ids = bad ? -1 : id;
+        k_scales = bad ? __uint_as_float(0x7fc00000u) : c.ks[at];
+        v_logs = __builtin_amdgcn_logf(bad ? 0.0f : c.vs[at]);
+        // waited for here: behind the branch that this is in, the wait would be for every load of the loop
+        asm volatile("" ::"v"(ids), "v"(k_scales), "v"(v_logs));
+    };
+    auto number = [&](int page) { return __builtin_amdgcn_readlane(ids, min(page, end) - base); };
+    auto of = [&](float x, int page) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), page - base)); };
+
+    uint4 kr[kLoads], vr[kLoads];
+    auto load = [&](uint4* to, const uint8_t* from, int page) {
+        const uint8_t* p = from + ((int64_t)max(number(page), 0) * c.heads + head) * (kPage * D);
+#pragma unroll
+        for (int j = 0; j < kLoads; j++) to[j] = *(const uint4*)(p + (uint32_t)(min(tid + j * kThreads, 4 * D - 1) * 16));
+    };
+    // half piece n of K (n < 2 kLoads) and then V from their registers to LDS
+    auto unpack = [&](int n, _Float16* kb, _Float16* vb) {
+        const int j = n / 2 % kLoads, half = n & 1, w = min(tid + j * kThreads, 4 * D - 1);
+        if (n < 2 * kLoads) {
+            const int tok = w / (D / 16), d = (w % (D / 16)) * 16 + half * 8;
+            // token 16 s + 8 h + j of 32 (j = 4 u + k) is the row that lane half h holds as score 8 s + j
+            const int row = (tok & 32) | ((tok & 16) | ((tok & 4) << 1) | ((tok & 8) >> 1) | (tok & 3));
+            *(f16x8*)(kb + row * kK + d) = half ? unpack8<CT>(kr[j].z, kr[j].w) : unpack8<CT>(kr[j].x, kr[j].y);
+        } else {
+            *(f16x8*)(vb + w / 4 * kV + w % 4 * 16 + half * 8) = half ? unpack8<CT>(vr[j].z, vr[j].w) : unpack8<CT>(vr[j].x, vr[j].y);
+        }
+    };
+    // slots of V behind the sequence's last token, which may hold the NaN code
+    auto mask_v = [&](int page) {
+        if constexpr (CT == KK_KV_E4M3) {
+            const int live = number(page) < 0 ? 0 : s.len - min(page, end) * kPage;
+            if (live >= kPage) return;
+#pragma unroll
+            for (int j = 0; j < kLoads; j++) {
+                const int t = min(tid + j * kThreads, 4 * D - 1) % 4 * 16;
+                uint32_t* v = (uint32_t*)&vr[j];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int left = live - (t + 4 * k);
+                    v[k] = left >= 4 ? v[k] : left <= 0 ? 0u : v[k] & (0xffffffffu >> (32 - 8 * left));
+                }
+            }
+        }
+    };
+    _Float16* const k_buf = lds;
+    _Float16* const v_buf = lds + kBufs * kKBuf;
+    if (page0 < page1) {  // the first pages' bytes are on their way while the queries are read
+        look(page0);
+        load(kr, c.k, page0);
+        load(vr, c.v, page0);
+    }
+
+    // the row of this lane's column, and what the wave's first and last row see
+    const int in = over + wave * 32 + col, i = i_first + in / a.group, hq = head * a.group + in % a.group;
     const bool on = i < s.m;
     f16x8 q[kSteps];
     float qs;
@@ -402,10 +496,7 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_many_kernel(KvCa
         float x[D / 2];
 #pragma unroll
         for (int j = 0; j < D / 2; j++) x[j] = 0.0f;
-        if (on)
-#pragma unroll
-            for (int j = 0; j < kSteps; j++)
-                load_query<8>(a, (int64_t)(s.r0 + i) * a.q_row + hq * a.q_head + j * 16 + h * 8, x + 8 * j);
+        if (on) load_query<kSteps>(a, (int64_t)(s.r0 + i) * a.q_row + hq * a.q_head + h * 8, 16, x);
         float top = 0.0f;
 #pragma unroll
         for (int j = 0; j < D / 2; j++) top = fmaxf(top, fabsf(x[j]));
@@ -418,15 +509,11 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_many_kernel(KvCa
 #pragma unroll
             for (int k = 0; k < 8; k++) q[j][k] = (_Float16)(x[8 * j + k] * down);
     }
-    const int pos = s.len - s.m + i;
-    const int hi = on ? (a.causal ? max(0, min(s.len, pos + 1)) : s.len) : 0;
-    const int lo = a.window ? max(0, pos - a.window + 1) : 0;
-    // what the wave's first and last row see
-    const int i0 = (int)((r_first + wave * 32) / a.group), i1 = (int)min((int64_t)s.m - 1, (r_first + wave * 32 + 31) / a.group);
     const int off = s.len - s.m;
+    const int hi = on ? (a.causal ? max(0, min(s.len, off + i + 1)) : s.len) : 0;
+    const int lo = a.window ? max(0, off + i - a.window + 1) : 0;
+    const int i0 = i_first + (over + wave * 32) / a.group, i1 = min(s.m - 1, i_first + (over + wave * 32 + 31) / a.group);
     const int all_lo = a.window ? off + i1 - a.window + 1 : 0, all_hi = a.causal ? min(s.len, off + i0 + 1) : s.len;
-    const int any_lo = a.window ? max(0, off + i0 - a.window + 1) : 0;
-    const int any_hi = i0 >= s.m ? 0 : a.causal ? max(0, min(s.len, off + i1 + 1)) : s.len;
 
     f32x16 o[kDim];
 #pragma unroll
@@ -435,114 +522,117 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attend_many_kernel(KvCa
         for (int k = 0; k < 16; k++) o[d][k] = 0.0f;
     RowSum rs;
 
-    uint4 kr[kLoads], vr[kLoads];
-    auto load = [&](const PageIn& p) {
-        const uint4 *kb = (const uint4*)(c.k + p.at * (kPage * D)), *vb = (const uint4*)(c.v + p.at * (kPage * D));
-#pragma unroll
-        for (int j = 0; j < kLoads; j++) {
-            const int w = tid + j * 256;
-            if (4 * D % 256 == 0 || w < 4 * D) kr[j] = kb[w], vr[j] = vb[w];
-        }
+    const int k_at = col * kK + h * 8, v_at = col * kV + h * 8;  // of this lane's operands
+    // operand n of a page: K's of the first product, then V's of the second
+    auto operand = [&](int n, const _Float16* kb, const _Float16* vb) {
+        return n < kFirst ? *(const f16x8*)(kb + k_at + (n & 1) * 32 * kK + (n >> 1) * 16)
+                          : *(const f16x8*)(vb + v_at + (n - kFirst) % kDim * 32 * kV + (n - kFirst) / kDim * 16);
     };
-    auto store = [&](int live, int buf) {
-        _Float16 *kb = lds + buf * kBuf, *vb = kb + kPage * kK;
-#pragma unroll
-        for (int j = 0; j < kLoads; j++) {
-            const int w = tid + j * 256;
-            if (4 * D % 256 != 0 && w >= 4 * D) continue;
-            const int tok = w / (D / 16), d = (w % (D / 16)) * 16;
-            // token 16 s + 8 h + j of 32 (j = 4 u + k) is the row that lane half h holds as score 8 s + j
-            const int row = (tok & 32) | ((tok & 16) | ((tok & 4) << 1) | ((tok & 8) >> 1) | (tok & 3));
-            *(f16x8*)(kb + row * kK + d) = unpack8<CT>(kr[j].x, kr[j].y);
-            *(f16x8*)(kb + row * kK + d + 8) = unpack8<CT>(kr[j].z, kr[j].w);
-            const int dv = w / 4, t = (w % 4) * 16;
-            if (CT == KK_KV_E4M3 && live < kPage) {
-                uint32_t* v = (uint32_t*)&vr[j];
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int left = live - (t + 4 * k);
-                    v[k] = left >= 4 ? v[k] : left <= 0 ? 0u : v[k] & (0xffffffffu >> (32 - 8 * left));
-                }
-            }
-            *(f16x8*)(vb + dv * kV + t) = unpack8<CT>(vr[j].x, vr[j].y);
-            *(f16x8*)(vb + dv * kV + t + 8) = unpack8<CT>(vr[j].z, vr[j].w);
-        }
-    };
+    int side = 0;  // the page's buffer: page number modulo kBufs, counted from page0
+    auto next_side = [](int x) { return x + 1 == kBufs ? 0 : x + 1; };
 
-    PageIn now, next;
-    if (page0 < page1) {
-        now = page_in(c, B, s, page0, head, tid == 0);
-        load(now);
-        store(now.live, 0);
-    }
-    __syncthreads();
-    int buf = 0;
-    for (int page = page0; page < page1; page++, buf ^= 1) {
-        const bool more = page + 1 < page1;
-        if (more) {
-            next = page_in(c, B, s, page + 1, head, tid == 0);
-            load(next);
-        }
+    // One page: its scores `sc` are there, and the next page's are left in `nx`.  What there is no page for is computed from
+    // what the buffers hold and not used.  K of page + kBufs and V of the one before go into the buffers that K of this page
+    // and V of the page before were in: all waves have read those (K in the part before, V at least a barrier ago).
+    auto one = [&](int page, f32x16* sc, f32x16* nx) {
+        const int after = next_side(side);
+        const _Float16 *kb = k_buf + after * kKBuf, *vb = v_buf + side * kVBuf;
+        if (page + kBufs + 1 - base > 63) look(page);
+        f16x8 f[kAhead];
+#pragma unroll
+        for (int n = 0; n < kAhead; n++) f[n] = operand(n, kb, vb);
         const int t0 = page * kPage;
-        if (t0 < any_hi && t0 + kPage > any_lo) {
-            const _Float16 *kb = lds + buf * kBuf, *vb = kb + kPage * kK;
-            f32x16 sc[2];
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int k = 0; k < 16; k++) sc[t][k] = 0.0f;
-#pragma unroll
-            for (int j = 0; j < kSteps; j++)
-#pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const f16x8 k = *(const f16x8*)(kb + (t * 32 + col) * kK + j * 16 + h * 8);
-                    sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[j], sc[t], 0, 0, 0);
-                }
-            float c1 = qs * now.k_scale;
-            if (!(t0 >= all_lo && t0 + kPage <= all_hi)) {
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int k = 0; k < 16; k++) {
-                        const int tok = t0 + t * 32 + (k >> 3) * 16 + h * 8 + (k & 7);
-                        sc[t][k] = tok >= lo && tok < hi ? sc[t][k] * c1 : -INFINITY;
-                    }
-                c1 = 1.0f;
-            }
-            float mx = -INFINITY;
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int k = 0; k < 16; k++) mx = fmaxf(mx, sc[t][k]);
-            mx = other_half(mx, true) * c1;
-            float f, add, w;
-            if (rs.page(now.v_scale, mx, f, add, w))
-#pragma unroll
-                for (int d = 0; d < kDim; d++) o[d] *= f;
-            f16x8 pr[4];
-            float sum = 0.0f;
+        float c1 = qs * of(k_scales, page);
+        if (!(t0 >= all_lo && t0 + kPage <= all_hi)) {
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
                 for (int k = 0; k < 16; k++) {
-                    const float e = __builtin_amdgcn_exp2f(fmaf(sc[t][k], c1, add));
-                    sum += e;
-                    pr[t * 2 + (k >> 3)][k & 7] = (_Float16)e;
+                    const int tok = t0 + t * 32 + (k >> 3) * 16 + h * 8 + (k & 7);
+                    sc[t][k] = tok >= lo && tok < hi ? sc[t][k] * c1 : -INFINITY;
                 }
-            rs.l = fmaf(sum, w, rs.l);
-#pragma unroll
-            for (int d = 0; d < kDim; d++)
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const f16x8 v = *(const f16x8*)(vb + (d * 32 + col) * kV + u * 16 + h * 8);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pr[u], o[d], 0, 0, 0);
-                }
+            c1 = 1.0f;
         }
-        if (more) {
-            store(next.live, buf ^ 1);
-            now = next;
+        float top[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) top[k] = fmaxf(sc[k >> 1][8 * (k & 1)], sc[k >> 1][8 * (k & 1) + 1]);
+#pragma unroll
+        for (int j = 2; j < 8; j += 2)
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                top[k] = fmaxf(fmaxf(top[k], sc[k >> 1][8 * (k & 1) + j]), sc[k >> 1][8 * (k & 1) + j + 1]);
+        const float mx = other_half(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), true) * c1;
+        float by, add, w;
+        if (rs.page(of(v_logs, page), mx, by, add, w))
+#pragma unroll
+            for (int d = 0; d < kDim; d++) o[d] *= by;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int k = 0; k < 16; k++) nx[t][k] = 0.0f;
+        f16x8 pr[4];
+        float sum = 0.0f;
+#pragma unroll
+        for (int n = 0; n < kFirst; n++) {
+            nx[n & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[n % kAhead], q[n >> 1], nx[n & 1], 0, 0, 0);
+            f[n % kAhead] = operand(n + kAhead, kb, vb);
+#pragma unroll
+            for (int k = 16 * n / kFirst; k < 16 * (n + 1) / kFirst; k++) {
+                const float e0 = __builtin_amdgcn_exp2f(fmaf(sc[k >> 3][2 * (k & 7)], c1, add));
+                const float e1 = __builtin_amdgcn_exp2f(fmaf(sc[k >> 3][2 * (k & 7) + 1], c1, add));
+                const f16x2 e = {(_Float16)e0, (_Float16)e1};
+                pr[k >> 2][2 * (k & 3)] = e[0], pr[k >> 2][2 * (k & 3) + 1] = e[1];
+                sum = __builtin_amdgcn_fdot2(e, f16x2{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        rs.l = fmaf(sum, w, rs.l);
+        if constexpr (kApart) __syncthreads();
+        mask_v(page + kBufs - 1);
+        constexpr int kPieces = 4 * kLoads;
+        _Float16 *k_to = k_buf + side * kKBuf, *v_to = v_buf + (side == 0 ? kBufs - 1 : side - 1) * kVBuf;
+#pragma unroll
+        for (int n = 0; n < kSecond; n++) {
+            const int d = n % kDim, u = n / kDim;
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[(kFirst + n) % kAhead], pr[u], o[d], 0, 0, 0);
+            if (n + kAhead < kSecond) f[(kFirst + n) % kAhead] = operand(kFirst + n + kAhead, kb, vb);
+#pragma unroll
+            for (int k = kPieces * n / kSecond; k < kPieces * (n + 1) / kSecond; k++) unpack(k, k_to, v_to);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        load(kr, c.k, page + kBufs + 1);
+        load(vr, c.v, page + kBufs);
+        side = after;
+        __syncthreads();
+    };
+
+    if (page0 < page1) {
+        f32x16 sa[2], sb[2];
+#pragma unroll
+        for (int p = 0; p < kBufs; p++) {  // K of the first kBufs pages, V of one less, and the next ones' bytes
+            mask_v(page0 + p);
+#pragma unroll
+            for (int n = 0; n < (p + 1 < kBufs ? 4 : 2) * kLoads; n++) unpack(n, k_buf + p * kKBuf, v_buf + p * kVBuf);
+            load(kr, c.k, page0 + p + 1);
+            if (p + 1 < kBufs) load(vr, c.v, page0 + p + 1);
         }
         __syncthreads();
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int k = 0; k < 16; k++) sa[t][k] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < kFirst; n++)
+            sa[n & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(operand(n, k_buf, v_buf), q[n >> 1], sa[n & 1], 0, 0, 0);
+        __syncthreads();  // K's first buffer is written again by the first page
+        if (kApart && wave >= 4) __syncthreads();
+        for (int page = page0;;) {
+            one(page, sa, sb);
+            if (++page == page1) break;
+            one(page, sb, sa);
+            if (++page == page1) break;
+        }
+        if (kApart && wave < 4) __syncthreads();
     }
     const float l = other_half(rs.l, false), last = rs.last();
     if (!on) return;
@@ -649,7 +739,8 @@ hipError_t run(const kk_kv_cache& c, const kk_kv_batch& b, const AttnPlan& p, co
     const dim3 grid((unsigned)(p.tiles * c.heads * p.parts));
     hipError_t rc;
     if (!p.few)
-        rc = launch(attend_many_kernel<D, CT>, grid, dim3(256), 0, s, cd, bd, a);
+        rc = launch(p.tile_rows == 256 ? attend_many_kernel<D, CT, D <= 128 ? 8 : 4> : attend_many_kernel<D, CT, 4>, grid,
+                    dim3(2 * p.tile_rows), 0, s, cd, bd, a);
     else if (p.row_tiles == 1 && p.waves == 8)
         rc = launch(attend_few_kernel<D, CT, 1, D <= 192 ? 8 : 4>, grid, dim3(D <= 192 ? 512 : 256), 0, s, cd, bd, a);
     else if (p.row_tiles == 1)
@@ -674,7 +765,7 @@ hipError_t launch_kv_attention(const kk_kv_cache& c, const kk_kv_batch& b, const
     d.heads = a.heads, d.group = a.heads / c.heads, d.type = a.type, d.causal = a.causal, d.window = a.window;
     d.q_vec = (uintptr_t)a.q % 16 == 0 && a.q_row % 8 == 0 && a.q_head % 8 == 0;
     d.out_vec = (uintptr_t)a.out % 8 == 0 && a.out_row % 4 == 0 && a.out_head % 4 == 0;
-    d.chunk = p.chunk, d.parts = p.parts, d.tile_rows = p.few ? 16 * p.row_tiles : kManyRows;
+    d.chunk = p.chunk, d.parts = p.parts, d.tile_rows = p.tile_rows;
 #define KK_ATTN_CASE(D) \
     case D: return c.type == KK_KV_INT8 ? run<D, KK_KV_INT8>(c, b, p, d, s) : run<D, KK_KV_E4M3>(c, b, p, d, s);
     switch (c.dim) {

@@ -12,7 +12,6 @@ namespace kk {
 
 constexpr int kPage = KK_KV_PAGE;
 constexpr int kFewRows = 32;     // rows of a (sequence, cache head) up to which attention reads the cache into registers
-constexpr int kManyRows = 128;   // rows of a block of the attention kernel for prompts
 constexpr int kMostParts = 256;  // of the token axis
 
 struct KvBatchDev {
@@ -104,6 +103,7 @@ struct AttnPlan {
     bool few;         // at most kFewRows rows of a (sequence, cache head)
     int row_tiles;    // few: 16-row tiles of a block (1 or 2)
     int waves;        // few: of a block, 8 while its blocks leave CUs idle, else 4
+    int tile_rows;    // rows of a block: many, 256 where that fills the device, or 128
     int64_t tiles;    // blocks along the rows
     int chunk, parts; // pages of a part, parts of the axis
     int64_t ws_bytes; // partial results, 0 for one part
@@ -113,10 +113,11 @@ inline AttnPlan attention_plan(const kk_kv_cache& c, const kk_kv_batch& b, const
     const int64_t group = a.heads / c.heads, rows = b.max_new * group;
     p.few = rows <= kFewRows;
     p.row_tiles = rows <= 16 ? 1 : 2;
-    p.tiles = p.few ? b.n : b.rows * group / kManyRows + b.n;
+    p.tile_rows = p.few ? 16 * p.row_tiles : c.dim <= 128 && (b.rows * group / 256 + b.n) * c.heads >= n_cu ? 256 : 128;
+    p.tiles = p.few ? b.n : b.rows * group / p.tile_rows + b.n;
     int64_t pages = ((int64_t)b.max_len + kPage - 1) / kPage;
     if (a.window) {  // a block's rows stand at most that many tokens apart, and N tokens touch at most N / 64 + 2 pages
-        const int64_t seen = (int64_t)a.window + (p.few ? b.max_new : kManyRows / group + 1);
+        const int64_t seen = (int64_t)a.window + (p.few ? b.max_new : p.tile_rows / group + 1);
         pages = std::min(pages, seen / kPage + 2);
     }
     pages = std::max<int64_t>(pages, 1);

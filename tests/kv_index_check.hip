@@ -104,10 +104,10 @@ int main(int argc, char** argv) {
                     end = (int64_t)s.m * group;
                     if (end > 16 * p.row_tiles) bad++;
                 } else {
-                    const int i = find(x, group, kManyRows, 1, s);
-                    const int64_t all = i < 0 ? 0 : (int64_t)s.m * group, tiles = (all + kManyRows - 1) / kManyRows;
+                    const int i = find(x, group, p.tile_rows, 1, s);
+                    const int64_t all = i < 0 ? 0 : (int64_t)s.m * group, tiles = (all + p.tile_rows - 1) / p.tile_rows;
                     if (i < 0 || i >= tiles) continue;
-                    first = (tiles - 1 - i) * kManyRows, end = std::min(all, first + kManyRows);
+                    first = (int64_t)(tiles - 1 - i) * p.tile_rows, end = std::min(all, first + p.tile_rows);
                 }
                 for (int64_t r = first; r < end; r++) seen[(size_t)(s.r0 + r / group) * group + r % group]++;
                 const int i0 = (int)(first / group), i1 = (int)std::min<int64_t>(s.m - 1, (end - 1) / group);
