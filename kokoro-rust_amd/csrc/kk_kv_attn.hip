@@ -55,10 +55,9 @@ __device__ __forceinline__ void q_units(float top, float& down, float& up) {
     up = __uint_as_float((uint32_t)(e - 14) << 23);
 }
 
-// P pieces of 8 query values, `step` values apart, to f32: the loads of all of them before the first is used.
+// P pieces of 8 query values, `step` values apart: all loads before the first is used, and then to f32.
 template <int P>
-__device__ __forceinline__ void load_query(const AttnDev& a, int64_t at, int step, float* x) {
-    uint16_t e[P][8];
+__device__ __forceinline__ void load_query(const AttnDev& a, int64_t at, int step, uint16_t (*e)[8]) {
     const uint16_t* p = (const uint16_t*)a.q + at;
     if (a.q_vec) {
 #pragma unroll
@@ -72,6 +71,9 @@ __device__ __forceinline__ void load_query(const AttnDev& a, int64_t at, int ste
 #pragma unroll
             for (int k = 0; k < 8; k++) e[j][k] = p[j * step + k];
     }
+}
+template <int P>
+__device__ __forceinline__ void query_values(const AttnDev& a, const uint16_t (*e)[8], float* x) {
 #pragma unroll
     for (int j = 0; j < P; j++)
 #pragma unroll
@@ -213,14 +215,17 @@ attend_few_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
         for (int j = 0; j < D / 4; j++) x[j] = 0.0f;
         if (on) {
             const int64_t at = (int64_t)(s.r0 + i) * a.q_row + (head * a.group + r % a.group) * a.q_head;
+            uint16_t e[D / 32][8];
             if constexpr (kWide) {  // 16 values of each 64 a lane: the two halves of 8 apart
-                float y[2][D / 8];
-                load_query<D / 64>(a, at + g * 16, 64, y[0]);
-                load_query<D / 64>(a, at + g * 16 + 8, 64, y[1]);
+                float y[D / 4];
+                load_query<D / 64>(a, at + g * 16, 64, e);
+                load_query<D / 64>(a, at + g * 16 + 8, 64, e + D / 64);
+                query_values<D / 32>(a, e, y);
 #pragma unroll
-                for (int j = 0; j < D / 4; j++) x[j] = y[j / 8 & 1][j / 16 * 8 + j % 8];
+                for (int j = 0; j < D / 4; j++) x[j] = y[(j / 8 & 1) * (D / 8) + j / 16 * 8 + j % 8];
             } else {
-                load_query<D / 32>(a, at + g * 8, 32, x);
+                load_query<D / 32>(a, at + g * 8, 32, e);
+                query_values<D / 32>(a, e, x);
             }
         }
         float top = 0.0f;
@@ -424,6 +429,13 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) attend_many_kernel(K
     if (part >= sp.parts) return;
     const int page0 = sp.lo + part * a.chunk, page1 = min(page0 + a.chunk, sp.hi);
 
+    // the row of this lane's column, and what the wave's first and last row see; its queries are on their way while the page
+    // numbers are read, and the first pages' bytes while the queries are converted
+    const int in = over + wave * 32 + col, i = i_first + in / a.group, hq = head * a.group + in % a.group;
+    const bool on = i < s.m;
+    uint16_t raw[kSteps][8] = {};
+    if (on) load_query<kSteps>(a, (int64_t)(s.r0 + i) * a.q_row + hq * a.q_head + h * 8, 16, raw);
+
     // numbers and scales of the pages from `base` on, one a lane; a page that does not exist is page 0 with a NaN scale of K, and its
     // V is masked: rows that do not see it stay clean
     int base = page0, ids = 0;
@@ -481,23 +493,20 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) attend_many_kernel(K
     };
     _Float16* const k_buf = lds;
     _Float16* const v_buf = lds + kBufs * kKBuf;
-    if (page0 < page1) {  // the first pages' bytes are on their way while the queries are read
+    uint4 k_first[kBufs][kLoads], v_first[kBufs][kLoads];
+    if (page0 < page1) {
         look(page0);
-        load(kr, c.k, page0);
-        load(vr, c.v, page0);
+#pragma unroll
+        for (int p = 0; p < kBufs; p++) {
+            load(k_first[p], c.k, page0 + p);
+            if (p + 1 < kBufs) load(v_first[p], c.v, page0 + p);
+        }
     }
-
-    // the row of this lane's column, and what the wave's first and last row see
-    const int in = over + wave * 32 + col, i = i_first + in / a.group, hq = head * a.group + in % a.group;
-    const bool on = i < s.m;
     f16x8 q[kSteps];
     float qs;
     {
-        float x[D / 2];
-#pragma unroll
-        for (int j = 0; j < D / 2; j++) x[j] = 0.0f;
-        if (on) load_query<kSteps>(a, (int64_t)(s.r0 + i) * a.q_row + hq * a.q_head + h * 8, 16, x);
-        float top = 0.0f;
+        float x[D / 2], top = 0.0f;
+        query_values<kSteps>(a, raw, x);
 #pragma unroll
         for (int j = 0; j < D / 2; j++) top = fmaxf(top, fabsf(x[j]));
         top = other_half(top, true);
@@ -538,6 +547,7 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) attend_many_kernel(K
         const int after = next_side(side);
         const _Float16 *kb = k_buf + after * kKBuf, *vb = v_buf + side * kVBuf;
         if (page + kBufs + 1 - base > 63) look(page);
+        if constexpr (kApart) __builtin_amdgcn_s_setprio(1);  // this half takes longer than the other waves' second product
         f16x8 f[kAhead];
 #pragma unroll
         for (int n = 0; n < kAhead; n++) f[n] = operand(n, kb, vb);
@@ -587,7 +597,10 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) attend_many_kernel(K
             __builtin_amdgcn_sched_barrier(0);
         }
         rs.l = fmaf(sum, w, rs.l);
-        if constexpr (kApart) __syncthreads();
+        if constexpr (kApart) {
+            __builtin_amdgcn_s_setprio(0);
+            __syncthreads();
+        }
         mask_v(page + kBufs - 1);
         constexpr int kPieces = 4 * kLoads;
         _Float16 *k_to = k_buf + side * kKBuf, *v_to = v_buf + (side == 0 ? kBufs - 1 : side - 1) * kVBuf;
@@ -609,13 +622,15 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) attend_many_kernel(K
     if (page0 < page1) {
         f32x16 sa[2], sb[2];
 #pragma unroll
-        for (int p = 0; p < kBufs; p++) {  // K of the first kBufs pages, V of one less, and the next ones' bytes
-            mask_v(page0 + p);
+        for (int p = 0; p < kBufs; p++) {  // K of the first kBufs pages, V of one less
+#pragma unroll
+            for (int j = 0; j < kLoads; j++) kr[j] = k_first[p][j], vr[j] = v_first[p][j];
+            if (p + 1 < kBufs) mask_v(page0 + p);
 #pragma unroll
             for (int n = 0; n < (p + 1 < kBufs ? 4 : 2) * kLoads; n++) unpack(n, k_buf + p * kKBuf, v_buf + p * kVBuf);
-            load(kr, c.k, page0 + p + 1);
-            if (p + 1 < kBufs) load(vr, c.v, page0 + p + 1);
         }
+        load(kr, c.k, page0 + kBufs);
+        load(vr, c.v, page0 + kBufs - 1);
         __syncthreads();
 #pragma unroll
         for (int t = 0; t < 2; t++)
