@@ -107,25 +107,49 @@ __device__ __forceinline__ uint32_t pack4(f32x4 x) {
     }
 }
 
+// The same for numbers that are finite and at most the largest stored one (and a rounding): int8 by adding 1.5 x 2^23, whose sum
+// has the nearest even integer in its low bits.
+template <int CT>
+__device__ __forceinline__ uint32_t pack4_finite(f32x4 x) {
+    if constexpr (CT == KK_KV_E4M3) {
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
+    } else {
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+#pragma clang fp contract(off)
+            const float r = x[i] + 12582912.0f;
+            u[i] = __float_as_uint(r);
+        }
+        const uint32_t a = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u), b = __builtin_amdgcn_perm(u[3], u[2], 0x0c0c0400u);
+        return __builtin_amdgcn_perm(b, a, 0x05040100u);
+    }
+}
+
 // ------------------------------------------------------------------ values in 16 and 32 bits
 
+// `mask`: of a value's bits without its sign, whose order is that of the sizes; from `inf` on they are no numbers.
 template <int T>
 struct ElemOf;
 template <>
 struct ElemOf<KK_BF16> {
     typedef uint16_t type;
+    static constexpr uint32_t mask = 0x7fff, inf = 0x7f80;
     static __device__ __forceinline__ float load(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
     static __device__ __forceinline__ uint16_t store(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
 };
 template <>
 struct ElemOf<KK_F16> {
     typedef uint16_t type;
+    static constexpr uint32_t mask = 0x7fff, inf = 0x7c00;
     static __device__ __forceinline__ float load(uint16_t v) { return (float)__builtin_bit_cast(_Float16, v); }
     static __device__ __forceinline__ uint16_t store(float f) { return __builtin_bit_cast(uint16_t, (_Float16)f); }
 };
 template <>
 struct ElemOf<KK_F32> {
     typedef float type;
+    static constexpr uint32_t mask = 0x7fffffff, inf = 0x7f800000;
     static __device__ __forceinline__ float load(float v) { return v; }
     static __device__ __forceinline__ float store(float f) { return f; }
 };

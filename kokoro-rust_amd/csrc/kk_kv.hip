@@ -9,11 +9,10 @@
 namespace kk {
 namespace {
 
-// The page that a block works on; its number in the cache, or -1 for one that does not exist.
+// The page that a block works on.
 template <int THREADS>
-__device__ __forceinline__ bool kv_page(const KvCacheDev& c, const KvBatchDev& B, int per_seq, bool report, KvPage& p,
-                                        int& page, int* found) {
-    KvSeq s;
+__device__ __forceinline__ bool kv_page(const KvCacheDev& c, const KvBatchDev& B, int per_seq, bool report, KvSeq& s, KvPage& p,
+                                        int* found) {
     int i;
     if (per_seq) {
         const int b = blockIdx.x / per_seq;
@@ -30,12 +29,14 @@ __device__ __forceinline__ bool kv_page(const KvCacheDev& c, const KvBatchDev& B
         if (report && threadIdx.x == 0 && s.m > s.len) kv_fault(c, KK_KV_BAD_BATCH);
         return false;
     }
-    page = B.table[s.b * B.stride + p.at];
-    if (page < 0 || page >= c.pages) {
-        if (report && threadIdx.x == 0) kv_fault(c, KK_KV_BAD_PAGE);
-        page = -1;
-    }
     return true;
+}
+
+// Its number in the cache, or -1 for one that does not exist.
+__device__ __forceinline__ int kv_page_id(const KvCacheDev& c, int id, bool report) {
+    if (id >= 0 && id < c.pages) return id;
+    if (report && threadIdx.x == 0) kv_fault(c, KK_KV_BAD_PAGE);
+    return -1;
 }
 
 // 4 x 4 bytes transposed: o[i] byte j = w[j] byte i.
@@ -58,50 +59,99 @@ __device__ __forceinline__ uint32_t byte_mask(int first, int lo, int hi) {  // b
 
 constexpr int kKvThreads = 256;
 
+template <class E>
+__device__ __forceinline__ E bits_of(uint32_t u) {
+    if constexpr (sizeof(E) == 4)
+        return __uint_as_float(u);
+    else
+        return (E)u;
+}
+
+// The largest of a thread's values by their bits without signs, of those below `limit`.
+template <int T, int N>
+__device__ __forceinline__ uint32_t raw_max(const typename ElemOf<T>::type (*raw)[8], uint32_t limit) {
+    if constexpr (T == KK_F32) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < N; j++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const uint32_t u = __float_as_uint(raw[j][i]) & ElemOf<T>::mask;
+                m = max(m, u < limit ? u : 0u);
+            }
+        return m;
+    } else {
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+        u16x2 m = {0, 0};
+#pragma unroll
+        for (int j = 0; j < N; j++)
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                u16x2 u = {(uint16_t)(raw[j][i] & ElemOf<T>::mask), (uint16_t)(raw[j][i + 1] & ElemOf<T>::mask)};
+                if (limit != ~0u) u = u16x2{u[0] < limit ? u[0] : (uint16_t)0, u[1] < limit ? u[1] : (uint16_t)0};
+                m = __builtin_elementwise_max(m, u);
+            }
+        return max((uint32_t)m[0], (uint32_t)m[1]);
+    }
+}
+
+// The largest over the block's threads; `words`: one of LDS a wave, not used by anything before.
+__device__ __forceinline__ uint32_t block_max(uint32_t m, uint32_t* words) {
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, k));
+    if ((threadIdx.x & 63) == 0) words[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = words[0];
+#pragma unroll
+    for (int i = 1; i < kKvThreads / 64; i++) m = max(m, words[i]);
+    return m;
+}
+
 template <int T, int CT, int D>
 __global__ void __launch_bounds__(kKvThreads) kv_write_kernel(KvCacheDev c, KvBatchDev B, KvRowsDev R, int per_seq) {
     constexpr int kChunks = D / 8, kMine = kPage * kChunks / kKvThreads;  // 8-value chunks of a token, of a thread
     constexpr int kLd = D + 4;                                           // bytes of a token's row in LDS
     __shared__ int found[2];
-    __shared__ float wave_top[kKvThreads / 64];
+    __shared__ uint32_t block_top[2 * kKvThreads / 64];
     __shared__ uint32_t lds[kPage * kLd / 4];
     const int head = blockIdx.y >> 1, is_v = blockIdx.y & 1, tid = threadIdx.x;
+    KvSeq s;
     KvPage p;
-    int id;
-    if (!kv_page<kKvThreads>(c, B, per_seq, blockIdx.y == 0, p, id, found) || id < 0) return;
-    float* scale_at = (is_v ? c.vs : c.ks) + (int64_t)id * c.heads + head;
-    const float scale_was = p.lo ? *scale_at : 0.0f;
+    if (!kv_page<kKvThreads>(c, B, per_seq, blockIdx.y == 0, s, p, found)) return;
+    int id = B.table[s.b * B.stride + p.at];  // used behind the loads of the new tokens
     const void* src = is_v ? R.v : R.k;
     const int64_t row_step = is_v ? R.v_row : R.k_row, head_step = is_v ? R.v_head : R.k_head;
     const bool vec = is_v ? R.v_vec : R.k_vec;
-    uint8_t* page = (is_v ? c.v : c.k) + ((int64_t)id * c.heads + head) * (kPage * D);
-
-    float x[kMine][8];
-    float top = 0.0f;
+    // every load before the first is used: threads whose slot is not written load the nearest one that is, and drop it
+    typedef typename ElemOf<T>::type E;
+    E raw[kMine][8];
+    const E* from = (const E*)src + head * head_step;
 #pragma unroll
     for (int j = 0; j < kMine; j++) {
         const int slot = (tid + j * kKvThreads) / kChunks, ch = (tid + j * kKvThreads) % kChunks;
-        if (slot >= p.lo && slot < p.hi) {
-            load_values<T, 8>(src, (p.row0 + slot - p.lo) * row_step + head * head_step + ch * 8, vec, x[j]);
+        const E* q = from + (p.row0 + min(max(slot, p.lo), p.hi - 1) - p.lo) * row_step + ch * 8;
+        if (vec) {
+#pragma unroll
+            for (int i = 0; i < 8; i += 16 / (int)sizeof(E)) {
+                const uint4 w = *(const uint4*)(q + i);
+                __builtin_memcpy(&raw[j][i], &w, 16);
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[j][i] = 0.0f;
+            for (int i = 0; i < 8; i++) raw[j][i] = q[i];
         }
     }
-#pragma unroll
-    for (int j = 0; j < kMine; j++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float m = fabsf(x[j][i]);
-            top = fmaxf(top, m <= 3.402823466e38f ? m : 0.0f);  // NaN and infinities do not count
-        }
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
-    if ((tid & 63) == 0) wave_top[tid >> 6] = top;
-    __syncthreads();
-    top = wave_top[0];
-#pragma unroll
-    for (int i = 1; i < kKvThreads / 64; i++) top = fmaxf(top, wave_top[i]);
+    id = kv_page_id(c, id, blockIdx.y == 0);
+    if (id < 0) return;
+    float* scale_at = (is_v ? c.vs : c.ks) + (int64_t)id * c.heads + head;
+    const float scale_was = p.lo ? *scale_at : 0.0f;
+    uint8_t* page = (is_v ? c.v : c.k) + ((int64_t)id * c.heads + head) * (kPage * D);
+    // The largest size, on the bits: two instructions for two values in 16 bits.  The other slots' threads hold values that are
+    // written too and change nothing.  A block that holds infinities or NaN finds it again without them.
+    const uint32_t most = block_max(raw_max<T, kMine>(raw, ~0u), block_top);
+    const bool finite = most < ElemOf<T>::inf;
+    const uint32_t top_bits = finite ? most : block_max(raw_max<T, kMine>(raw, ElemOf<T>::inf), block_top + kKvThreads / 64);
+    const float top = sizeof(E) == 4 ? __uint_as_float(top_bits) : ElemOf<T>::load(bits_of<E>(top_bits));
 
     const float want = top > 0.0f ? fmaxf(top * (CT == KK_KV_E4M3 ? 1.0f / 448.0f : 1.0f / 127.0f), kScaleLeast) : 0.0f;
     const float scale = fmaxf(scale_was, want);
@@ -112,9 +162,10 @@ __global__ void __launch_bounds__(kKvThreads) kv_write_kernel(KvCacheDev c, KvBa
 #pragma unroll
     for (int j = 0; j < kMine; j++) {
         const int slot = (tid + j * kKvThreads) / kChunks, ch = (tid + j * kKvThreads) % kChunks;
-        uint2 w;
-        w.x = pack4<CT>(f32x4{x[j][0] * inv, x[j][1] * inv, x[j][2] * inv, x[j][3] * inv});
-        w.y = pack4<CT>(f32x4{x[j][4] * inv, x[j][5] * inv, x[j][6] * inv, x[j][7] * inv});
+        f32x4 lo, hi;
+#pragma unroll
+        for (int i = 0; i < 4; i++) lo[i] = ElemOf<T>::load(raw[j][i]) * inv, hi[i] = ElemOf<T>::load(raw[j][4 + i]) * inv;
+        const uint2 w = finite ? uint2{pack4_finite<CT>(lo), pack4_finite<CT>(hi)} : uint2{pack4<CT>(lo), pack4<CT>(hi)};
         if (is_v) {
             lds[slot * (kLd / 4) + ch * 2] = w.x;
             lds[slot * (kLd / 4) + ch * 2 + 1] = w.y;
@@ -182,9 +233,10 @@ __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(KvCacheDev c, KvBat
     __shared__ int found[2];
     __shared__ uint32_t lds[kPage * kLd / 4];
     const int head = blockIdx.y >> 1, is_v = blockIdx.y & 1, tid = threadIdx.x;
+    KvSeq s;
     KvPage p;
-    int id;
-    if (!kv_page<kKvThreads>(c, B, per_seq, blockIdx.y == 0, p, id, found)) return;
+    if (!kv_page<kKvThreads>(c, B, per_seq, blockIdx.y == 0, s, p, found)) return;
+    const int id = kv_page_id(c, B.table[s.b * B.stride + p.at], blockIdx.y == 0);
     const bool bad = id < 0;
     const int64_t at = (int64_t)(bad ? 0 : id) * c.heads + head;
     const float scale = bad ? __uint_as_float(0x7fc00000u) : (is_v ? c.vs : c.ks)[at];

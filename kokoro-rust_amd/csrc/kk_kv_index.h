@@ -34,7 +34,7 @@ __host__ __device__ inline bool kv_seq(const KvBatchDev& B, int b, KvSeq& s) {
     const int64_t m = (int64_t)B.row_start[b + 1] - s.r0;
     s.len = B.len[b];
     s.m = (int)m;
-    return s.r0 >= 0 && m >= 0 && m <= B.max_new && s.r0 + m <= B.rows && s.len >= 0 && s.len <= B.max_len;
+    return (s.r0 >= 0) & (m >= 0) & (m <= B.max_new) & (s.r0 + m <= B.rows) & (s.len >= 0) & (s.len <= B.max_len);
 }
 
 // A sequence with m rows has at most m G / M + E tiles of M (E = 1 for tiles of its own rows, 2 for pages, where the first
