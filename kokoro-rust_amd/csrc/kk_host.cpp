@@ -94,6 +94,7 @@ std::string kv_attention_error(const kk_kv_cache* c, const kk_kv_batch* b, const
     if (a->window && !a->causal) return "a window needs causal";
     if (b->n == 0 || b->rows == 0 || b->max_new == 0) return "";
     if (!a->q || !a->out) return "null array";
+    if (a->q == a->out) return "the output is the queries' array";
     if (!aligned(a->q, 2) || !aligned(a->out, 2)) return "an array is not aligned to its values";
     return "";
 }

@@ -103,9 +103,7 @@ struct PageIn {
     float k_scale, v_scale;
     int live;  // slots that hold tokens of the sequence: the bytes of V behind them, which may be the NaN code, are masked
 };
-__device__ __forceinline__ PageIn page_in(const KvCacheDev& c, const KvBatchDev& B, const KvSeq& s, int page, int head,
-                                          bool report) {
-    int id = __builtin_amdgcn_readfirstlane(B.table[s.b * B.stride + page]);
+__device__ __forceinline__ PageIn page_in(const KvCacheDev& c, const KvSeq& s, int page, int id, int head, bool report) {
     const bool bad = id < 0 || id >= c.pages;
     if (bad) {
         if (report) kv_fault(c, KK_KV_BAD_PAGE);
@@ -167,6 +165,10 @@ attend_few_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
     const int part = rest / B.n, b = rest % B.n;  // parts that only long sequences have come last: few blocks end empty meanwhile
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
+    auto number = [&](int page) { return __builtin_amdgcn_readfirstlane(B.table[b * B.stride + page]); };
+    // without a window the wave's first page is known before the sequence's length: its number is loaded beside that
+    const int guess = part * a.chunk + wave;
+    const int early = !a.window && guess < B.width ? B.table[b * B.stride + guess] : 0;
     KvSeq s;
     if (!kv_seq(B, b, s)) {
         if (threadIdx.x == 0 && head == 0 && part == 0) kv_fault(c, KK_KV_BAD_BATCH);
@@ -198,7 +200,7 @@ attend_few_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
     int page = page0 + wave;
     PageIn now;
     if (page < page1) {
-        now = page_in(c, B, s, page, head, report);
+        now = page_in(c, s, page, a.window ? number(page) : __builtin_amdgcn_readfirstlane(early), head, report);
         load_k(now);
     }
 
@@ -286,7 +288,7 @@ attend_few_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
         const PageIn p = now;
         page += W;
         if (page < page1) {
-            now = page_in(c, B, s, page, head, report);
+            now = page_in(c, s, page, number(page), head, report);
             load_k(now);
         }
         const bool whole = t0 >= all_lo && t0 + kPage <= all_hi;

@@ -109,6 +109,24 @@ def test_write_special_values(ctx, cache_kind):
         assert torch.equal(o.cpu(), cache.tokens([2], 7, part).float())
 
 
+@pytest.mark.parametrize("cache_kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("kind", ["bf16", "f16", "f32"])
+def test_write_beside_infinities(ctx, cache_kind, kind):
+    """Infinities and NaN in some heads of a page that is written in two calls, none in the others; values that round to the
+    largest number of their type; ties of the 8-bit rounding."""
+    cache = R.Cache(cache_kind, 3, 96, 3)
+    g = torch.Generator().manual_seed(7)
+    x = torch.randn(80, 3, 96, generator=g)
+    x[:, 2] = torch.randint(-254, 255, (80, 96), generator=g) / 2.0  # halves in units of a scale of 1
+    x[0, 2, 0] = x[70, 2, 1] = 127.0
+    x[3, 0, 5], x[4, 0, 6], x[70, 0, 7], x[50, 1, 9] = np.inf, -np.inf, np.nan, torch.finfo(R.TYPES[kind]).max
+    x = x.to(R.TYPES[kind]).cuda()
+    for start, n in ((0, 30), (30, 40), (70, 10)):
+        batch = R.Batch([n], [start + n], [[2, 0]], max_len=100, width=2)
+        R.write(ctx, cache, batch, x[start:start + n], -x[start:start + n], _code(kind))
+        cache.same()
+
+
 @pytest.mark.parametrize("n, most", [(90, 1), (40, 9), (3, 2000)])
 def test_write_many_sequences(ctx, n, most):
     """Batches on both ways of finding a block's page (each sequence's pages, and a search), ragged, some without rows; packed

@@ -101,7 +101,7 @@ def test_rows_refusals(kw, word):
     (dict(type=3), "type"), (dict(heads=0), "multiple"), (dict(heads=7), "multiple"), (dict(heads=8192), "multiple"),
     (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("inf")), "scale"), (dict(causal=2), "causal"),
     (dict(window=-1), "window"), (dict(window=(1 << 30) + 1), "window"), (dict(window=5, causal=0), "causal"),
-    (dict(q=None), "null"), (dict(out=None), "null"), (dict(q=P + 1), "aligned")])
+    (dict(q=None), "null"), (dict(out=None), "null"), (dict(q=P + 1), "aligned"), (dict(out=8 * P), "queries")])
 def test_attention_refusals(kw, word):
     from kokoro_hip import api
     for name in ("kk_kv_attention", "kk_kv_attention_workspace"):
