@@ -74,18 +74,30 @@ __device__ __forceinline__ void load_query(const AttnDev& a, int64_t at, int ste
 }
 template <int P>
 __device__ __forceinline__ void query_values(const AttnDev& a, const uint16_t (*e)[8], float* x) {
+    // a branch, not a choice for each value: code that runs once costs the time to fetch it
+    if (a.type == KK_BF16) {
 #pragma unroll
-    for (int j = 0; j < P; j++)
+        for (int j = 0; j < P; j++)
 #pragma unroll
-        for (int k = 0; k < 8; k++)
-            x[8 * j + k] = a.type == KK_BF16 ? ElemOf<KK_BF16>::load(e[j][k]) : ElemOf<KK_F16>::load(e[j][k]);
+            for (int k = 0; k < 8; k++) x[8 * j + k] = ElemOf<KK_BF16>::load(e[j][k]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < P; j++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) x[8 * j + k] = ElemOf<KK_F16>::load(e[j][k]);
+    }
 }
 
 // Four values of a row, next to each other, behind a division by l (or as a part's).
 __device__ __forceinline__ void store_out4(const AttnDev& a, int64_t at, const float* x) {
     uint16_t e[4];
+    if (a.type == KK_BF16) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) e[i] = a.type == KK_BF16 ? ElemOf<KK_BF16>::store(x[i]) : ElemOf<KK_F16>::store(x[i]);
+        for (int i = 0; i < 4; i++) e[i] = ElemOf<KK_BF16>::store(x[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) e[i] = ElemOf<KK_F16>::store(x[i]);
+    }
     uint16_t* p = (uint16_t*)a.out + at;
     if (a.out_vec) {
         uint2 w;
@@ -179,6 +191,21 @@ attend_few_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
     if (part >= sp.parts) return;
     const int page0 = sp.lo + part * a.chunk, page1 = min(page0 + a.chunk, sp.hi);
 
+    // the rows of this lane's columns: their queries are loaded first, so that they are there while K is on its way
+    uint16_t raw[NT][D / 32][8] = {};
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const int r = n * 16 + col, i = r / a.group;
+        if (i >= s.m) continue;
+        const int64_t at = (int64_t)(s.r0 + i) * a.q_row + (head * a.group + r % a.group) * a.q_head;
+        if constexpr (kWide) {  // 16 values of each 64 a lane: the two halves of 8 apart
+            load_query<D / 64>(a, at + g * 16, 64, raw[n]);
+            load_query<D / 64>(a, at + g * 16 + 8, 64, raw[n] + D / 64);
+        } else {
+            load_query<D / 32>(a, at + g * 8, 32, raw[n]);
+        }
+    }
+
     uint4 kr[4][kLoads];
     auto load_k = [&](const PageIn& p) {
         const uint8_t* base = c.k + p.at * (kPage * D);
@@ -204,32 +231,17 @@ attend_few_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
         load_k(now);
     }
 
-    // the rows of this lane's columns: queries and the tokens [lo, hi) that they see
     f16x8 q[NT][kSteps];
     float qs[NT];
-    int lo[NT], hi[NT];
+    int lo[NT], hi[NT];  // the tokens that a row sees
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         const int r = n * 16 + col, i = r / a.group;
         const bool on = i < s.m;
-        float x[D / 4];
+        float x[D / 4], y[D / 4];
+        query_values<D / 32>(a, raw[n], y);
 #pragma unroll
-        for (int j = 0; j < D / 4; j++) x[j] = 0.0f;
-        if (on) {
-            const int64_t at = (int64_t)(s.r0 + i) * a.q_row + (head * a.group + r % a.group) * a.q_head;
-            uint16_t e[D / 32][8];
-            if constexpr (kWide) {  // 16 values of each 64 a lane: the two halves of 8 apart
-                float y[D / 4];
-                load_query<D / 64>(a, at + g * 16, 64, e);
-                load_query<D / 64>(a, at + g * 16 + 8, 64, e + D / 64);
-                query_values<D / 32>(a, e, y);
-#pragma unroll
-                for (int j = 0; j < D / 4; j++) x[j] = y[(j / 8 & 1) * (D / 8) + j / 16 * 8 + j % 8];
-            } else {
-                load_query<D / 32>(a, at + g * 8, 32, e);
-                query_values<D / 32>(a, e, x);
-            }
-        }
+        for (int j = 0; j < D / 4; j++) x[j] = kWide ? y[(j / 8 & 1) * (D / 8) + j / 16 * 8 + j % 8] : y[j];
         float top = 0.0f;
 #pragma unroll
         for (int j = 0; j < D / 4; j++) top = fmaxf(top, fabsf(x[j]));
