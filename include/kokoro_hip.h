@@ -359,7 +359,7 @@ typedef struct {
  * in page table[b][t / 64], slot t % 64.  max_new and max_len bound the rows and the tokens of any sequence;
  * they size the launch.  Rows outside all sequences are neither read nor written.
  * Checked on the device: a sequence whose rows leave [0, rows), exceed max_new, or whose len leaves [0, max_len]
- * is left out (KK_KV_BAD_BATCH; the table is not read); a page number outside [0, pages) is not accessed: nothing
+ * is left out (KK_KV_BAD_BATCH; no page of it is accessed); a page number outside [0, pages) is not accessed: nothing
  * is written there, and what is read there is NaN (KK_KV_BAD_PAGE). */
 #define KK_KV_BAD_BATCH 1
 #define KK_KV_BAD_PAGE 2
@@ -422,7 +422,7 @@ typedef struct {
     size_t workspace_bytes;
 } kk_kv_attention_args;
 /* The workspace that kk_kv_attention needs for these arguments (0: none), or negative KK_ERR_* for arguments that it would
- * refuse.  It depends on n, rows, max_new, max_len, heads, dim and window alone. */
+ * refuse.  It depends on n, rows, max_new, max_len, both head counts, dim, window and the device's compute units alone. */
 int64_t kk_kv_attention_workspace(kk_ctx* ctx, const kk_kv_cache* cache, const kk_kv_batch* batch,
                                   const kk_kv_attention_args* args, char* err, size_t errlen);
 int kk_kv_attention(kk_ctx* ctx, const kk_kv_cache* cache, const kk_kv_batch* batch, const kk_kv_attention_args* args,

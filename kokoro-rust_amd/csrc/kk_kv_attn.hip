@@ -178,9 +178,10 @@ attend_few_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
     auto number = [&](int page) { return __builtin_amdgcn_readfirstlane(B.table[b * B.stride + page]); };
-    // without a window the wave's first page is known before the sequence's length: its number is loaded beside that
+    // without a window the wave's first page is known before the sequence's length: its number is loaded beside that (the table
+    // holds max_len tokens of every sequence; where max_len is 0 there may be none)
     const int guess = part * a.chunk + wave;
-    const int early = !a.window && guess < B.width ? B.table[b * B.stride + guess] : 0;
+    const int early = !a.window && (int64_t)guess * kPage < B.max_len ? B.table[b * B.stride + guess] : 0;
     KvSeq s;
     if (!kv_seq(B, b, s)) {
         if (threadIdx.x == 0 && head == 0 && part == 0) kv_fault(c, KK_KV_BAD_BATCH);

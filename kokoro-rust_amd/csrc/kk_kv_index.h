@@ -17,10 +17,10 @@ constexpr int kMostParts = 256;  // of the token axis
 struct KvBatchDev {
     const int32_t *row_start, *len, *table;
     int64_t stride;
-    int n, rows, max_new, max_len, width;
+    int n, rows, max_new, max_len;
 };
 inline KvBatchDev kv_dev(const kk_kv_batch& b) {
-    return {b.row_start, b.len, b.table, b.table_stride, b.n, b.rows, b.max_new, b.max_len, b.table_width};
+    return {b.row_start, b.len, b.table, b.table_stride, b.n, b.rows, b.max_new, b.max_len};
 }
 
 struct KvSeq {

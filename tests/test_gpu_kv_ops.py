@@ -595,3 +595,16 @@ def test_nothing_to_do(ctx):
         ctx.kv_attention(cache.args, batch.args, args)
     cache.same()
     assert not q.any() and int(cache.fault) == 0
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_no_tokens_and_no_table(ctx, new):
+    """max_len 0 needs no page table, whatever its width says: rows that see nothing give zeros."""
+    cache, _ = _filled(ctx, "int8", 1, 64, [10], 4)
+    batch = R.Batch([new], [0], [[]], max_len=0, width=4)
+    batch.args.table = None
+    q = torch.ones(new, 1, 64, dtype=torch.float16, device="cuda")
+    out = torch.ones_like(q)
+    args, _ = R.attention_args(ctx, cache, batch, q, out, _code("f16"), 0.1)
+    ctx.kv_attention(cache.args, batch.args, args)
+    assert not out.any() and int(cache.fault) == 0
