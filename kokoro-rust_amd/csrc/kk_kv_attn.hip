@@ -692,15 +692,14 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) attend_many_kernel(K
 
 // ------------------------------------------------------------------ the parts joined
 
-// out = sum_p 2^{m_p - m} O_p / sum_p 2^{m_p - m} l_p for each (row, head), by J waves that take every J-th part: one where there
-// are few parts, four where there are many.  Bound by the latency of three dependent loads (the sequence, m, O).
-template <int D, int J>
+// out = sum_p 2^{m_p - m} O_p / sum_p 2^{m_p - m} l_p, a wave for each (row, head).  Bound by the latency of three dependent
+// loads (the sequence, m, O).
+template <int D>
 __global__ void __launch_bounds__(256) attend_join_kernel(KvBatchDev B, AttnDev a) {
     constexpr int N = (D + 63) / 64;
-    __shared__ float lds[J][64 * N + 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t w = J == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
-    const int row = (int)(w / a.heads), hq = (int)(w % a.heads), p0 = J == 1 ? 0 : wave;
+    const int64_t w = (int64_t)blockIdx.x * 4 + wave;
+    const int row = (int)(w / a.heads), hq = (int)(w % a.heads);
     if (row >= B.rows) return;
     KvSeq s;
     bool have = false;
@@ -732,25 +731,12 @@ __global__ void __launch_bounds__(256) attend_join_kernel(KvBatchDev B, AttnDev 
     for (int k = 0; k < N; k++) x[k] = 0.0f;
     const int dim = min(lane, D - 1 - 64 * (N - 1));  // of the last 64 values
 #pragma unroll 8
-    for (int p = p0; p < sp.parts; p += J) {
+    for (int p = 0; p < sp.parts; p++) {
         const float2 ml = a.ml[at + p];
         const float f = __builtin_amdgcn_exp2f(ml.x - ref);
         l = fmaf(ml.y, f, l);
 #pragma unroll
         for (int k = 0; k < N; k++) x[k] = fmaf(a.acc[(at + p) * D + (k < N - 1 ? lane : dim) + 64 * k], f, x[k]);
-    }
-    if constexpr (J > 1) {
-#pragma unroll
-        for (int k = 0; k < N; k++) lds[wave][lane + 64 * k] = x[k];
-        if (lane == 0) lds[wave][64 * N] = l;
-        __syncthreads();
-        if (wave != 0) return;
-#pragma unroll
-        for (int j = 1; j < J; j++) {
-            l += lds[j][64 * N];
-#pragma unroll
-            for (int k = 0; k < N; k++) x[k] += lds[j][lane + 64 * k];
-        }
     }
     const float inv = 1.0f / l;
     uint16_t* out = (uint16_t*)a.out + row * a.out_row + hq * a.out_head;
@@ -779,8 +765,7 @@ hipError_t run(const kk_kv_cache& c, const kk_kv_batch& b, const AttnPlan& p, co
         rc = launch(attend_few_kernel<D, CT, 2, 4>, grid, dim3(256), 0, s, cd, bd, a);
     if (rc != hipSuccess || p.parts == 1) return rc;
     const int64_t sums = (int64_t)b.rows * a.heads;
-    if (p.parts > 16) return launch(attend_join_kernel<D, 4>, dim3((unsigned)sums), dim3(256), 0, s, bd, a);
-    return launch(attend_join_kernel<D, 1>, dim3((unsigned)ceil_div(sums, 4)), dim3(256), 0, s, bd, a);
+    return launch(attend_join_kernel<D>, dim3((unsigned)ceil_div(sums, 4)), dim3(256), 0, s, bd, a);
 }
 
 }  // namespace

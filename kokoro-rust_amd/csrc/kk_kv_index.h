@@ -58,7 +58,8 @@ inline KvTiles kv_tiles(const kk_kv_batch& b) {
     const int64_t per = b.max_new < 2 ? 1 : (b.max_new - 2) / kPage + 2;  // pages that max_new rows can touch
     const int64_t flat = b.rows / kPage + 2 * (int64_t)b.n;
     // A ragged batch of few long and many short sequences would start mostly empty blocks for the longest one's pages; an even
-    // one needs no search.
+    // one needs no search.  Measured, writing and reading back, us flat against per sequence: two of 8,000 rows among 512 of one 83
+    // and 1,106; 64 of one row 13.9 and 11.8.
     if (per * b.n <= 2 * flat) return {(int)per, per * b.n};
     return {0, flat};
 }
@@ -102,7 +103,7 @@ __host__ __device__ inline Span span_of(const KvSeq& s, bool causal, int window,
 struct AttnPlan {
     bool few;         // at most kFewRows rows of a (sequence, cache head)
     int row_tiles;    // few: 16-row tiles of a block (1 or 2)
-    int waves;        // few: of a block, 8 while its blocks leave CUs idle, else 4
+    int waves;        // few: of a block, 8 or 4
     int tile_rows;    // rows of a block: many, 256 where that fills the device, or 128
     int64_t tiles;    // blocks along the rows
     int chunk, parts; // pages of a part, parts of the axis
@@ -113,12 +114,21 @@ inline AttnPlan attention_plan(const kk_kv_cache& c, const kk_kv_batch& b, const
     const int64_t group = a.heads / c.heads, rows = b.max_new * group;
     p.few = rows <= kFewRows;
     p.row_tiles = rows <= 16 ? 1 : 2;
-    p.tile_rows = p.few ? 16 * p.row_tiles : c.dim <= 128 && (b.rows * group / 256 + b.n) * c.heads >= n_cu ? 256 : 128;
+    // tiles of M rows, about: each sequence's last one is half full
+    auto about = [&](int M) {
+        return std::max<int64_t>(b.n == 1 ? (b.rows * group + M - 1) / M : b.rows * group / M + b.n / 2, 1);
+    };
+    // pages that a row sees, about
+    auto seen = [&](int64_t pages) { return a.causal && !a.window ? pages - b.max_new / (2 * kPage) : pages; };
+    // Many rows: 256 a block cost the matrix cores 5% less than 2 x 128 (four prompts of 512 rows behind 8,000 tokens 275 against 295
+    // us, one prompt of 4,096 158 against 169), where they fill the device and see enough pages; else the finer blocks end
+    // sooner (a prompt of 2,048 57 against 67, 32 prompts of 512 155 against 178, a prompt of 2,500 72 against 80).
+    p.tile_rows = p.few ? 16 * p.row_tiles : c.dim <= 128 && about(256) * c.heads >= n_cu && seen(b.max_len / kPage) >= 24 ? 256 : 128;
     p.tiles = p.few ? b.n : b.rows * group / p.tile_rows + b.n;
     int64_t pages = ((int64_t)b.max_len + kPage - 1) / kPage;
     if (a.window) {  // a block's rows stand at most that many tokens apart, and N tokens touch at most N / 64 + 2 pages
-        const int64_t seen = (int64_t)a.window + (p.few ? b.max_new : p.tile_rows / group + 1);
-        pages = std::min(pages, seen / kPage + 2);
+        const int64_t tokens = (int64_t)a.window + (p.few ? b.max_new : p.tile_rows / group + 1);
+        pages = std::min(pages, tokens / kPage + 2);
     }
     pages = std::max<int64_t>(pages, 1);
     const int64_t blocks = p.tiles * c.heads;
@@ -128,14 +138,27 @@ inline AttnPlan attention_plan(const kk_kv_cache& c, const kk_kv_batch& b, const
     // 32, 64, 128: one sequence of 8,000 tokens 11.2, 12.5, 15.1, 22.2, 34.9, 57.7; of 131,000: 66, 54, 52, 49, 48, 71; 64 of
     // 200 to 8,191: 123, 104, 97, 99, 107, 119; 64 of 8,191: 250, 210, 189, 177, 173, 164.  Up to 1,000 tokens one block's 8
     // waves, without a second launch, are as fast (11.5 against 11.8).
-    if (p.few)
+    // Many rows: as many parts as the device holds blocks of at once (two of 128 rows a CU at up to 128 values a head), of 3 pages
+    // or more, where the time of the pages saved (0.0094 us a value of the head: 1.2 us a page of 128) is more than the second
+    // kernel's 4 us and what the parts write and read.  Measured at 32 heads of 128 over 8, us whole against split: 16 rows behind
+    // 8,000 tokens 159 and 20, behind 64,000 1,210 and 52; 100 behind 8,000 162 and 37; two of 512 behind 8,000 235 and 178;
+    // where the rule does not split: 700 rows behind 700 36 and 48, 1,024 alone 30 and 46, 1,500 behind 8,000 270 and 281.
+    if (p.few) {
         chunk = pages <= 16 ? pages : std::min<int64_t>(std::max<int64_t>((pages * blocks + 2 * n_cu - 1) / (2 * n_cu), 4), 32);
-    else if (2 * blocks <= n_cu)
-        chunk = std::max<int64_t>(pages * blocks / n_cu, 16);
+    } else {
+        const int64_t fit = (p.tile_rows == 128 && c.dim <= 128 ? 2 : 1) * n_cu;  // blocks that the device holds at once
+        const int64_t full = about(p.tile_rows) * c.heads, parts = std::max<int64_t>((fit + full / 16) / full, 1);
+        const int64_t part = std::max<int64_t>((pages + parts - 1) / parts, 3);
+        const double saved = 0.0094 * c.dim * (double)(seen(pages) - part);
+        const double join = 4.0 + 2e-6 * c.dim * (double)((int64_t)b.rows * a.heads * ((pages + part - 1) / part));
+        if (part < pages && saved > join) chunk = part;
+    }
     chunk = std::max(chunk, (pages + kMostParts - 1) / kMostParts);
     p.parts = (int)((pages + chunk - 1) / chunk);
     p.chunk = (int)((pages + p.parts - 1) / p.parts);
     p.parts = (int)((pages + p.chunk - 1) / p.chunk);
+    // 8 waves where the blocks leave CUs idle and have the pages: 1,000 tokens of one sequence 10.5 us against 11.9 with 4, of 16
+    // 12.1 against 14.6; 4 where blocks share CUs (64 of 1,000: 24.8 against 27.3 with 8).
     p.waves = blocks * p.parts <= n_cu && p.chunk > 4 ? 8 : 4;
     if (p.parts > 1) p.ws_bytes = (int64_t)b.rows * a.heads * p.parts * (c.dim * (int64_t)sizeof(float) + 2 * (int64_t)sizeof(float));
     return p;
