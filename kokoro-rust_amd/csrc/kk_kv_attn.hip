@@ -164,6 +164,12 @@ struct RowSum {
 // lane group g's scores are those of tokens 16 g .. 16 g + 15 in order, the 16 bytes that it loads of each row of V.
 // K of the next page is loaded while this one's softmax and second product run, V while its first product runs.  The waves
 // leave their O, m and l in LDS, and after one barrier the block's threads join them.
+// Measured at 32 heads of 128 over 8: one token each of 64 conversations of 200 to 8,191 tokens (536 MB) 101 us and the join's
+// 4.7, 5.1 TB/s over both (a kernel that only reads reaches 6.0, nontemporal, as these loads are, 6.5; with plain ones this
+// kernel takes 4% longer, the drafts 8%); five drafts
+// behind 131,000 tokens (269 MB) 46 us, 5.9 TB/s, and 4.8; one token behind 500 8 us, a chain of about 15,000 cycles: the sequence
+// 2,000, page and queries 4,500, the one page 3,700, the join of the waves 5,500.  For 17 to 32 rows each operand of the
+// cache feeds two products.
 template <int D, int CT, int NT, int W>
 __global__ void __launch_bounds__(64 * W, D <= 192 && D * NT <= 256 ? 2 : 1)
 attend_few_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
@@ -416,6 +422,12 @@ attend_few_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
 // ([token][dim]), V by value ([dim][token]), rows padded by 16 bytes (16-byte reads of 8 lanes then cover all banks).  Within 32
 // tokens K's rows are stored so that a lane's 8 scores of one step are 8 tokens in order, as its 16 bytes of V hold them.
 // Page numbers and scales are read 64 pages at a time, one a lane.
+// Measured: four prompts of 4,096 tokens at 32 heads of 128 over 8 (550 GFLOP) 608-620 us, 887-904 TFLOP/s, 40% of the matrix
+// cores' rate at the 2.1 GHz that the device holds meanwhile: in the loop a SIMD takes 1,950 cycles for a wave's page, 1,024 of
+// them for its 32 products of 32 cycles; a block's start and end cost another 20,000, and half of what the diagonal's pages compute is masked.
+// Of 1,000 to 4,096 tokens (278 GFLOP) 329-372 us, 750-843 TFLOP/s.  Products and exponentials in turn made 703 TFLOP/s where
+// interleaved and half a page apart make 887.  64 rows a wave (half the reads of LDS) were slower, 575 against 740 then: the
+// accumulators no longer fit beside the operands and are moved.
 template <int D, int CT, int W>
 __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) attend_many_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
     constexpr int kRows = 32 * W, kThreads = 64 * W;
@@ -693,7 +705,8 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) attend_many_kernel(K
 // ------------------------------------------------------------------ the parts joined
 
 // out = sum_p 2^{m_p - m} O_p / sum_p 2^{m_p - m} l_p, a wave for each (row, head).  Bound by the latency of three dependent
-// loads (the sequence, m, O).
+// loads (the sequence, m, O): 4.7 us for 64 rows of 32 heads in 4 parts as for 5 rows in 64.  Four waves that share the parts were no
+// faster: one token behind 1,000,000 tokens, 256 parts, 338 us against 339.
 template <int D>
 __global__ void __launch_bounds__(256) attend_join_kernel(KvBatchDev B, AttnDev a) {
     constexpr int N = (D + 63) / 64;

@@ -9,6 +9,11 @@
 // before it works on the first, which hides the loads' latency without many waves.  The row's angles are computed once: lane i
 // takes pair i, pos * f_i / 2 pi in f64, its fraction to f32 and sincospi there (2^-24 of a turn at any position), and
 // the wave's lanes read theirs from LDS.
+//
+// Measured: 16,384 rows of 40 heads of 128 values in 16 bits, 336 MB in 66-71 us, 4.8-5.1 TB/s (a copy of that size moves 5.0-5.3);
+// 4,801 rows of 24 heads of 64 in f32, 59 MB in 11.5 us; one row 4.2 us, which is the launch and the latency of its one trip
+// to memory.  Before a unit's loads went ahead of the work on the one before (then they waited for each other) the first took 159 us.
+// Without 16-byte pieces (an odd address) it takes 245 us: every value is a load of its own.
 #include <algorithm>
 #include <cmath>
 
@@ -176,7 +181,8 @@ hipError_t run(NormRopeDev d, bool wide, bool inter, int n_cu, hipStream_t s) {
     const int pairs = d.dim / (wide ? 2 * V : 2);
     while (d.lanes < 64 && d.lanes < pairs) d.lanes *= 2, d.log2_lanes++;
     d.units = (int)ceil_div(d.heads, 64 / d.lanes);
-    // 16 waves a CU, which with kAhead units each cover the memory's latency; rows that are fewer are shared
+    // 16 waves a CU, which with kAhead units each cover the memory's latency; rows that are fewer are shared: one row's five units
+    // go to five waves
     const int64_t most = (int64_t)n_cu * 16;
     d.split = (int)std::min<int64_t>(d.units, std::max<int64_t>(1, most / d.rows));
     d.waves = (int)(std::min<int64_t>(d.rows, most / d.split) * d.split);

@@ -608,3 +608,53 @@ def test_no_tokens_and_no_table(ctx, new):
     args, _ = R.attention_args(ctx, cache, batch, q, out, _code("f16"), 0.1)
     ctx.kv_attention(cache.args, batch.args, args)
     assert not out.any() and int(cache.fault) == 0
+
+
+@pytest.mark.parametrize("cache_kind, group", [("int8", 1), ("e4m3", 12)])
+def test_far_addresses(ctx, cache_kind, group):
+    """Pages and rows that lie more than 2^32 bytes and 2^31 values into their arrays give, bit for bit, what near ones give."""
+    from kokoro_hip import api
+    heads, dim, n, far_pages = 4, 256, 130, (1 << 16) + 9
+    g = torch.Generator().manual_seed(group)
+    k, v = (torch.randn(n, heads, dim, generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+    q = torch.randn(3, heads * group, dim, generator=g).to(torch.bfloat16).cuda()
+    row = (1 << 30) + 8  # rows 1 and 2 are 2^30 and 2^31 values behind row 0
+    width = (heads * group + 2 * heads) * dim
+
+    def run(pages, numbers, row):
+        rows = torch.empty(2 * row + 2 * width, dtype=torch.bfloat16, device="cuda")
+        kind = torch.int8 if cache_kind == "int8" else torch.uint8
+        dev = {"k": torch.empty(pages, heads, PAGE, dim, dtype=kind, device="cuda"), "v": torch.empty(pages, heads, dim, PAGE, dtype=kind, device="cuda"),
+               "k_scale": torch.empty(pages, heads, device="cuda"), "v_scale": torch.empty(pages, heads, device="cuda")}
+        for part in ("k", "v"):
+            dev[part][numbers] = 0
+        fault = torch.zeros(1, dtype=torch.int32, device="cuda")
+        cache = api.KvCache(type=api.KV_INT8 if cache_kind == "int8" else api.KV_E4M3, heads=heads, dim=dim, pages=pages,
+                            fault=fault.data_ptr(), **{x: y.data_ptr() for x, y in dev.items()})
+        view = lambda at, h: rows[at:].as_strided((3, h, dim), (row, dim, 1))  # noqa: E731
+        qr, kr, vr, out = view(0, heads * group), view(heads * group * dim, heads), view((heads * group + heads) * dim, heads), view(width, heads * group)
+        qr.copy_(q), kr.copy_(k[-3:]), vr.copy_(v[-3:])
+        first, last, whole = R.Batch([n - 3], [n - 3], [numbers]), R.Batch([3], [n], [numbers]), R.Batch([n], [n], [numbers])
+        ctx.kv_write(cache, first.args, R.rows_of(_code("bf16"), k, v))
+        ctx.kv_write(cache, last.args, R.rows_of(_code("bf16"), kr, vr))
+        back = torch.empty(2, n, heads, dim, dtype=torch.bfloat16, device="cuda")
+        ctx.kv_read(cache, whole.args, R.rows_of(_code("bf16"), back[0], back[1]))
+        holder = type("", (), {"args": cache})
+        args, space = R.attention_args(ctx, holder, last, qr, out, _code("bf16"), 0.07)
+        ctx.kv_attention(cache, last.args, args)
+        kr.zero_(), vr.zero_()
+        ctx.kv_read(cache, last.args, R.rows_of(_code("bf16"), kr, vr))
+        turned = out.clone()
+        pos = torch.arange(3, dtype=torch.int32, device="cuda")
+        rope = api.NormRope(type=_code("bf16"), dim=dim, rows=3, q_heads=heads * group, k_heads=0, q=qr.data_ptr(), q_row=row, q_head=dim,
+                            q_out=out.data_ptr(), q_out_row=row, q_out_head=dim, norm=1, eps=1e-6, pos=pos.data_ptr(), rot=dim, theta=1e4)
+        ctx.qk_norm_rope(rope)
+        got = [back.cpu(), turned.cpu(), out.clone().cpu(), kr.clone().cpu(), vr.clone().cpu()] + [dev[x][numbers].cpu() for x in dev]
+        assert int(fault) == 0
+        return got
+
+    near = run(5, [3, 0, 4], 2 * width)
+    far = run(far_pages, [far_pages - 1, 1, far_pages - 2], row)
+    for a, b in zip(near, far):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    assert near[1].isfinite().all() and near[1].float().abs().amax() > 0
