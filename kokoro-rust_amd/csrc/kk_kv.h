@@ -38,8 +38,9 @@ __device__ __forceinline__ void kv_fault(const KvCacheDev& c, int bit) {
     if (c.fault) atomicOr(c.fault, bit);
 }
 
-// Which sequence's tile a block works on (kv_tile_base).  Every thread of the block calls this; `found` is two words of LDS.  Returns the tile's number in its
-// sequence, or -1 (a number that no sequence uses, or a bad sequence).
+// Which sequence's tile a block works on (kv_tile_base).  Every thread of the block calls this; `found` is two words of LDS.
+// Returns the tile's number in its sequence, or -1 (a number that no sequence uses, or a bad sequence).  Where row_start falls, two
+// sequences may claim a tile: what is left in `found` is then checked against the sequence as any tile is.
 template <int THREADS>
 __device__ __forceinline__ int kv_find(const KvCacheDev& c, const KvBatchDev& B, int64_t tile, int64_t G, int M, int E,
                                        bool report, KvSeq& s, int* found) {
@@ -167,25 +168,6 @@ __device__ __forceinline__ uint2 stream_load(const uint2* p) {
 }
 
 // N values next to each other, as 16-byte accesses where `vec` says that they lie on such a boundary.
-template <int T, int N>
-__device__ __forceinline__ void load_values(const void* base, int64_t at, bool vec, float* x) {
-    typedef typename ElemOf<T>::type E;
-    constexpr int W = 16 / (int)sizeof(E);
-    const E* p = (const E*)base + at;
-    E e[N];
-    if (vec && N % W == 0) {
-#pragma unroll
-        for (int i = 0; i < N; i += W) {
-            const uint4 q = *(const uint4*)(p + i);
-            __builtin_memcpy(e + i, &q, 16);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) e[i] = p[i];
-    }
-#pragma unroll
-    for (int i = 0; i < N; i++) x[i] = ElemOf<T>::load(e[i]);
-}
 template <int T, int N>
 __device__ __forceinline__ void store_values(void* base, int64_t at, bool vec, const float* x) {
     typedef typename ElemOf<T>::type E;
