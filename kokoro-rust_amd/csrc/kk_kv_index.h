@@ -11,7 +11,10 @@
 namespace kk {
 
 constexpr int kPage = KK_KV_PAGE;
-constexpr int kFewRows = 32;     // rows of a (sequence, cache head) up to which attention reads the cache into registers
+// Rows of a (sequence, cache head) up to which attention reads the cache into registers.  17 to 32 rows there against the kernel of many
+// rows, us: five drafts of 64 conversations of 1,000 to 4,000 tokens 81 and 188, behind 60,000 tokens 32 and 46; at 256 values
+// a head, where two tiles' registers barely fit, 154 and 197, 64 and 61.
+constexpr int kFewRows = 32;
 constexpr int kMostParts = 256;  // of the token axis
 
 struct KvBatchDev {
