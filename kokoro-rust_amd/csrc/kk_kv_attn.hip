@@ -5,6 +5,8 @@
 // in one pass over the pages, keeping per row M, the largest s_t + log2 b seen, and m, the largest s_t (or up to kSlack below them),
 //   P_t = 2^{s_t + log2 b - M + kLift},  O = sum P_t v_t = 2^{kLift - M} sum 2^{s_t} b v_t,
 //   l = sum_t 2^{s_t - m}: a page's sum of P_t times 2^{M - kLift - log2 b - m},  out = 2^{M - kLift - m} O / l.
+// That sum is of P_t in f32, before the rounding to f16 that O's product needs: f16 ends at 2^-24, and a page whose V is small
+// beside another's may vanish in O, but its tokens' weights may not in l.
 // Folding log2 b into the exponent costs nothing (it goes into the constant of the fused multiply-add) and leaves the
 // stored numbers themselves as operands: int8 and e4m3 are exact in f16, so K and V enter the matrix cores without a
 // rounding, Q as f16 scaled per row to [2^14, 2^15) (a bf16 value keeps its 8 bits down to 2^-28 of the row's largest), and
@@ -427,7 +429,8 @@ attend_few_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
 // them for its 32 products of 32 cycles; a block's start and end cost another 20,000, and half of what the diagonal's pages compute is masked.
 // Of 1,000 to 4,096 tokens (278 GFLOP) 329-372 us, 750-843 TFLOP/s.  Products and exponentials in turn made 703 TFLOP/s where
 // interleaved and half a page apart make 887.  64 rows a wave (half the reads of LDS) were slower, 575 against 740 then: the
-// accumulators no longer fit beside the operands and are moved.
+// accumulators no longer fit beside the operands and are moved.  l from the unrounded exponentials costs no more than a dot
+// instruction over the rounded ones did: 606 us and 606 for the four prompts, e4m3 632 and 654, 430 and 423 at 64 values a head.
 template <int D, int CT, int W>
 __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) attend_many_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
     constexpr int kRows = 32 * W, kThreads = 64 * W;
@@ -619,7 +622,7 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) attend_many_kernel(K
                 const float e1 = __builtin_amdgcn_exp2f(fmaf(sc[k >> 3][2 * (k & 7) + 1], c1, add));
                 const f16x2 e = {(_Float16)e0, (_Float16)e1};
                 pr[k >> 2][2 * (k & 3)] = e[0], pr[k >> 2][2 * (k & 3) + 1] = e[1];
-                sum = __builtin_amdgcn_fdot2(e, f16x2{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
+                sum += e0 + e1;
             }
             __builtin_amdgcn_sched_barrier(0);
         }
