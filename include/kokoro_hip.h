@@ -422,7 +422,9 @@ typedef struct {
     size_t workspace_bytes;
 } kk_kv_attention_args;
 /* The workspace that kk_kv_attention needs for these arguments (0: none), or negative KK_ERR_* for arguments that it would
- * refuse.  It depends on n, rows, max_new, max_len, both head counts, dim, window and the device's compute units alone. */
+ * refuse.  It depends on n, rows, max_new, max_len, both head counts, dim, causal, window and the device's compute units alone.
+ * It does not always grow with them: fewer rows may be split into more parts, so a workspace that serves several batches is
+ * as large as the largest of theirs. */
 int64_t kk_kv_attention_workspace(kk_ctx* ctx, const kk_kv_cache* cache, const kk_kv_batch* batch,
                                   const kk_kv_attention_args* args, char* err, size_t errlen);
 int kk_kv_attention(kk_ctx* ctx, const kk_kv_cache* cache, const kk_kv_batch* batch, const kk_kv_attention_args* args,
