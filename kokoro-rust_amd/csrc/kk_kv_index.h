@@ -16,6 +16,7 @@ constexpr int kPage = KK_KV_PAGE;
 // a head, where two tiles' registers barely fit, 154 and 197, 64 and 61.
 constexpr int kFewRows = 32;
 constexpr int kMostParts = 256;  // of the token axis
+constexpr int64_t kMostThreads = ((int64_t)1 << 32) - 1;  // of a launch: HIP counts them in 32 bits
 
 struct KvBatchDev {
     const int32_t *row_start, *len, *table;
@@ -108,10 +109,15 @@ struct AttnPlan {
     int row_tiles;    // few: 16-row tiles of a block (1 or 2)
     int waves;        // few: of a block, 8 or 4
     int tile_rows;    // rows of a block: many, 256 where that fills the device, or 128
+    int threads;      // of a block, at most
     int64_t tiles;    // blocks along the rows
     int chunk, parts; // pages of a part, parts of the axis
     int64_t ws_bytes; // partial results, 0 for one part
 };
+inline bool join_fits(int64_t rows_heads) { return (rows_heads + 3) / 4 <= kMostThreads / 256; }
+inline bool attention_fits(const AttnPlan& p, const kk_kv_batch& b, int heads, int cache_heads) {
+    return p.tiles * cache_heads * p.parts <= kMostThreads / p.threads && (p.parts == 1 || join_fits(b.rows * (int64_t)heads));
+}
 inline AttnPlan attention_plan(const kk_kv_cache& c, const kk_kv_batch& b, const kk_kv_attention_args& a, int n_cu) {
     AttnPlan p{};
     const int64_t group = a.heads / c.heads, rows = b.max_new * group;
@@ -126,8 +132,11 @@ inline AttnPlan attention_plan(const kk_kv_cache& c, const kk_kv_batch& b, const
     // Many rows: 256 a block cost the matrix cores 5% less than 2 x 128 (four prompts of 512 rows behind 8,000 tokens 275 against 295
     // us, one prompt of 4,096 158 against 169), where they fill the device and see enough pages; else the finer blocks end
     // sooner (a prompt of 2,048 57 against 67, 32 prompts of 512 155 against 178, a prompt of 2,500 72 against 80).
-    p.tile_rows = p.few ? 16 * p.row_tiles : c.dim <= 128 && about(256) * c.heads >= n_cu && seen(b.max_len / kPage) >= 24 ? 256 : 128;
-    p.tiles = p.few ? b.n : b.rows * group / p.tile_rows + b.n;
+    auto tiles = [&](int M) { return b.rows * group / M + b.n; };
+    p.tile_rows = p.few ? 16 * p.row_tiles
+                  : c.dim <= 128 && about(256) * c.heads >= n_cu && seen(b.max_len / kPage) >= 24 && tiles(256) * c.heads <= kMostThreads / 512
+                      ? 256 : 128;
+    p.tiles = p.few ? b.n : tiles(p.tile_rows);
     int64_t pages = ((int64_t)b.max_len + kPage - 1) / kPage;
     if (a.window) {  // a block's rows stand at most that many tokens apart, and N tokens touch at most N / 64 + 2 pages
         const int64_t tokens = (int64_t)a.window + (p.few ? b.max_new : p.tile_rows / group + 1);
@@ -156,13 +165,17 @@ inline AttnPlan attention_plan(const kk_kv_cache& c, const kk_kv_batch& b, const
         const double join = 4.0 + 2e-6 * c.dim * (double)((int64_t)b.rows * a.heads * ((pages + part - 1) / part));
         if (part < pages && saved > join) chunk = part;
     }
-    chunk = std::max(chunk, (pages + kMostParts - 1) / kMostParts);
+    // A launch holds so many blocks, and the second one four rows' heads a block: sequences by the hundred thousand get fewer parts.
+    int64_t most = std::min<int64_t>(kMostParts, std::max<int64_t>(kMostThreads / (p.few ? 256 : 2 * p.tile_rows) / blocks, 1));
+    if (!join_fits(b.rows * (int64_t)a.heads)) most = 1;
+    chunk = std::max(chunk, (pages + most - 1) / most);
     p.parts = (int)((pages + chunk - 1) / chunk);
     p.chunk = (int)((pages + p.parts - 1) / p.parts);
     p.parts = (int)((pages + p.chunk - 1) / p.chunk);
     // 8 waves where the blocks leave CUs idle and have the pages: 1,000 tokens of one sequence 10.5 us against 11.9 with 4, of 16
     // 12.1 against 14.6; 4 where blocks share CUs (64 of 1,000: 24.8 against 27.3 with 8).
     p.waves = blocks * p.parts <= n_cu && p.chunk > 4 ? 8 : 4;
+    p.threads = p.few ? 64 * p.waves : 2 * p.tile_rows;
     if (p.parts > 1) p.ws_bytes = (int64_t)b.rows * a.heads * p.parts * (c.dim * (int64_t)sizeof(float) + 2 * (int64_t)sizeof(float));
     return p;
 }

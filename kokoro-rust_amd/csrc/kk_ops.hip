@@ -9,7 +9,7 @@
 namespace kk {
 namespace {
 
-constexpr int64_t kMostBlocks = (int64_t)1 << 23;  // x 256 threads: a launch's threads are counted in 32 bits
+constexpr char kTooLarge[] = "the batch is too large for one launch";
 
 int refuse(char* err, size_t errlen, int code, const std::string& m) {
     if (err && errlen) std::snprintf(err, errlen, "%s", m.c_str());
@@ -60,12 +60,6 @@ auto no_throw(char* err, size_t errlen, F&& f) -> decltype(f()) {
 
 bool empty(const kk_kv_batch& b) { return b.n == 0 || b.rows == 0 || b.max_new == 0; }
 
-std::string blocks_error(const kk_kv_batch& b, const AttnPlan& p, int heads, int cache_heads) {
-    if (p.tiles * cache_heads > kMostBlocks / p.parts || (p.parts > 1 && (int64_t)b.rows * heads > kMostBlocks))
-        return "the batch is too large for one launch";
-    return "";
-}
-
 }  // namespace
 }  // namespace kk
 
@@ -115,8 +109,7 @@ int64_t kk_kv_attention_workspace(kk_ctx* ctx, const kk_kv_cache* cache, const k
         if (!ctx) return refuse(err, errlen, KK_ERR_INVALID, "null context");
         if (empty(*batch)) return 0;
         const AttnPlan p = attention_plan(*cache, *batch, *args, ctx_cus(ctx));
-        const std::string f = blocks_error(*batch, p, args->heads, cache->heads);
-        if (!f.empty()) return refuse(err, errlen, KK_ERR_INVALID, f);
+        if (!attention_fits(p, *batch, args->heads, cache->heads)) return refuse(err, errlen, KK_ERR_INVALID, kTooLarge);
         return p.ws_bytes;
     });
 }
@@ -129,8 +122,7 @@ int kk_kv_attention(kk_ctx* ctx, const kk_kv_cache* cache, const kk_kv_batch* ba
         if (!ctx) return refuse(err, errlen, KK_ERR_INVALID, "null context");
         if (empty(*batch)) return (int)KK_OK;
         const AttnPlan p = attention_plan(*cache, *batch, *args, ctx_cus(ctx));
-        const std::string f = blocks_error(*batch, p, args->heads, cache->heads);
-        if (!f.empty()) return refuse(err, errlen, KK_ERR_INVALID, f);
+        if (!attention_fits(p, *batch, args->heads, cache->heads)) return refuse(err, errlen, KK_ERR_INVALID, kTooLarge);
         if (p.ws_bytes && (!args->workspace || (int64_t)args->workspace_bytes < p.ws_bytes || (uintptr_t)args->workspace % 16))
             return refuse(err, errlen, KK_ERR_INVALID,
                           "the workspace is null, not 16-byte aligned or smaller than " + std::to_string(p.ws_bytes) + " bytes");

@@ -1,5 +1,8 @@
 // CPU check of how attention over the 8-bit cache is launched (attention_plan in kokoro-rust_amd/csrc/kk_kv_index.h).
 //   key    changes one field of random calls at a time and prints the names of those that ever changed the workspace's size
+//   fits   random calls over the whole range of sizes: prints "calls N refused R violations V", a violation being a call that is
+//          refused although blocks of its kind, whole and of 128 rows, fit into a launch, or whose launches hold 2^32 threads
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <functional>
@@ -84,9 +87,50 @@ int key() {
     return 0;
 }
 
+int fits() {
+    auto spread = [](int64_t most) { return (int64_t)std::exp2(std::log2((double)most) * below(1 << 20) / (1 << 20)); };
+    const uint64_t limit = (uint64_t)1 << 32;
+    long calls = 0, refused = 0, bad = 0;
+    auto check = [&](const Call& x) {
+        const AttnPlan p = attention_plan(x.c, x.b, x.a, x.n_cu);
+        const int64_t group = x.a.heads / x.c.heads, rows_heads = (int64_t)x.b.rows * x.a.heads;
+        const bool few = (int64_t)x.b.max_new * group <= 32;
+        const uint64_t least = (uint64_t)(few ? x.b.n : x.b.rows * group / 128 + x.b.n) * x.c.heads * 256;
+        const uint64_t blocks = (uint64_t)p.tiles * x.c.heads * p.parts;
+        const uint64_t block = few ? 64 * p.waves : 2 * p.tile_rows;
+        const bool ok = attention_fits(p, x.b, x.a.heads, x.c.heads);
+        calls++, refused += !ok;
+        bad += ok != (least < limit);
+        if (ok) bad += blocks * block >= limit || (p.parts > 1 && (uint64_t)(rows_heads + 3) / 4 * 256 >= limit);
+        bad += p.chunk < 1 || p.parts < 1 || (p.parts > 1) != (p.ws_bytes > 0);
+        return ok;
+    };
+    for (int i = 0; i < 300000; i++) {
+        Call x;
+        x.c.dim = dim_of(), x.c.heads = (int)spread(4096), x.a.heads = x.c.heads * (int)spread(4096 / x.c.heads);
+        x.a.causal = below(2), x.a.window = x.a.causal && below(2) ? (int)spread(1 << 30) : 0, x.n_cu = 1 + below(400);
+        x.b.n = (int)spread(1 << 20), x.b.rows = (int)spread(1 << 28), x.b.max_new = (int)spread(1 << 28);
+        x.b.max_len = (int)spread(1 << 30);
+        check(x);
+    }
+    // 2^23 blocks of 512 threads are 2^32: the finer blocks are taken
+    Call x;
+    x.c.dim = 128, x.c.heads = x.a.heads = 8, x.a.causal = 1;
+    x.b.n = (1 << 20) - 1000, x.b.rows = 256000, x.b.max_new = 200, x.b.max_len = 5000;
+    bad += !check(x);
+    x.b.n--;
+    bad += !check(x) || attention_plan(x.c, x.b, x.a, x.n_cu).tile_rows != 256;
+    // as many sequences as a batch may have, at the largest bound
+    x.b.n = 1 << 20, x.b.rows = 1 << 20, x.b.max_new = 1, x.b.max_len = 1 << 30, x.a.heads = 32;
+    bad += !check(x);
+    std::printf("calls %ld refused %ld violations %ld\n", calls, refused, bad);
+    return 0;
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
     if (argc > 1 && !std::strcmp(argv[1], "key")) return key();
+    if (argc > 1 && !std::strcmp(argv[1], "fits")) return fits();
     return 2;
 }

@@ -25,3 +25,9 @@ def test_workspace_depends_on_what_the_header_names(check):
     said = re.search(r"It depends on ([^.]*?) alone\.", text).group(1)
     named = set(re.split(r", | and ", said.replace("the device's ", "").replace("both head counts", "query heads, cache heads")))
     assert set(check("key").split("\n")) - {""} == named
+
+
+def test_no_batch_is_refused_for_its_split(check):
+    """Whatever fits into a launch in one part is accepted, with parts that fit too; and what is accepted holds no 2^32 threads."""
+    calls, refused, bad = map(int, check("fits").split()[1::2])
+    assert bad == 0 and 0 < refused < calls // 2
