@@ -141,7 +141,8 @@ __global__ void __launch_bounds__(256) norm_rope_kernel(NormRopeDev a) {
 #pragma unroll
                     for (int i = 0; i < 2 * V; i++) {
                         v[j][i] = ElemOf<T>::load(raw[n][j][i / V].e[i % V]);
-                        sum = fmaf(v[j][i], mine[j] ? v[j][i] : 0.0f, sum);
+                        const float own = mine[j] ? v[j][i] : 0.0f;  // both factors: an infinity times 0 is NaN
+                        sum = fmaf(own, own, sum);
                     }
                 if (a.norm) {
                     for (int m = 1; m < a.lanes; m <<= 1) sum += __shfl_xor(sum, m);
