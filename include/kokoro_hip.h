@@ -338,7 +338,8 @@ int kk_qk_norm_rope(kk_ctx* ctx, const kk_norm_rope* args, void* stream, char* e
 /* A cache of keys and values: pages of KK_KV_PAGE tokens of every head, 8 bits a value, and one scale for
  * each (page, head) of K and one of V; a value is its stored number times its scale.  V is stored with a
  * value's tokens next to each other, which is how the matrix cores read it.  Scales are at least 2^-90, or
- * 0 for a page that holds only zeros. */
+ * 0 for a page that holds only zeros.  What kk_kv_write stores is finite.  Pages that a caller fills by other means hold finite
+ * numbers and scales too for every token of a sequence: e4m3's NaN code in V spreads to rows that do not see its token. */
 #define KK_KV_PAGE 64
 #define KK_KV_INT8 1 /* -127..127 */
 #define KK_KV_E4M3 2 /* 8-bit floating point, 4 bits of exponent and 3 of mantissa, up to 448 */
@@ -408,9 +409,12 @@ int kk_kv_read(kk_ctx* ctx, const kk_kv_cache* cache, const kk_kv_batch* batch, 
  * gives zeros.  Scores, softmax and sums are f32; the stored numbers enter the matrix products exactly, the
  * queries to 2^-24 of a row's largest value, probabilities with 11 bits (scales of V that differ by over 2^100 within what a
  * row sees are out of f32's range).  The result does not depend on what else
- * is in the batch, except that the axis is split by max_len and the batch's size (the order of f32 sums). */
+ * is in the batch, except that the kernel is chosen by max_new and the axis split by max_len and the batch's size (the order of
+ * f32 sums, and the power of two at which probabilities are rounded).  One choice is made for the whole batch: single
+ * tokens beside a piece of a prompt (over 32 rows of a cache head) run on the kernel for many rows, and two calls can take half
+ * the time (63 tokens beside 512 rows behind 2,000: 185 us in one, 108 in two; 15 such tokens 73 and 74). */
 typedef struct {
-    int32_t type;  /* KK_BF16 or KK_F16: q and out */
+    int32_t type;  /* KK_BF16 or KK_F16: q and out (the products take operands of 16 bits) */
     int32_t heads; /* query heads, a multiple of cache->heads */
     const void* q;
     int64_t q_row, q_head; /* in values */
@@ -423,8 +427,9 @@ typedef struct {
 } kk_kv_attention_args;
 /* The workspace that kk_kv_attention needs for these arguments (0: none), or negative KK_ERR_* for arguments that it would
  * refuse.  It depends on n, rows, max_new, max_len, both head counts, dim, causal, window and the device's compute units alone.
- * It does not always grow with them: fewer rows may be split into more parts, so a workspace that serves several batches is
- * as large as the largest of theirs. */
+ * It is sized by the bounds: 4,096 one-token sequences with max_len 131,072 take 4.4 GB at 32 heads of 128, whatever their
+ * lengths are.  It does not always grow with them: fewer rows may be split into more parts, so a workspace that serves
+ * several batches is as large as the largest of theirs. */
 int64_t kk_kv_attention_workspace(kk_ctx* ctx, const kk_kv_cache* cache, const kk_kv_batch* batch,
                                   const kk_kv_attention_args* args, char* err, size_t errlen);
 int kk_kv_attention(kk_ctx* ctx, const kk_kv_cache* cache, const kk_kv_batch* batch, const kk_kv_attention_args* args,

@@ -6,7 +6,8 @@
 // cache holds a value's tokens next to each other: bytes are written [token][dim] and taken out as 4 x 4 byte blocks.
 //
 // Measured at 8 heads of 128 values, a kernel alone: writing 14,000 tokens of eight prompts (bf16, int8; 86 MB) 21 us, 4.1 TB/s,
-// reading them back 17 us, 5.1 TB/s; reading 32,001 tokens (197 MB) 31 us, 6.4 TB/s; one token each of 64 conversations 7.5 us, its
+// where the last-level cache holds their rows, 33 us, 2.6 TB/s, where it does not (a block reads 256 bytes of each packed row,
+// whose neighbours other blocks read much later); reading them back 17 us, 5.1 TB/s; reading 32,001 tokens (197 MB) 31 us, 6.4 TB/s; one token each of 64 conversations 7.5 us, its
 // 1,024 blocks' chain of length, page number, scale and bytes.  Writing was 29 us while each load waited for the one before and
 // each value was checked for infinities: now all of a page's loads are in flight together, the sizes are compared on the bits, and
 // only a block that holds an infinity or NaN checks its values.

@@ -169,9 +169,10 @@ struct RowSum {
 // Measured at 32 heads of 128 over 8: one token each of 64 conversations of 200 to 8,191 tokens (536 MB) 101 us and the join's
 // 4.7, 5.1 TB/s over both (a kernel that only reads reaches 6.0, nontemporal, as these loads are, 6.5; with plain ones this
 // kernel takes 4% longer, the drafts 8%); five drafts
-// behind 131,000 tokens (269 MB) 46 us, 5.9 TB/s, and 4.8; one token behind 500 8 us, a chain of about 15,000 cycles: the sequence
-// 2,000, page and queries 4,500, the one page 3,700, the join of the waves 5,500.  For 17 to 32 rows each operand of the
-// cache feeds two products.
+// behind 131,000 tokens (269 MB) 46 us, 5.9 TB/s, and 4.8; one token behind 500 8 us, a chain of about 15,000 cycles of the
+// block's first wave: the sequence 2,100, its loads' addresses 1,300, queries and K 2,000, the one page 3,600, its sums to LDS 700,
+// the wait for the wave that ends last 3,500-4,100, and the sums over the waves 1,400.  For 17 to 32 rows each operand of
+// the cache feeds two products.
 template <int D, int CT, int NT, int W>
 __global__ void __launch_bounds__(64 * W, D <= 192 && D * NT <= 256 ? 2 : 1)
 attend_few_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
@@ -424,10 +425,12 @@ attend_few_kernel(KvCacheDev c, KvBatchDev B, AttnDev a) {
 // ([token][dim]), V by value ([dim][token]), rows padded by 16 bytes (16-byte reads of 8 lanes then cover all banks).  Within 32
 // tokens K's rows are stored so that a lane's 8 scores of one step are 8 tokens in order, as its 16 bytes of V hold them.
 // Page numbers and scales are read 64 pages at a time, one a lane.
-// Measured: four prompts of 4,096 tokens at 32 heads of 128 over 8 (550 GFLOP) 608-620 us, 887-904 TFLOP/s, 40% of the matrix
+// Measured: four prompts of 4,096 tokens at 32 heads of 128 over 8 (550 GFLOP) 600-620 us, 887-915 TFLOP/s, 40% of the matrix
 // cores' rate at the 2.1 GHz that the device holds meanwhile: in the loop a SIMD takes 1,950 cycles for a wave's page, 1,024 of
-// them for its 32 products of 32 cycles; a block's start and end cost another 20,000, and half of what the diagonal's pages compute is masked.
-// Of 1,000 to 4,096 tokens (278 GFLOP) 329-372 us, 750-843 TFLOP/s.  Products and exponentials in turn made 703 TFLOP/s where
+// them for its 32 products of 32 cycles; a block's start and end cost another 20,000 (kBufs pages of K
+// are unpacked and stored before the first product, which needs one), and half of what the diagonal's pages compute is masked.
+// Of 1,000 to 4,096 tokens (278 GFLOP) 327-372 us, 750-850 TFLOP/s.  Four prompts of 2,048 at 16 heads: of 256 values over 4
+// 238 us, of 192 over 2 179 us, 576-579 TFLOP/s: 386 to 499 registers leave one wave a SIMD, with nothing to overlap with.  Products and exponentials in turn made 703 TFLOP/s where
 // interleaved and half a page apart make 887.  64 rows a wave (half the reads of LDS) were slower, 575 against 740 then: the
 // accumulators no longer fit beside the operands and are moved.  l from the unrounded exponentials costs no more than a dot
 // instruction over the rounded ones did: 606 us and 606 for the four prompts, e4m3 632 and 654, 430 and 423 at 64 values a head.
@@ -709,7 +712,7 @@ __global__ void __launch_bounds__(64 * W, D <= 128 ? 2 : 1) attend_many_kernel(K
 
 // out = sum_p 2^{m_p - m} O_p / sum_p 2^{m_p - m} l_p, a wave for each (row, head).  Bound by the latency of three dependent
 // loads (the sequence, m, O): 4.7 us for 64 rows of 32 heads in 4 parts as for 5 rows in 64.  Four waves that share the parts were no
-// faster: one token behind 1,000,000 tokens, 256 parts, 338 us against 339.
+// faster: one token behind 1,000,000 tokens, 253 parts, 338 us against 339.
 template <int D>
 __global__ void __launch_bounds__(256) attend_join_kernel(KvBatchDev B, AttnDev a) {
     constexpr int N = (D + 63) / 64;

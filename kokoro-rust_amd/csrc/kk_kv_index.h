@@ -13,7 +13,8 @@ namespace kk {
 constexpr int kPage = KK_KV_PAGE;
 // Rows of a (sequence, cache head) up to which attention reads the cache into registers.  17 to 32 rows there against the kernel of many
 // rows, us: five drafts of 64 conversations of 1,000 to 4,000 tokens 81 and 188, behind 60,000 tokens 32 and 46; at 256 values
-// a head, where two tiles' registers barely fit, 154 and 197, 64 and 61.
+// a head, where two tiles take all 512 registers and 200 bytes of scratch a lane, 154 and 197, 64 and 61: one sequence alone loses
+// a little there, a batch gains.
 constexpr int kFewRows = 32;
 constexpr int kMostParts = 256;  // of the token axis
 constexpr int64_t kMostThreads = ((int64_t)1 << 32) - 1;  // of a launch: HIP counts them in 32 bits

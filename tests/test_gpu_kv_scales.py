@@ -39,12 +39,12 @@ def _bound(want, size, score, most, n, dim, kind, top):
 
 
 @pytest.mark.parametrize("cache_kind, kind", [("int8", "bf16"), ("e4m3", "f16")])
-@pytest.mark.parametrize("bits", [28, 40, 80])
+@pytest.mark.parametrize("bits", [28, 40, 80, 97])
 @pytest.mark.parametrize("order", ["large first", "large last", "large in the middle", "small ahead"])
 @pytest.mark.parametrize("plan", PLANS)
 def test_small_values_keep_their_weight(ctx, plan, order, bits, cache_kind, kind):
-    """One page's values are 2^bits times larger than the others'.  Scores are level over all pages, or some 8 bits higher on
-    two pages of small values."""
+    """One page's values are 2^bits times larger than the others' (97: from near the smallest scale there is, 2^-90).  Scores are
+    level over all pages, or some 8 bits higher on two pages of small values."""
     new, n, heads, group, dim, seqs, parts = PLANS[plan]
     pages = -(-n // PAGE)
     cache = R.Cache(cache_kind, heads, dim, pages + 2)
@@ -54,6 +54,7 @@ def test_small_values_keep_their_weight(ctx, plan, order, bits, cache_kind, kind
     at = {"large first": 0, "small ahead": 0, "large last": (n - new - 1) // PAGE, "large in the middle": 1}[order]
     far = torch.ones(n, dtype=torch.bool)
     far[at * PAGE:(at + 1) * PAGE] = False
+    v *= 2.0 ** 12 if bits > 80 else 1.0
     v[far] *= 2.0 ** -bits
     q = 1 + 0.3 * torch.randn(new + seqs - 1, heads * group, dim, generator=g)
     scale = 1.0 / dim ** 0.5
