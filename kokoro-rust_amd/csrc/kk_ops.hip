@@ -123,7 +123,7 @@ int kk_kv_attention(kk_ctx* ctx, const kk_kv_cache* cache, const kk_kv_batch* ba
         if (empty(*batch)) return (int)KK_OK;
         const AttnPlan p = attention_plan(*cache, *batch, *args, ctx_cus(ctx));
         if (!attention_fits(p, *batch, args->heads, cache->heads)) return refuse(err, errlen, KK_ERR_INVALID, kTooLarge);
-        if (p.ws_bytes && (!args->workspace || (int64_t)args->workspace_bytes < p.ws_bytes || (uintptr_t)args->workspace % 16))
+        if (p.ws_bytes && (!args->workspace || args->workspace_bytes < (size_t)p.ws_bytes || (uintptr_t)args->workspace % 16))
             return refuse(err, errlen, KK_ERR_INVALID,
                           "the workspace is null, not 16-byte aligned or smaller than " + std::to_string(p.ws_bytes) + " bytes");
         return entry(ctx, err, errlen, [&] { return launch_kv_attention(*cache, *batch, *args, p, (hipStream_t)stream); });

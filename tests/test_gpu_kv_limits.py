@@ -51,3 +51,22 @@ def test_large_bounds(ctx):
         batch = api.KvBatch(n=n, rows=n, max_new=1, max_len=bound, row_start=p, len=p, table=p, table_width=-(-bound // 64), table_stride=0)
         parts = ctx.kv_attention_workspace(cache, batch, args) / (n * 32 * (128 + 2) * 4)
         assert parts == int(parts) <= min(256, -(-bound // 64)) and parts * n * 8 * 256 < 1 << 32
+
+
+@pytest.mark.parametrize("said", [1 << 40, (1 << 63) + 5, (1 << 64) - 1])
+def test_a_workspace_of_any_stated_size(ctx, said):
+    """A workspace that is as large as needed and said to be larger, up to the largest number that its size can be."""
+    from kokoro_hip import api
+    cache = R.Cache("int8", 1, 64, 40)
+    tables = R.deal([2000], 40, np.random.default_rng(1))
+    k, v = torch.randn(2, 2000, 1, 64, generator=torch.Generator().manual_seed(2)).cuda()
+    R.write(ctx, cache, R.Batch([2000], [2000], tables), k, v, api.F32)
+    batch = R.Batch([1], [2000], tables)
+    q = torch.randn(1, 2, 64, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    out = torch.zeros_like(q)
+    args, space = R.attention_args(ctx, cache, batch, q, out, api.BF16, 0.2)
+    need, args.workspace_bytes = args.workspace_bytes, said
+    assert need > 0
+    ctx.kv_attention(cache.args, batch.args, args)
+    R.check_attention(out, q, cache, batch, 0.2, True, 0, "bf16")
+    assert (space[need:] == 0xA5).all()
