@@ -134,9 +134,9 @@ inline AttnPlan attention_plan(const kk_kv_cache& c, const kk_kv_batch& b, const
     // us, one prompt of 4,096 158 against 169), where they fill the device and see enough pages; else the finer blocks end
     // sooner (a prompt of 2,048 57 against 67, 32 prompts of 512 155 against 178, a prompt of 2,500 72 against 80).
     auto tiles = [&](int M) { return b.rows * group / M + b.n; };
-    p.tile_rows = p.few ? 16 * p.row_tiles
-                  : c.dim <= 128 && about(256) * c.heads >= n_cu && seen(b.max_len / kPage) >= 24 && tiles(256) * c.heads <= kMostThreads / 512
-                      ? 256 : 128;
+    const bool coarse = c.dim <= 128 && about(256) * c.heads >= n_cu && seen(b.max_len / kPage) >= 24 &&
+                        tiles(256) * c.heads <= kMostThreads / 512;
+    p.tile_rows = p.few ? 16 * p.row_tiles : coarse ? 256 : 128;
     p.tiles = p.few ? b.n : tiles(p.tile_rows);
     int64_t pages = ((int64_t)b.max_len + kPage - 1) / kPage;
     if (a.window) {  // a block's rows stand at most that many tokens apart, and N tokens touch at most N / 64 + 2 pages
@@ -166,7 +166,7 @@ inline AttnPlan attention_plan(const kk_kv_cache& c, const kk_kv_batch& b, const
         const double join = 4.0 + 2e-6 * c.dim * (double)((int64_t)b.rows * a.heads * ((pages + part - 1) / part));
         if (part < pages && saved > join) chunk = part;
     }
-    // A launch holds so many blocks, and the second one four rows' heads a block: sequences by the hundred thousand get fewer parts.
+    // Both launches must hold their blocks (the join's are four (row, head) each): sequences by the hundred thousand get fewer parts.
     int64_t most = std::min<int64_t>(kMostParts, std::max<int64_t>(kMostThreads / (p.few ? 256 : 2 * p.tile_rows) / blocks, 1));
     if (!join_fits(b.rows * (int64_t)a.heads)) most = 1;
     chunk = std::max(chunk, (pages + most - 1) / most);
