@@ -435,6 +435,133 @@ int64_t kk_kv_attention_workspace(kk_ctx* ctx, const kk_kv_cache* cache, const k
 int kk_kv_attention(kk_ctx* ctx, const kk_kv_cache* cache, const kk_kv_batch* batch, const kk_kv_attention_args* args,
                     void* stream, char* err, size_t errlen);
 
+/* ------------------------------------------------------------------ products of ragged rows: experts and adapters
+ * The matrix products around that attention, on the same terms (the caller's device memory and stream, nothing allocated,
+ * kept or synchronized; they can be captured into a graph): a feed-forward part of experts (kk_expert_route, kk_expert_product
+ * twice, kk_expert_join), and projections that all requests share with a low-rank adapter (a voice's, a persona's) for each
+ * (kk_adapter_product).  Matrices are [outputs][inputs], inputs next to each other; strides are in values.  Products are of
+ * 16-bit operands with f32 sums, rounded once.  What only the device knows (start, places, adapters) is checked by
+ * the kernels: `fault` is one word, or NULL, where a kernel that meets a bad one sets KK_PRODUCT_BAD_* bits. */
+#define KK_PRODUCT_BAD_START 1   /* a group that leaves [0, entries] or ends before it begins: left out */
+#define KK_PRODUCT_BAD_PLACE 2   /* a place outside x_rows or y_rows: nothing is read or written for its entry */
+#define KK_PRODUCT_BAD_ADAPTER 4 /* an adapter number of `adapters` or more: the row's result is that of a row without one */
+#define KK_MOST_EXPERTS 1024
+#define KK_MOST_CHOICES 32
+#define KK_MOST_RANK 256
+
+/* The `top` experts of each row with the largest logits, the largest first and of equal ones the lowest (-0 equals 0), their
+ * weights, and the choices grouped by expert.
+ *  - An expert whose logit is -inf or NaN is never chosen; +inf counts as the largest finite number.  A row with fewer than
+ *    `top` others (padding: none) has expert -1 and weight 0 in the rest.
+ *  - weight: KK_SCORE_SOFTMAX, the softmax over all experts of the row; KK_SCORE_SIGMOID, 1 / (1 + exp(-logit)).  With `renorm`
+ *    divided by their sum over the row's choices; then times `scale`.  Computed in f32.
+ *  - choice j of row r has the number r * top + j.  start[e]..start[e + 1] are the places of expert e's choices in `place`, which
+ *    lists their numbers in rising order; start[experts] of them in all, and -1 behind. */
+#define KK_SCORE_SOFTMAX 0
+#define KK_SCORE_SIGMOID 1
+typedef struct {
+    int32_t type;           /* KK_BF16, KK_F16, KK_F32: the logits */
+    int32_t rows;           /* >= 0, rows * top at most 2^28 */
+    int32_t experts;        /* 1..KK_MOST_EXPERTS */
+    int32_t top;            /* 1..KK_MOST_CHOICES, at most `experts` */
+    const void* logits;     /* [rows] rows of `experts` values */
+    int64_t logits_row;
+    int32_t score, renorm;
+    float scale;            /* finite */
+    int32_t* expert;        /* [rows][top] */
+    float* weight;          /* [rows][top] */
+    int32_t* start;         /* [experts + 1] */
+    int32_t* place;         /* [rows * top] */
+    void* workspace;        /* 16-byte aligned, kk_expert_route_workspace bytes or more; need not be cleared */
+    size_t workspace_bytes;
+} kk_expert_route_args;
+/* The workspace that kk_expert_route needs (0: none), or negative KK_ERR_* for arguments that it would refuse.  It depends on rows,
+ * experts and top alone. */
+int64_t kk_expert_route_workspace(kk_ctx* ctx, const kk_expert_route_args* args, char* err, size_t errlen);
+int kk_expert_route(kk_ctx* ctx, const kk_expert_route_args* args, void* stream, char* err, size_t errlen);
+
+/* Products grouped by expert: for each entry i in [start[g], start[g + 1])
+ *   y[y_place ? y_place[i] : i] = act(w_g x[x_place ? x_place[i] / x_div : i] + bias_g)
+ * with matrix g at w + g * w_group.  gate = KK_GATE_NONE: `outputs` rows a matrix, act(z) = z.  With a gate a matrix has
+ * 2 * outputs rows, first the gates' and then the others', and act(z)_o = f(z_o) z_{outputs + o}: KK_GATE_SILU f(z) = z / (1 + exp(-z)),
+ * KK_GATE_GELU f(z) = z / 2 (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))), computed in f32 before the one rounding.
+ * The layer's first product takes kk_expert_route's `place` as x_place with x_div = top (rows of the layer's input to
+ * entries), its second as y_place (entries to rows of y by row and choice, as kk_expert_join reads them).  Rows of y that no
+ * entry goes to are left as they were; two entries with one place write the same row, in no order.  y overlaps no input.
+ * The result of an entry depends on `entries` and `groups` (by which a kernel is chosen: the order of f32 sums), not on the others. */
+#define KK_GATE_NONE 0
+#define KK_GATE_SILU 1
+#define KK_GATE_GELU 2
+typedef struct {
+    int32_t type;           /* KK_BF16 or KK_F16: x, w, y */
+    int32_t groups;         /* 1..KK_MOST_EXPERTS */
+    int32_t entries;        /* >= 0: start[groups] at most, by which the launch is sized; at most 2^28 */
+    int32_t inputs;         /* a multiple of 8 */
+    int32_t outputs;        /* >= 1 */
+    const int32_t* start;   /* [groups + 1], not falling */
+    const void* x;          /* 16-byte aligned, as are w and their strides */
+    int64_t x_rows, x_row;
+    const int32_t* x_place; /* [entries] or NULL */
+    int32_t x_div;          /* >= 1 where x_place is given */
+    const void* w;
+    int64_t w_row, w_group;
+    const float* bias;      /* [groups][rows of a matrix], or NULL */
+    int32_t gate;
+    void* y;
+    int64_t y_rows, y_row;
+    const int32_t* y_place; /* [entries] or NULL */
+    int32_t* fault;
+} kk_expert_product_args;
+int kk_expert_product(kk_ctx* ctx, const kk_expert_product_args* args, void* stream, char* err, size_t errlen);
+
+/* out[r] = base[r] + sum_j weight[r][j] y[r * top + j], in f32 in the order of j, rounded once.  A choice whose expert is
+ * negative is left out, its row of y not read.  `base` (the layer's input, a shared expert's result) may be NULL: 0.  `out`
+ * may be `base` (same stride) and overlaps nothing otherwise. */
+typedef struct {
+    int32_t type;           /* KK_BF16, KK_F16, KK_F32: y, base, out */
+    int32_t rows, top;      /* rows >= 0; top 1..KK_MOST_CHOICES */
+    int32_t values;         /* of a row, >= 1 */
+    const void* y;          /* [rows * top] rows */
+    int64_t y_row;
+    const int32_t* expert;  /* [rows][top] */
+    const float* weight;    /* [rows][top] */
+    const void* base;
+    int64_t base_row;
+    void* out;
+    int64_t out_row;
+} kk_expert_join_args;
+int kk_expert_join(kk_ctx* ctx, const kk_expert_join_args* args, void* stream, char* err, size_t errlen);
+
+/* y[r] = w x[r] + bias + scale[i] b_i (a_i x[r]) with i = adapter[r]; a row whose adapter is negative has no third term.  The rows
+ * may be in any order; those of one request next to each other are the fast case.  a_i x is kept with 16 bits or more before
+ * b_i.  With adapters = 0 it is the projection alone. */
+typedef struct {
+    int32_t type;           /* KK_BF16 or KK_F16: x, w, a, b */
+    int32_t out_type;       /* `type` or KK_F32: y */
+    int32_t rows;           /* >= 0, at most 2^24 */
+    int32_t inputs;         /* a multiple of 8 */
+    int32_t outputs;        /* >= 1 */
+    const void* x;          /* 16-byte aligned, as are w, a, b and their strides */
+    int64_t x_row;
+    const void* w;
+    int64_t w_row;
+    const float* bias;      /* [outputs], or NULL */
+    void* y;                /* overlaps no input */
+    int64_t y_row;
+    int32_t adapters;       /* >= 0 */
+    int32_t rank;           /* a multiple of 8, up to KK_MOST_RANK; adapters of a lower rank end in zeros */
+    const void* a;          /* [adapters][rank][inputs] */
+    const void* b;          /* [adapters][outputs][rank] */
+    const float* scale;     /* [adapters] */
+    const int32_t* adapter; /* [rows] */
+    int32_t* fault;
+    void* workspace;        /* 16-byte aligned, kk_adapter_product_workspace bytes or more; need not be cleared */
+    size_t workspace_bytes;
+} kk_adapter_product_args;
+/* As kk_expert_route_workspace.  It depends on rows, inputs, outputs, adapters, rank and the device's compute units alone. */
+int64_t kk_adapter_product_workspace(kk_ctx* ctx, const kk_adapter_product_args* args, char* err, size_t errlen);
+int kk_adapter_product(kk_ctx* ctx, const kk_adapter_product_args* args, void* stream, char* err, size_t errlen);
+
 /* ------------------------------------------------------------------ output formats (src/wav.rs)
  * PCM_16 encoding of the last run's audio on the device (wav::encode, src/wav.rs:63-80): per
  * sample v = round_ties_even(s * 32767) in f32; values outside [-32768, 32767] (NaN and the

@@ -99,6 +99,89 @@ std::string kv_attention_error(const kk_kv_cache* c, const kk_kv_batch* b, const
     return "";
 }
 
+std::string expert_route_error(const kk_expert_route_args* a) {
+    if (!a) return "null arguments";
+    if (a->type != KK_BF16 && a->type != KK_F16 && a->type != KK_F32) return "unknown type " + std::to_string(a->type);
+    if (a->experts < 1 || a->experts > KK_MOST_EXPERTS) return "expert count " + std::to_string(a->experts) + " out of range";
+    if (a->top < 1 || a->top > KK_MOST_CHOICES || a->top > a->experts) return "top " + std::to_string(a->top) + " out of range";
+    if (a->rows < 0 || (int64_t)a->rows * a->top > kMostRows) return "rows out of range";
+    if (a->score != KK_SCORE_SOFTMAX && a->score != KK_SCORE_SIGMOID) return "unknown score " + std::to_string(a->score);
+    if (a->renorm != 0 && a->renorm != 1) return "renorm is 0 or 1";
+    if (!std::isfinite(a->scale)) return "scale must be finite";
+    if (!a->start || (a->rows && (!a->logits || !a->expert || !a->weight || !a->place))) return "null array";
+    if (!aligned(a->logits, value_bytes(a->type)) || !aligned(a->expert, 4) || !aligned(a->weight, 4) || !aligned(a->start, 4) ||
+        !aligned(a->place, 4))
+        return "an array is not aligned to its values";
+    return "";
+}
+
+// Of the matrices and rows that the products load in 16-byte pieces.
+static std::string product_error(int type, int inputs, int outputs, const void* x, int64_t x_row, const void* w, int64_t w_row,
+                                 int64_t w_group, const void* y, size_t y_bytes) {
+    if (type != KK_BF16 && type != KK_F16) return "unknown type " + std::to_string(type);
+    if (inputs < 8 || inputs % 8 || inputs > kMostRows) return "inputs " + std::to_string(inputs) + " is no multiple of 8 in range";
+    if (outputs < 1 || outputs > kMostRows) return "outputs out of range";
+    if (!x || !w || !y) return "null array";
+    if (!aligned(x, 16) || !aligned(w, 16) || x_row % 8 || w_row % 8 || w_group % 8)
+        return "rows of x or w are not 16-byte aligned";
+    if (!aligned(y, y_bytes)) return "an array is not aligned to its values";
+    return "";
+}
+
+std::string expert_product_error(const kk_expert_product_args* a) {
+    if (!a) return "null arguments";
+    if (a->groups < 1 || a->groups > KK_MOST_EXPERTS) return "group count " + std::to_string(a->groups) + " out of range";
+    if (a->entries < 0 || a->entries > kMostRows) return "entries out of range";
+    if (a->gate != KK_GATE_NONE && a->gate != KK_GATE_SILU && a->gate != KK_GATE_GELU) return "unknown gate " + std::to_string(a->gate);
+    const std::string e = product_error(a->type, a->inputs, a->outputs, a->entries ? a->x : a->w, a->x_row, a->w, a->w_row, a->w_group,
+                                        a->entries ? a->y : a->w, 2);
+    if (!e.empty() || a->entries == 0) return e;
+    if (!a->start) return "null array";
+    if (!aligned(a->start, 4) || !aligned(a->x_place, 4) || !aligned(a->y_place, 4) || !aligned(a->bias, 4) || !aligned(a->fault, 4))
+        return "an array is not aligned to its values";
+    if (a->x_place && a->x_div < 1) return "x_div must be at least 1";
+    if (a->x_rows < (a->x_place ? 1 : a->entries)) return "x has fewer rows than entries";
+    if (a->y_rows < (a->y_place ? 1 : a->entries)) return "y has fewer rows than entries";
+    if (a->y == a->x) return "the output is an input";
+    return "";
+}
+
+std::string expert_join_error(const kk_expert_join_args* a) {
+    if (!a) return "null arguments";
+    if (a->type != KK_BF16 && a->type != KK_F16 && a->type != KK_F32) return "unknown type " + std::to_string(a->type);
+    if (a->top < 1 || a->top > KK_MOST_CHOICES) return "top " + std::to_string(a->top) + " out of range";
+    if (a->rows < 0 || (int64_t)a->rows * a->top > kMostRows) return "rows out of range";
+    if (a->values < 1 || a->values > kMostRows) return "values out of range";
+    if (a->rows == 0) return "";
+    if (!a->y || !a->expert || !a->weight || !a->out) return "null array";
+    const size_t e = value_bytes(a->type);
+    if (!aligned(a->y, e) || !aligned(a->base, e) || !aligned(a->out, e) || !aligned(a->expert, 4) || !aligned(a->weight, 4))
+        return "an array is not aligned to its values";
+    if (a->out == a->y) return "the output is an input";
+    if (a->out == a->base && a->out_row != a->base_row) return "an output in place of its input has other strides";
+    return "";
+}
+
+std::string adapter_product_error(const kk_adapter_product_args* a) {
+    if (!a) return "null arguments";
+    if (a->rows < 0 || a->rows > kMostRows / 16) return "rows out of range";
+    if (a->out_type != a->type && a->out_type != KK_F32) return "the output's type is neither the inputs' nor f32";
+    const std::string e = product_error(a->type, a->inputs, a->outputs, a->rows ? a->x : a->w, a->x_row, a->w, a->w_row, 0,
+                                        a->rows ? a->y : a->w, value_bytes(a->out_type));
+    if (!e.empty()) return e;
+    if (a->adapters < 0) return "adapters out of range";
+    if (a->adapters && (a->rank < 8 || a->rank % 8 || a->rank > KK_MOST_RANK))
+        return "rank " + std::to_string(a->rank) + " is no multiple of 8 in [8, 256]";
+    if (!aligned(a->bias, 4) || !aligned(a->fault, 4)) return "an array is not aligned to its values";
+    if (a->rows == 0) return "";
+    if (a->y == a->x || a->y == a->w) return "the output is an input";
+    if (!a->adapters) return "";
+    if (!a->a || !a->b || !a->scale || !a->adapter) return "null array";
+    if (!aligned(a->a, 16) || !aligned(a->b, 16)) return "rows of a or b are not 16-byte aligned";
+    if (!aligned(a->scale, 4) || !aligned(a->adapter, 4)) return "an array is not aligned to its values";
+    return "";
+}
+
 }  // namespace kk
 
 using kk::kGapN;

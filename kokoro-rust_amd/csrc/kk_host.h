@@ -25,4 +25,10 @@ std::string kv_batch_error(const kk_kv_cache* c, const kk_kv_batch* b);
 std::string kv_rows_error(const kk_kv_rows* r);
 std::string kv_attention_error(const kk_kv_cache* c, const kk_kv_batch* b, const kk_kv_attention_args* a);
 
+// The same of the products of ragged rows.
+std::string expert_route_error(const kk_expert_route_args* a);
+std::string expert_product_error(const kk_expert_product_args* a);
+std::string expert_join_error(const kk_expert_join_args* a);
+std::string adapter_product_error(const kk_adapter_product_args* a);
+
 }  // namespace kk

@@ -1,10 +1,11 @@
-// kk_ops.hip -- the C entries of the operators over an 8-bit cache: checks, the context's device, the launch.
+// kk_ops.hip -- the C entries of a language model's operators (attention over an 8-bit cache, products of ragged rows): checks, the context's device, the launch.
 // They enqueue on the caller's stream, allocate nothing and touch nothing of the context but its device.
 #include <cstdio>
 #include <new>
 
 #include "kk_host.h"
 #include "kk_kv.h"
+#include "kk_product.h"
 
 namespace kk {
 namespace {
@@ -56,6 +57,13 @@ auto no_throw(char* err, size_t errlen, F&& f) -> decltype(f()) {
     } catch (...) {
         return KK_ERR_INVALID;
     }
+}
+
+bool bad_workspace(const void* p, size_t bytes, int64_t need) {
+    return need && (!p || bytes < (size_t)need || (uintptr_t)p % 16);
+}
+std::string workspace_error(int64_t need) {
+    return "the workspace is null, not 16-byte aligned or smaller than " + std::to_string(need) + " bytes";
 }
 
 bool empty(const kk_kv_batch& b) { return b.n == 0 || b.rows == 0 || b.max_new == 0; }
@@ -123,10 +131,77 @@ int kk_kv_attention(kk_ctx* ctx, const kk_kv_cache* cache, const kk_kv_batch* ba
         if (empty(*batch)) return (int)KK_OK;
         const AttnPlan p = attention_plan(*cache, *batch, *args, ctx_cus(ctx));
         if (!attention_fits(p, *batch, args->heads, cache->heads)) return refuse(err, errlen, KK_ERR_INVALID, kTooLarge);
-        if (p.ws_bytes && (!args->workspace || args->workspace_bytes < (size_t)p.ws_bytes || (uintptr_t)args->workspace % 16))
-            return refuse(err, errlen, KK_ERR_INVALID,
-                          "the workspace is null, not 16-byte aligned or smaller than " + std::to_string(p.ws_bytes) + " bytes");
+        if (bad_workspace(args->workspace, args->workspace_bytes, p.ws_bytes))
+            return refuse(err, errlen, KK_ERR_INVALID, workspace_error(p.ws_bytes));
         return entry(ctx, err, errlen, [&] { return launch_kv_attention(*cache, *batch, *args, p, (hipStream_t)stream); });
+    });
+}
+
+int64_t kk_expert_route_workspace(kk_ctx* ctx, const kk_expert_route_args* args, char* err, size_t errlen) {
+    return no_throw(err, errlen, [&]() -> int64_t {
+        const std::string e = expert_route_error(args);
+        if (!e.empty()) return refuse(err, errlen, KK_ERR_INVALID, e);
+        if (!ctx) return refuse(err, errlen, KK_ERR_INVALID, "null context");
+        return route_workspace(*args);
+    });
+}
+
+int kk_expert_route(kk_ctx* ctx, const kk_expert_route_args* args, void* stream, char* err, size_t errlen) {
+    return no_throw(err, errlen, [&] {
+        const std::string e = expert_route_error(args);
+        if (!e.empty()) return refuse(err, errlen, KK_ERR_INVALID, e);
+        if (!ctx) return refuse(err, errlen, KK_ERR_INVALID, "null context");
+        if (bad_workspace(args->workspace, args->workspace_bytes, route_workspace(*args)))
+            return refuse(err, errlen, KK_ERR_INVALID, workspace_error(route_workspace(*args)));
+        return entry(ctx, err, errlen, [&] { return launch_route(*args, (hipStream_t)stream); });
+    });
+}
+
+int kk_expert_product(kk_ctx* ctx, const kk_expert_product_args* args, void* stream, char* err, size_t errlen) {
+    return no_throw(err, errlen, [&] {
+        const std::string e = expert_product_error(args);
+        if (!e.empty()) return refuse(err, errlen, KK_ERR_INVALID, e);
+        if (!ctx) return refuse(err, errlen, KK_ERR_INVALID, "null context");
+        if (args->entries == 0) return (int)KK_OK;
+        const ProductPlan p = expert_plan(*args, ctx_cus(ctx));
+        if (!product_fits(p)) return refuse(err, errlen, KK_ERR_INVALID, kTooLarge);
+        return entry(ctx, err, errlen, [&] { return launch_expert_product(*args, p, (hipStream_t)stream); });
+    });
+}
+
+int kk_expert_join(kk_ctx* ctx, const kk_expert_join_args* args, void* stream, char* err, size_t errlen) {
+    return no_throw(err, errlen, [&] {
+        const std::string e = expert_join_error(args);
+        if (!e.empty()) return refuse(err, errlen, KK_ERR_INVALID, e);
+        if (!ctx) return refuse(err, errlen, KK_ERR_INVALID, "null context");
+        if ((int64_t)args->rows * args->values > kMostThreads) return refuse(err, errlen, KK_ERR_INVALID, kTooLarge);
+        return entry(ctx, err, errlen, [&] { return args->rows ? launch_join(*args, (hipStream_t)stream) : hipSuccess; });
+    });
+}
+
+int64_t kk_adapter_product_workspace(kk_ctx* ctx, const kk_adapter_product_args* args, char* err, size_t errlen) {
+    return no_throw(err, errlen, [&]() -> int64_t {
+        const std::string e = adapter_product_error(args);
+        if (!e.empty()) return refuse(err, errlen, KK_ERR_INVALID, e);
+        if (!ctx) return refuse(err, errlen, KK_ERR_INVALID, "null context");
+        if (args->rows == 0) return 0;
+        const ProductPlan p = adapter_plan(*args, ctx_cus(ctx));
+        if (!product_fits(p)) return refuse(err, errlen, KK_ERR_INVALID, kTooLarge);
+        return p.ws_bytes;
+    });
+}
+
+int kk_adapter_product(kk_ctx* ctx, const kk_adapter_product_args* args, void* stream, char* err, size_t errlen) {
+    return no_throw(err, errlen, [&] {
+        const std::string e = adapter_product_error(args);
+        if (!e.empty()) return refuse(err, errlen, KK_ERR_INVALID, e);
+        if (!ctx) return refuse(err, errlen, KK_ERR_INVALID, "null context");
+        if (args->rows == 0) return (int)KK_OK;
+        const ProductPlan p = adapter_plan(*args, ctx_cus(ctx));
+        if (!product_fits(p)) return refuse(err, errlen, KK_ERR_INVALID, kTooLarge);
+        if (bad_workspace(args->workspace, args->workspace_bytes, p.ws_bytes))
+            return refuse(err, errlen, KK_ERR_INVALID, workspace_error(p.ws_bytes));
+        return entry(ctx, err, errlen, [&] { return launch_adapter_product(*args, p, (hipStream_t)stream); });
     });
 }
 

@@ -33,6 +33,10 @@ EXPORTS = [
 ]
 BF16, F16, F32 = 1, 2, 3
 KV_PAGE, KV_INT8, KV_E4M3 = 64, 1, 2
+KK_PRODUCT_BAD_START, KK_PRODUCT_BAD_PLACE, KK_PRODUCT_BAD_ADAPTER = 1, 2, 4
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+GATE_NONE, GATE_SILU, GATE_GELU = 0, 1, 2
+MOST_EXPERTS, MOST_CHOICES, MOST_RANK = 1024, 32, 256
 KV_BAD_BATCH, KV_BAD_PAGE = 1, 2
 NOALLOC_MAX_ROWS = 65536
 NOALLOC_MAX_ITEMS = 64
@@ -118,6 +122,39 @@ class KvAttention(C.Structure):
                 ("causal", C.c_int32), ("window", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+class ExpertRoute(C.Structure):
+    """kk_expert_route_args: device pointers as integers."""
+    _fields_ = [("type", C.c_int32), ("rows", C.c_int32), ("experts", C.c_int32), ("top", C.c_int32), ("logits", C.c_void_p),
+                ("logits_row", C.c_int64), ("score", C.c_int32), ("renorm", C.c_int32), ("scale", C.c_float),
+                ("expert", C.c_void_p), ("weight", C.c_void_p), ("start", C.c_void_p), ("place", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class ExpertProduct(C.Structure):
+    """kk_expert_product_args."""
+    _fields_ = [("type", C.c_int32), ("groups", C.c_int32), ("entries", C.c_int32), ("inputs", C.c_int32), ("outputs", C.c_int32),
+                ("start", C.c_void_p), ("x", C.c_void_p), ("x_rows", C.c_int64), ("x_row", C.c_int64), ("x_place", C.c_void_p),
+                ("x_div", C.c_int32), ("w", C.c_void_p), ("w_row", C.c_int64), ("w_group", C.c_int64), ("bias", C.c_void_p),
+                ("gate", C.c_int32), ("y", C.c_void_p), ("y_rows", C.c_int64), ("y_row", C.c_int64), ("y_place", C.c_void_p),
+                ("fault", C.c_void_p)]
+
+
+class ExpertJoin(C.Structure):
+    """kk_expert_join_args."""
+    _fields_ = [("type", C.c_int32), ("rows", C.c_int32), ("top", C.c_int32), ("values", C.c_int32), ("y", C.c_void_p),
+                ("y_row", C.c_int64), ("expert", C.c_void_p), ("weight", C.c_void_p), ("base", C.c_void_p),
+                ("base_row", C.c_int64), ("out", C.c_void_p), ("out_row", C.c_int64)]
+
+
+class AdapterProduct(C.Structure):
+    """kk_adapter_product_args."""
+    _fields_ = [("type", C.c_int32), ("out_type", C.c_int32), ("rows", C.c_int32), ("inputs", C.c_int32), ("outputs", C.c_int32),
+                ("x", C.c_void_p), ("x_row", C.c_int64), ("w", C.c_void_p), ("w_row", C.c_int64), ("bias", C.c_void_p),
+                ("y", C.c_void_p), ("y_row", C.c_int64), ("adapters", C.c_int32), ("rank", C.c_int32), ("a", C.c_void_p),
+                ("b", C.c_void_p), ("scale", C.c_void_p), ("adapter", C.c_void_p), ("fault", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 class LaunchRecord(C.Structure):
     _fields_ = [("name", C.c_char * 48), ("cls", C.c_char * 32), ("ms", C.c_double), ("flop", C.c_double),
                 ("bytes", C.c_double)]
@@ -198,6 +235,14 @@ def lib():
         L.kk_kv_write.argtypes = [vp, C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(KvRows), vp, cp, sz]
         L.kk_kv_read.argtypes = L.kk_kv_write.argtypes
         L.kk_kv_attention.argtypes = [vp, C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(KvAttention), vp, cp, sz]
+        L.kk_expert_route.argtypes = [vp, C.POINTER(ExpertRoute), vp, cp, sz]
+        L.kk_expert_route_workspace.argtypes = [vp, C.POINTER(ExpertRoute), cp, sz]
+        L.kk_expert_route_workspace.restype = i64
+        L.kk_expert_product.argtypes = [vp, C.POINTER(ExpertProduct), vp, cp, sz]
+        L.kk_expert_join.argtypes = [vp, C.POINTER(ExpertJoin), vp, cp, sz]
+        L.kk_adapter_product.argtypes = [vp, C.POINTER(AdapterProduct), vp, cp, sz]
+        L.kk_adapter_product_workspace.argtypes = [vp, C.POINTER(AdapterProduct), cp, sz]
+        L.kk_adapter_product_workspace.restype = i64
         L.kk_kv_attention_workspace.argtypes = [vp, C.POINTER(KvCache), C.POINTER(KvBatch), C.POINTER(KvAttention), cp, sz]
         L.kk_kv_attention_workspace.restype = i64
         _lib = L
@@ -484,6 +529,46 @@ class Context:
         """kk_kv_attention_workspace: bytes (0: none needed)."""
         err = _err()
         n = lib().kk_kv_attention_workspace(self.h, C.byref(cache), C.byref(batch), C.byref(args), err, len(err))
+        if n < 0:
+            raise KKError(int(n), err.value.decode(errors="replace"))
+        return n
+
+    # -------------------------------------------------------------- products of ragged rows: experts and adapters
+    def expert_route(self, args, stream=0):
+        """kk_expert_route of an ExpertRoute, whose workspace holds expert_route_workspace bytes."""
+        rc = lib().kk_expert_route(self.h, C.byref(args), stream, _ops.err, 1024)
+        if rc:
+            _check(rc, _ops.err)
+
+    def expert_route_workspace(self, args):
+        """kk_expert_route_workspace: bytes (0: none needed)."""
+        return self._workspace(lib().kk_expert_route_workspace, args)
+
+    def expert_product(self, args, stream=0):
+        """kk_expert_product of an ExpertProduct."""
+        rc = lib().kk_expert_product(self.h, C.byref(args), stream, _ops.err, 1024)
+        if rc:
+            _check(rc, _ops.err)
+
+    def expert_join(self, args, stream=0):
+        """kk_expert_join of an ExpertJoin."""
+        rc = lib().kk_expert_join(self.h, C.byref(args), stream, _ops.err, 1024)
+        if rc:
+            _check(rc, _ops.err)
+
+    def adapter_product(self, args, stream=0):
+        """kk_adapter_product of an AdapterProduct, whose workspace holds adapter_product_workspace bytes."""
+        rc = lib().kk_adapter_product(self.h, C.byref(args), stream, _ops.err, 1024)
+        if rc:
+            _check(rc, _ops.err)
+
+    def adapter_product_workspace(self, args):
+        """kk_adapter_product_workspace: bytes (0: none needed)."""
+        return self._workspace(lib().kk_adapter_product_workspace, args)
+
+    def _workspace(self, call, args):
+        err = _err()
+        n = call(self.h, C.byref(args), err, len(err))
         if n < 0:
             raise KKError(int(n), err.value.decode(errors="replace"))
         return n
