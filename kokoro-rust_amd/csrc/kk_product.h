@@ -41,8 +41,8 @@ struct ProductDev {
     const uint16_t *a, *b;
     const float* scale;
     const int32_t* adapter;
-    int adapters, rank, slots;
-    float* h;           // [rows][rank], times the adapter's scale; or NULL:
+    int adapters, rank, slots, shrink;
+    float* h;           // [rows][rank], times the adapter's scale; or
     uint16_t* h2;       // [rows][2 rank]: each 8 values' first 16 bits and then what these leave, in units of h_unit[row]
     float* h_unit;      // [rows]
     float* part;        // [splits][entries][outputs]
@@ -52,8 +52,8 @@ struct ProductDev {
 // How a product is launched.
 enum { kFew = 0, kTiled = 1 };
 struct ProductPlan {
-    int kernel;     // kFew: up to 16 rows a block, from memory to registers; kTiled: through LDS
-    int M, N;       // rows and outputs of a tile
+    int kernel;     // kFew: up to 96 rows a block, from memory to registers; kTiled: through LDS
+    int M, N, KS;   // rows and outputs of a tile (few rows: of a unit, whose inputs KS waves share)
     int64_t blocks; // of the main kernel
     int splits, k_split;
     bool joined;    // adapters: parts of the main product are summed, and the adapters' share added, by a kernel of their own
