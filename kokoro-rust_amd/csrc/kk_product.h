@@ -1,5 +1,8 @@
 // kk_product.h -- products of ragged rows (experts, adapters): what their kernels share, and how the host sizes them.
 #pragma once
+#include <algorithm>
+#include <type_traits>
+
 #include "kk_kv.h"
 
 namespace kk {
@@ -9,21 +12,17 @@ struct Rows {
     int g, first, count;
 };
 
-// Which rows row tile `tile` holds.  A group of m rows has at most m / M + 1 tiles of M, so the numbers from start / M + g on
-// are its own, without a sum over the groups before it; some of them stay empty.  Groups that a bad `start` lets overlap may claim one
-// tile together: what is left in `i` is then checked against the group as any tile is.
-__host__ __device__ inline int64_t row_tiles(int64_t entries, int groups, int M) { return entries / M + groups; }
-__host__ __device__ inline bool group_ok(int s0, int s1, int entries) { return s0 >= 0 && s1 >= s0 && s1 <= entries; }
-__host__ __device__ inline bool group_has(int s0, int s1, int g, int64_t tile, int M, int& i) {
-    const int64_t base = (int64_t)(s0 / M) + g;
-    i = (int)(tile - base);
-    return tile >= base && tile < (int64_t)(s1 / M) + g + 1;
+// Row tiles of a group: as many as its rows need.  A tile's number counts those of the groups before it.
+__host__ __device__ inline int64_t row_tiles(int64_t entries, int groups, int M) {  // at most
+    const int64_t n = entries / M + groups;
+    return n < entries ? n : entries;
 }
-__host__ __device__ inline bool group_rows(int s0, int s1, int g, int i, int M, Rows& r) {
+__host__ __device__ inline bool group_ok(int s0, int s1, int entries) { return s0 >= 0 && s1 >= s0 && s1 <= entries; }
+// Tile i of group g, whose rows are [s0, s1).
+__host__ __device__ inline void group_rows(int s0, int s1, int g, int i, int M, Rows& r) {
     r.g = g, r.first = s0 + i * M;
     const int left = s1 - r.first;
     r.count = left < M ? left : M;
-    return left > 0;
 }
 
 struct ProductDev {
@@ -35,33 +34,35 @@ struct ProductDev {
     const int32_t *start, *x_place, *y_place;  // start NULL: one group of all entries
     int32_t* fault;
     int x_div, entries, groups, inputs, outputs, gate;
-    int y_vec;     // 8-byte (f32: 16-byte) stores of 4 outputs
+    int y_vec;     // 1: 4 outputs in one store, 2: 8
     int tiles, tiles_n;
     // adapters
     const uint16_t *a, *b;
     const float* scale;
     const int32_t* adapter;
-    int adapters, rank, slots, shrink;
-    float* h;           // [rows][rank], times the adapter's scale; or
-    uint16_t* h2;       // [rows][2 rank]: each 8 values' first 16 bits and then what these leave, in units of h_unit[row]
-    float* h_unit;      // [rows]
-    float* part;        // [splits][entries][outputs]
+    int adapters, rank;
+    int shrink, slots, h_splits, h_k;  // blocks that make h, how many share a row tile's adapters, and its inputs
+    float* h;        // [h_splits][rows][rank], times the adapter's scale
+    uint16_t* h2;    // [rows][2 rank]: each 8 values' first 16 bits and then what these leave, in units of h_unit[row]
+    float* h_unit;   // [rows]
+    float* part;     // [splits][entries][outputs]
     int splits, k_split;
 };
 
 // How a product is launched.
-enum { kFew = 0, kTiled = 1 };
+enum { k32, k64, k128Narrow, k128, k128Wide, k256 };  // tiles, by their rows of x
 struct ProductPlan {
-    int kernel;     // kFew: up to 96 rows a block, from memory to registers; kTiled: through LDS
-    int M, N, KS;   // rows and outputs of a tile (few rows: of a unit, whose inputs KS waves share)
-    int64_t blocks; // of the main kernel
-    int splits, k_split;
-    bool joined;    // adapters: parts of the main product are summed, and the adapters' share added, by a kernel of their own
-    int64_t ws_h, ws_unit, ws_part, ws_bytes;  // workspace
+    int tile;
+    int64_t blocks;  // of the main kernel
+    int tiles, tiles_n, splits, k_split;
+    bool joined;     // adapters: parts of the main product are summed, and the adapters' share added, by a kernel of their own
+    int h_tile, slots, h_splits, h_k;
+    int64_t shrink;
+    int64_t ws_h2, ws_unit, ws_part, ws_bytes;  // workspace
 };
 ProductPlan expert_plan(const kk_expert_product_args& a, int n_cu);
 ProductPlan adapter_plan(const kk_adapter_product_args& a, int n_cu);
-inline bool product_fits(const ProductPlan& p) { return p.blocks * 512 <= kMostThreads; }
+inline bool product_fits(const ProductPlan& p) { return p.shrink * 512 <= kMostThreads / 2; }
 
 hipError_t launch_expert_product(const kk_expert_product_args& a, const ProductPlan& p, hipStream_t s);
 hipError_t launch_adapter_product(const kk_adapter_product_args& a, const ProductPlan& p, hipStream_t s);

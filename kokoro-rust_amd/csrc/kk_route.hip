@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(256) join_kernel(JoinDev a) {
     auto load = [&](const void* p, int64_t from, float (&v)[V]) {
         const E* x = (const E*)p + from;
         if constexpr (V > 1) {
-            const uint4 q = stream_load((const uint4*)x);
+            const uint4 q = *(const uint4*)x;
             E e[V];
             __builtin_memcpy(e, &q, 16);
 #pragma unroll
