@@ -33,7 +33,8 @@ struct ProductDev {
     void* y;
     const int32_t *start, *x_place, *y_place;  // start NULL: one group of all entries
     int32_t* fault;
-    int x_div, entries, groups, inputs, outputs, gate;
+    double x_inv;  // 1 / x_div
+    int entries, groups, inputs, outputs, gate;
     int y_vec;     // 1: 4 outputs in one store, 2: 8
     int tiles, tiles_n;
     // adapters
@@ -62,7 +63,9 @@ struct ProductPlan {
 };
 ProductPlan expert_plan(const kk_expert_product_args& a, int n_cu);
 ProductPlan adapter_plan(const kk_adapter_product_args& a, int n_cu);
-inline bool product_fits(const ProductPlan& p) { return p.shrink * 512 <= kMostThreads / 2; }
+inline bool product_fits(const ProductPlan& p) {
+    return p.shrink * 512 <= kMostThreads / 2 && (int64_t)p.tiles * p.tiles_n <= (1 << 27) / p.splits;
+}
 
 hipError_t launch_expert_product(const kk_expert_product_args& a, const ProductPlan& p, hipStream_t s);
 hipError_t launch_adapter_product(const kk_adapter_product_args& a, const ProductPlan& p, hipStream_t s);

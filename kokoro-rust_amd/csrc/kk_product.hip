@@ -30,23 +30,26 @@ __device__ __forceinline__ void fault(const ProductDev& p, int bit) {
 }
 
 // The row of x of entry e, or -1.
-__device__ __forceinline__ int64_t x_of(const ProductDev& p, int e) {
+__device__ __forceinline__ int x_of(const ProductDev& p, int e) {
     if (!p.x_place) return e;
     const int place = p.x_place[e];
-    if (place < 0 || place / p.x_div >= p.x_rows) {
-        fault(p, KK_PRODUCT_BAD_PLACE);
-        return -1;
-    }
-    return place / p.x_div;
+    // place / x_div: the half keeps the product's rounding away from whole numbers
+    const int row = (int)(((double)place + 0.5) * p.x_inv);
+    if (place >= 0 && row < p.x_rows) return row;
+    fault(p, KK_PRODUCT_BAD_PLACE);
+    return -1;
 }
-__device__ __forceinline__ int64_t y_of(const ProductDev& p, int e) {
-    if (!p.y_place) return e;
-    const int place = p.y_place[e];
-    if (place < 0 || place >= p.y_rows) {
-        fault(p, KK_PRODUCT_BAD_PLACE);
-        return -1;
+// The row of y of entry e, or -1 where it or the row of x is none.
+__device__ __forceinline__ int y_of(const ProductDev& p, int e) {
+    int place = e;
+    if (p.y_place) {
+        place = p.y_place[e];
+        if (place < 0 || place >= p.y_rows) {
+            fault(p, KK_PRODUCT_BAD_PLACE);
+            return -1;
+        }
     }
-    return place;
+    return p.x_place && x_of(p, e) < 0 ? -1 : place;
 }
 __device__ __forceinline__ int adapter_of(const ProductDev& p, int row) {
     const int id = p.adapter[row];
@@ -193,6 +196,10 @@ __device__ __forceinline__ void run_stages(const Place<C>& at, const uint16_t* (
         barrier();
     };
     wait(steps < S - 1);
+    // whatever the addresses still depend on (a place's load, a register kept in scratch) is waited for here: a wait of the compiler's
+    // own inside the loop would be for all loads
+#pragma unroll
+    for (int q = 0; q < Q; q++) asm volatile("" : "+v"(src[q]));
     if (live) {
 #pragma unroll
         for (int i = 0; i < kRead; i++) acc.read(at, 0, at.lds, 0, i);
@@ -418,26 +425,28 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
     // outputs wide, which share rows of x and matrices in its L2.
     const Groups groups = sum_groups<C::M>(p, more_lds);
     const int block = blockIdx.x - (OUT == 0 ? p.shrink : 0), blocks = gridDim.x - (OUT == 0 ? p.shrink : 0);
-    const int tall = groups.tiles * p.splits;
-    const int64_t total = (int64_t)tall * p.tiles_n;
-    const int64_t per = (total + 7) / 8, end = min(total, (block % 8 + 1) * per);
-    int64_t t = block % 8 * per + block / 8;
-    const int stride = blocks / 8;
-    auto work_of = [&](int64_t t) {
+    const int tall = groups.tiles * p.splits, total = tall * p.tiles_n;
+    const int per = (total + 7) / 8, end = min(total, (block % 8 + 1) * per);
+    int t = block % 8 * per + block / 8;
+    auto work_of = [&](int t) {
         Work w;
-        const int strip = (int)(t / (8 * (int64_t)tall)), wide = min(8, p.tiles_n - 8 * strip), in = (int)(t - strip * (8 * (int64_t)tall));
-        w.n0 = (8 * strip + in % wide) * kOutN;
-        const int rest = in / wide;
-        w.split = rest % p.splits;
-        w.r = rows_of<C::M>(p, groups, rest / p.splits);
+        const int strip = t / (8 * tall), wide = min(8, p.tiles_n - 8 * strip), in = t - strip * (8 * tall), rest = in / wide;
+        w.n0 = (8 * strip + (in - rest * wide)) * kOutN;
+        const int tile = rest / p.splits;
+        w.split = rest - tile * p.splits;
+        w.r = rows_of<C::M>(p, groups, tile);
         w.k_lo = w.split * p.k_split;
         const int k = min(p.inputs, w.k_lo + p.k_split) - w.k_lo;
         w.steps = k / K, w.rest = k % K;
         return w;
     };
-    // where this lane's loads begin
+    // the rows of x that this lane loads
+    auto rows_in = [&](const Work& w, int (&row)[C::QX]) {
+#pragma unroll
+        for (int q = 0; q < C::QX; q++) row[q] = max(x_of(p, w.r.first + min(at.row(q), w.r.count - 1)), 0);
+    };
     const uint16_t* src[C::Q];
-    auto aim = [&](const Work& w) {
+    auto aim = [&](const Work& w, const int (&x_row)[C::QX]) {
         const uint16_t* wg = p.w + w.r.g * p.w_group + w.k_lo + at.piece;
 #pragma unroll
         for (int q = 0; q < C::QW; q++) {
@@ -447,28 +456,41 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
                 o = min(w.n0 + row / 64 * 32 + row % 32, p.outputs - 1) + (row & 32 ? p.outputs : 0);
             else
                 o = min(w.n0 + row, p.outputs - 1);
-            src[q] = wg + (int64_t)o * p.w_row;
+            src[q] = wg + o * p.w_row;
         }
 #pragma unroll
-        for (int q = 0; q < C::QX; q++) {
-            const int64_t from = x_of(p, w.r.first + min(at.row(q), w.r.count - 1));
-            src[C::QW + q] = p.x + max(from, (int64_t)0) * p.x_row + w.k_lo + at.piece;
-        }
+        for (int q = 0; q < C::QX; q++) src[C::QW + q] = p.x + x_row[q] * p.x_row + w.k_lo + at.piece;
     };
     if (t >= end) return;
     Work w = work_of(t);
-    aim(w);
+    int x_row[C::QX];
+    rows_in(w, x_row);
+    aim(w, x_row);
     if (!EXT) begin<C>(at, src, w.steps);
     for (;;) {
+        // while the first stages are on their way: where this tile's results go, and what the next tile is
+        int to[C::FM];
+#pragma unroll
+        for (int j = 0; j < C::FM; j++) {
+            const int row = at.wm * (C::M / C::WM) + j * 32 + at.col;
+            to[j] = row < w.r.count ? OUT == 0 ? w.r.first + row : y_of(p, w.r.first + row) : -1;
+        }
+        const Work now = w;
+        t += blocks / 8;
+        const bool again = t < end;
+        if (again) {
+            w = work_of(t);
+            rows_in(w, x_row);
+        }
         acc.clear();
         if constexpr (EXT) {
             // each adapter's b beside the rows' h, which is zero in rows of another
             constexpr int kIds = (C::M + 63) / 64;
             int ids[kIds], mine[C::QX];  // of the tile's rows, a lane each; and of the rows that this lane loads
 #pragma unroll
-            for (int i = 0; i < kIds; i++) ids[i] = i * 64 + at.lane < w.r.count ? adapter_of(p, w.r.first + i * 64 + at.lane) : -1;
+            for (int i = 0; i < kIds; i++) ids[i] = i * 64 + at.lane < now.r.count ? adapter_of(p, now.r.first + i * 64 + at.lane) : -1;
 #pragma unroll
-            for (int q = 0; q < C::QX; q++) mine[q] = at.row(q) < w.r.count ? adapter_of(p, w.r.first + at.row(q)) : -1;
+            for (int q = 0; q < C::QX; q++) mine[q] = at.row(q) < now.r.count ? adapter_of(p, now.r.first + at.row(q)) : -1;
             bool any = false;
             for (int id = next_adapter(ids, -1); id != INT32_MAX; id = next_adapter(ids, id)) {
                 any = true;
@@ -476,10 +498,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
                     run_alone<T, C>(at, acc, [&](int q, uint16_t* to) {
                         const int k = k0 + at.piece;  // of a row of h2, whose b lies at half of it
                         if (q < C::QW) {
-                            const int o = min(w.n0 + at.row(q), p.outputs - 1);
+                            const int o = min(now.n0 + at.row(q), p.outputs - 1);
                             piece_or_zero(at, k < 2 * p.rank, p.b + ((int64_t)id * p.outputs + o) * p.rank + k / 16 * 8, to);
                         } else {
-                            const int row = w.r.first + min(at.row(q - C::QW), w.r.count - 1);
+                            const int row = now.r.first + min(at.row(q - C::QW), now.r.count - 1);
                             piece_or_zero(at, k < 2 * p.rank && mine[q - C::QW] == id, p.h2 + (int64_t)row * (2 * p.rank) + k, to);
                         }
                     });
@@ -487,7 +509,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
             if (T == KK_F16 && any) {
 #pragma unroll
                 for (int j = 0; j < C::FM; j++) {
-                    const int row = w.r.first + min(at.wm * (C::M / C::WM) + j * 32 + at.col, w.r.count - 1);
+                    const int row = now.r.first + min(at.wm * (C::M / C::WM) + j * 32 + at.col, now.r.count - 1);
                     const float unit = adapter_of(p, row) < 0 ? 1.0f : p.h_unit[row];
 #pragma unroll
                     for (int n = 0; n < C::FN; n++)
@@ -496,80 +518,76 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
                 }
             }
             barrier();
-            begin<C>(at, src, w.steps);
+            begin<C>(at, src, now.steps);
         }
-        if (w.rest)  // the inputs behind the last whole stage
+        const int n0 = now.n0 + at.wn * (kOutN / C::WN);
+        int quad = at.half * 4;
+        asm volatile("" : "+v"(quad));  // what depends on it is computed where it is used: kept over the loop it would go to scratch
+        if (OUT != 0 && p.bias) {
+            const float* bias = p.bias + (int64_t)now.r.g * p.outputs * (GATED ? 2 : 1);
+#pragma unroll
+            for (int i = 0; i < C::FN; i++)
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    const int o = min(n0 + (GATED ? i / 2 : i) * 32 + k / 4 * 8 + quad + k % 4, p.outputs - 1);
+                    const float b = bias[GATED && i % 2 ? p.outputs + o : o];
+#pragma unroll
+                    for (int j = 0; j < C::FM; j++) acc.sum[i][j][k] += b;
+                }
+        }
+        if (now.rest)  // the inputs behind the last whole stage
             run_alone<T, C>(at, acc, [&](int q, uint16_t* to) {
-                piece_or_zero(at, at.piece < w.rest, src[q] + (w.steps - min(C::S - 1, w.steps)) * K, to);
+                piece_or_zero(at, at.piece < now.rest, src[q] + (now.steps - min(C::S - 1, now.steps)) * K, to);
             });
-        run_stages<T, C>(at, src, w.steps, at.wm * (C::M / C::WM) < w.r.count, acc);
+        run_stages<T, C>(at, src, now.steps, at.wm * (C::M / C::WM) < now.r.count, acc);
 
         // the next tile's first stages are on their way while this one's results are stored
-        const Work done = w;
-        t += stride;
-        const bool again = t < end;
         if (again) {
-            w = work_of(t);
-            aim(w);
+            aim(w, x_row);
             barrier();  // all waves have read the last stage
             if (!EXT) begin<C>(at, src, w.steps);
         }
-        const Rows& r = done.r;
-        const float* bias = p.bias ? p.bias + (int64_t)r.g * p.outputs * (GATED ? 2 : 1) : nullptr;
 #pragma unroll
         for (int j = 0; j < C::FM; j++) {
-            const int row = at.wm * (C::M / C::WM) + j * 32 + at.col, e = r.first + row;
-            const int n0 = done.n0 + at.wn * (kOutN / C::WN);
-            if constexpr (OUT == 0) {
-                if (row >= r.count) continue;
-                float* to = p.part + ((int64_t)done.split * p.entries + e) * p.outputs;
 #pragma unroll
-                for (int i = 0; i < C::FN; i++)
+            for (int i = 0; i < C::FN; i += GATED ? 2 : 1) {
+                __builtin_amdgcn_sched_barrier(0);  // one piece at a time: the sums fill the registers
+                const int o = n0 + i * (GATED ? 16 : 32);
+                float v[4][4];
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        v[q][k] = acc.sum[i][j][4 * q + k];
+                        if constexpr (GATED) v[q][k] = gated(p.gate, v[q][k], acc.sum[i + 1][j][4 * q + k]);
+                    }
+                if constexpr (OUT == 0) {
+                    if (to[j] < 0) continue;
+                    float* part = p.part + ((int64_t)now.split * p.entries + to[j]) * p.outputs;
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
-                        const int o = n0 + i * 32 + q * 8 + at.half * 4, left = p.outputs - o;
-                        float v[4];
-#pragma unroll
-                        for (int k = 0; k < 4; k++) v[k] = acc.sum[i][j][4 * q + k];
-                        if (left > 0) store4<KK_F32>(to, o, p.outputs % 4 == 0, left, v);
+                        const int at_o = o + q * 8 + quad, left = p.outputs - at_o;
+                        if (left > 0) store4<KK_F32>(part, at_o, p.outputs % 4 == 0, left, v[q]);
                     }
-            } else {
-                int64_t to = -1;
-                if (row < r.count && (!p.x_place || x_of(p, e) >= 0)) to = y_of(p, e);
+                } else if (OUT != KK_F32 && p.y_vec == 2 && o + 32 <= p.outputs) {
+                    // two quads of a row on two lanes 32 apart to eight outputs on each
 #pragma unroll
-                for (int i = 0; i < C::FN; i += GATED ? 2 : 1) {
-                    float v[4][4];
+                    for (int q = 0; q < 4; q += 2) {
+                        uint32_t s[2][2];
 #pragma unroll
-                    for (int q = 0; q < 4; q++)
+                        for (int h = 0; h < 2; h++)
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const int o = min(n0 + i * (GATED ? 16 : 32) + q * 8 + at.half * 4 + k, p.outputs - 1);
-                            v[q][k] = acc.sum[i][j][4 * q + k];
-                            if (bias) v[q][k] += bias[o];
-                            if constexpr (GATED)
-                                v[q][k] = gated(p.gate, v[q][k], acc.sum[i + 1][j][4 * q + k] + (bias ? bias[p.outputs + o] : 0.0f));
-                        }
-                    const int o = n0 + i * (GATED ? 16 : 32);
-                    if (sizeof(typename ElemOf<OUT>::type) == 2 && p.y_vec == 2 && o + 32 <= p.outputs) {
-                        // two quads of a row on two lanes 32 apart to eight outputs on each
+                            for (int k = 0; k < 2; k++)
+                                s[h][k] = (uint32_t)ElemOf<T>::store(v[q + h][2 * k]) | (uint32_t)ElemOf<T>::store(v[q + h][2 * k + 1]) << 16;
+                        const auto a = __builtin_amdgcn_permlane32_swap(s[0][0], s[1][0], false, false);
+                        const auto b = __builtin_amdgcn_permlane32_swap(s[0][1], s[1][1], false, false);
+                        if (to[j] >= 0) *(uint4*)((uint16_t*)p.y + to[j] * p.y_row + o + q * 8 + quad * 2) = uint4{a[0], b[0], a[1], b[1]};
+                    }
+                } else if (to[j] >= 0) {
 #pragma unroll
-                        for (int q = 0; q < 4; q += 2) {
-                            uint32_t s[2][2];
-#pragma unroll
-                            for (int h = 0; h < 2; h++)
-#pragma unroll
-                                for (int k = 0; k < 2; k++)
-                                    s[h][k] = (uint32_t)ElemOf<T>::store(v[q + h][2 * k]) | (uint32_t)ElemOf<T>::store(v[q + h][2 * k + 1]) << 16;
-                            const auto a = __builtin_amdgcn_permlane32_swap(s[0][0], s[1][0], false, false);
-                            const auto b = __builtin_amdgcn_permlane32_swap(s[0][1], s[1][1], false, false);
-                            if (to >= 0) *(uint4*)((uint16_t*)p.y + to * p.y_row + o + (q + at.half) * 8) = uint4{a[0], b[0], a[1], b[1]};
-                        }
-                    } else if (to >= 0) {
-#pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            const int at_o = o + q * 8 + at.half * 4, left = p.outputs - at_o;
-                            if (left > 0) store4<OUT>(p.y, to * p.y_row + at_o, p.y_vec, left, v[q]);
-                        }
+                    for (int q = 0; q < 4; q++) {
+                        const int at_o = o + q * 8 + quad, left = p.outputs - at_o;
+                        if (left > 0) store4<OUT == 0 ? KK_F32 : OUT>(p.y, to[j] * p.y_row + at_o, p.y_vec, left, v[q]);
                     }
                 }
             }
@@ -761,7 +779,7 @@ hipError_t launch_expert_product(const kk_expert_product_args& a, const ProductP
     ProductDev d{};
     d.x = (const uint16_t*)a.x, d.w = (const uint16_t*)a.w, d.x_row = a.x_row, d.w_row = a.w_row, d.w_group = a.w_group;
     d.x_rows = a.x_rows, d.y_rows = a.y_rows, d.y_row = a.y_row, d.bias = a.bias, d.y = a.y;
-    d.start = a.start, d.x_place = a.x_place, d.y_place = a.y_place, d.fault = a.fault, d.x_div = a.x_div;
+    d.start = a.start, d.x_place = a.x_place, d.y_place = a.y_place, d.fault = a.fault, d.x_inv = 1.0 / std::max(a.x_div, 1);
     d.entries = a.entries, d.groups = a.groups, d.inputs = a.inputs, d.outputs = a.outputs, d.gate = a.gate;
     d.y_vec = (uintptr_t)a.y % 16 == 0 && a.y_row % 8 == 0 ? 2 : (uintptr_t)a.y % 8 == 0 && a.y_row % 4 == 0;
     d.splits = p.splits, d.k_split = p.k_split, d.tiles = p.tiles, d.tiles_n = p.tiles_n;
