@@ -185,8 +185,8 @@ int64_t kk_adapter_product_workspace(kk_ctx* ctx, const kk_adapter_product_args*
         if (!e.empty()) return refuse(err, errlen, KK_ERR_INVALID, e);
         if (!ctx) return refuse(err, errlen, KK_ERR_INVALID, "null context");
         if (args->rows == 0) return 0;
-        const ProductPlan p = adapter_plan(*args, ctx_cus(ctx));
-        if (!product_fits(p)) return refuse(err, errlen, KK_ERR_INVALID, kTooLarge);
+        const AdapterPlan p = adapter_plan(*args, ctx_cus(ctx));
+        if (!product_fits(p.main) || !product_fits(p.rest)) return refuse(err, errlen, KK_ERR_INVALID, kTooLarge);
         return p.ws_bytes;
     });
 }
@@ -197,8 +197,8 @@ int kk_adapter_product(kk_ctx* ctx, const kk_adapter_product_args* args, void* s
         if (!e.empty()) return refuse(err, errlen, KK_ERR_INVALID, e);
         if (!ctx) return refuse(err, errlen, KK_ERR_INVALID, "null context");
         if (args->rows == 0) return (int)KK_OK;
-        const ProductPlan p = adapter_plan(*args, ctx_cus(ctx));
-        if (!product_fits(p)) return refuse(err, errlen, KK_ERR_INVALID, kTooLarge);
+        const AdapterPlan p = adapter_plan(*args, ctx_cus(ctx));
+        if (!product_fits(p.main) || !product_fits(p.rest)) return refuse(err, errlen, KK_ERR_INVALID, kTooLarge);
         if (bad_workspace(args->workspace, args->workspace_bytes, p.ws_bytes))
             return refuse(err, errlen, KK_ERR_INVALID, workspace_error(p.ws_bytes));
         return entry(ctx, err, errlen, [&] { return launch_adapter_product(*args, p, (hipStream_t)stream); });

@@ -36,13 +36,13 @@ struct ProductDev {
     double x_inv;  // 1 / x_div
     int entries, groups, inputs, outputs, gate;
     int y_vec;     // 1: 4 outputs in one store, 2: 8
-    int tiles, tiles_n;
+    int tiles, tiles_n, blocks;
     // adapters
     const uint16_t *a, *b;
     const float* scale;
     const int32_t* adapter;
     int adapters, rank;
-    int shrink, slots, h_splits, h_k;  // blocks that make h, how many share a row tile's adapters, and its inputs
+    int slots, h_splits, h_k;  // blocks that share a row tile's adapters, and its inputs
     float* h;        // [h_splits][rows][rank], times the adapter's scale
     uint16_t* h2;    // [rows][2 rank]: each 8 values' first 16 bits and then what these leave, in units of h_unit[row]
     float* h_unit;   // [rows]
@@ -51,24 +51,27 @@ struct ProductDev {
 };
 
 // How a product is launched.
-enum { k32, k64, k128Narrow, k128, k128Wide, k256 };  // tiles, by their rows of x
+enum { k64, k128, k128Wide, k256 };  // tiles, by their rows of x
 struct ProductPlan {
     int tile;
-    int64_t blocks;  // of the main kernel
-    int tiles, tiles_n, splits, k_split;
-    bool joined;     // adapters: parts of the main product are summed, and the adapters' share added, by a kernel of their own
-    int h_tile, slots, h_splits, h_k;
-    int64_t shrink;
+    int blocks, tiles, tiles_n, splits, k_split;
+    int64_t shrink;  // blocks of the adapters' h
+};
+struct AdapterPlan {
+    ProductPlan main, rest;  // of the first `rows` rows and of those behind
+    int rows;
+    bool joined;     // parts of the main product are summed, and the adapters' share added, by a kernel of their own
+    int slots, h_splits, h_k;
     int64_t ws_h2, ws_unit, ws_part, ws_bytes;  // workspace
 };
 ProductPlan expert_plan(const kk_expert_product_args& a, int n_cu);
-ProductPlan adapter_plan(const kk_adapter_product_args& a, int n_cu);
+AdapterPlan adapter_plan(const kk_adapter_product_args& a, int n_cu);
 inline bool product_fits(const ProductPlan& p) {
-    return p.shrink * 512 <= kMostThreads / 2 && (int64_t)p.tiles * p.tiles_n <= (1 << 27) / p.splits;
+    return p.shrink * 512 <= kMostThreads / 2 && (int64_t)p.tiles * p.tiles_n * p.splits <= 1 << 28;
 }
 
 hipError_t launch_expert_product(const kk_expert_product_args& a, const ProductPlan& p, hipStream_t s);
-hipError_t launch_adapter_product(const kk_adapter_product_args& a, const ProductPlan& p, hipStream_t s);
+hipError_t launch_adapter_product(const kk_adapter_product_args& a, const AdapterPlan& p, hipStream_t s);
 int64_t route_workspace(const kk_expert_route_args& a);
 hipError_t launch_route(const kk_expert_route_args& a, hipStream_t s);
 hipError_t launch_join(const kk_expert_join_args& a, hipStream_t s);

@@ -17,11 +17,17 @@ struct Mat<KK_BF16> {
     static __device__ __forceinline__ f32x16 mul(const uint4& a, const uint4& b, const f32x16& c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
+    static __device__ __forceinline__ f32x4 mul(const uint4& a, const uint4& b, const f32x4& c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
 };
 template <>
 struct Mat<KK_F16> {
     static __device__ __forceinline__ f32x16 mul(const uint4& a, const uint4& b, const f32x16& c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x4 mul(const uint4& a, const uint4& b, const f32x4& c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
 };
 
@@ -89,12 +95,12 @@ __device__ __forceinline__ void store4(void* base, int64_t at, int vec, int left
 
 // N rows of the matrix (outputs) and M rows of x, held by WN x WM waves in 32 x 32 tiles of the matrix cores, through LDS in stages of
 // 64 inputs, S of them in flight.
-template <int N_, int M_, int WN_, int WM_, int S_, int PER_CU_>
+template <int N_, int M_, int WN_, int WM_, int K_, int S_, int PER_CU_>
 struct Tile {
-    static constexpr int N = N_, M = M_, WN = WN_, WM = WM_, S = S_, kPerCu = PER_CU_, K = 64;
+    static constexpr int N = N_, M = M_, WN = WN_, WM = WM_, K = K_, S = S_, kPerCu = PER_CU_;
     static constexpr int kWaves = WN * WM, kThreads = 64 * kWaves;
     static constexpr int FN = N / WN / 32, FM = M / WM / 32;
-    static constexpr int kRowsIn = 8;  // rows that a wave's load covers: 8 pieces of 16 bytes of each
+    static constexpr int kPieces = K / 8, kRowsIn = 64 / kPieces;  // of 16 bytes of a row, and rows that a wave's load covers
     static constexpr int QW = N / kRowsIn / kWaves, QX = M / kRowsIn / kWaves, Q = QW + QX;
     static constexpr int kStage = (N + M) * K;  // in values
     static constexpr int kNext = kWaves * kRowsIn * K;  // from a wave's load to its next in LDS
@@ -116,8 +122,8 @@ __device__ __forceinline__ void barrier() {
     asm volatile("" ::: "memory");
 }
 
-// What a wave and a lane are in a tile.  A stage's rows are 128 bytes, eight pieces of 16, in an order that their row number turns
-// (by XOR with its bits 1 to 3), so that the 16 rows that LDS reads at once lie on all 64 banks; since the loads store lane after lane,
+// What a wave and a lane are in a tile.  A stage's rows are 64 inputs, eight pieces of 16 bytes, in an order that their row number turns
+// (by XOR with its bits 1 to 3; rows of 32 inputs, four pieces: bits 2 and 3), so that the 16 rows that LDS reads at once lie on all 64 banks; since the loads store lane after lane,
 // the order is made by which piece each lane loads.
 template <class C>
 struct Place {
@@ -127,10 +133,10 @@ struct Place {
     __device__ __forceinline__ explicit Place(uint16_t* l) : lds(l) {
         lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         wn = wave % C::WN, wm = wave / C::WN;
-        col = lane & 31, half = lane >> 5, turn = (col >> 1) & 7;
-        const int in_load = lane >> 3;
+        col = lane & 31, half = lane >> 5, turn = C::K == 64 ? (col >> 1) & 7 : (col >> 2) & 3;
+        const int in_load = lane / C::kPieces;
         row_in = wave * C::kRowsIn + in_load;
-        piece = ((lane & 7) ^ ((in_load >> 1) + 4 * (wave & 1))) * 8;
+        piece = ((lane % C::kPieces) ^ (C::K == 64 ? (in_load >> 1) + 4 * (wave & 1) : in_load >> 2)) * 8;
         in = lds + wave * (C::kRowsIn * C::K);
         in_at = lds_at(in);
     }
@@ -217,7 +223,8 @@ __device__ __forceinline__ void run_stages(const Place<C>& at, const uint16_t* (
                 from = at.lds + side * C::kStage;
             }
             // loads in the first half, so that they have the other to arrive
-            const int q0 = kk < 2 ? kk * Q / 2 : Q, q1 = kk < 2 ? (kk + 1) * Q / 2 : Q;
+            constexpr int kIn = kSub > 2 ? kSub / 2 : 1;
+            const int q0 = min(kk, kIn) * Q / kIn, q1 = min(kk + 1, kIn) * Q / kIn;
             if constexpr (kOn) {
                 int next = 0, q = q0;
 #pragma unroll
@@ -296,6 +303,122 @@ __device__ __forceinline__ int next_adapter(const int (&ids)[N], int id) {
     return __builtin_amdgcn_readfirstlane(m);
 }
 
+// ------------------------------------------------------------------ adapters: h = s a x
+
+// Of 16 rows, 32 ranks and a share of the inputs, of every slots-th of the rows' adapters.  Straight from memory to registers, in 16-byte
+// loads that are the operands; the waves share the inputs and leave their sums in LDS.  W * 16 * 36 floats of LDS.
+template <int T, int W>
+__device__ __forceinline__ void shrink_few(const ProductDev& p, int block, float* lds) {
+    constexpr int kLd = 36, J = 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, g = lane >> 4;
+    const int split = block % p.h_splits, ranks = (p.rank + 31) / 32;
+    int rest = block / p.h_splits;
+    const int r0 = rest % ranks * 32;
+    rest /= ranks;
+    const int slot = rest % p.slots, first = rest / p.slots * 16, count = min(16, p.entries - first);
+    const int ids[1] = {col < count ? adapter_of(p, first + col) : -1};
+    const int share = (p.h_k / W + 31) / 32 * 32;  // of a wave
+    const int k_lo = split * p.h_k + wave * share, k_hi = min(min(p.inputs, (split + 1) * p.h_k), k_lo + share);
+    const uint16_t* x = p.x + (int64_t)(first + max(min(col, count - 1), 0)) * p.x_row + g * 8;
+    int id = -1;
+    for (int n = 0;; n++) {
+        id = next_adapter(ids, id);
+        if (id == INT32_MAX) return;
+        if (n % p.slots != slot) continue;
+        const uint16_t* w[2];
+        f32x4 acc[2] = {};
+#pragma unroll
+        for (int t = 0; t < 2; t++) w[t] = p.a + ((int64_t)id * p.rank + min(r0 + t * 16 + col, p.rank - 1)) * p.inputs + g * 8;
+        for (int k0 = k_lo; k0 < k_hi; k0 += 32 * J) {
+            const uint4 zero = {0, 0, 0, 0};
+            uint4 a[J][2], b[J];
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                const int k = k0 + 32 * j;
+                const bool in = k + g * 8 < k_hi;
+                b[j] = in ? *(const uint4*)(x + k) : zero;
+#pragma unroll
+                for (int t = 0; t < 2; t++) a[j][t] = in ? *(const uint4*)(w[t] + k) : zero;
+            }
+#pragma unroll
+            for (int j = 0; j < J; j++)
+#pragma unroll
+                for (int t = 0; t < 2; t++) acc[t] = Mat<T>::mul(a[j][t], b[j], acc[t]);
+        }
+        __syncthreads();  // the sums of the adapter before have been read
+#pragma unroll
+        for (int t = 0; t < 2; t++) *(f32x4*)&lds[(wave * 16 + col) * kLd + t * 16 + g * 4] = acc[t];
+        __syncthreads();
+        for (int i = threadIdx.x; i < 512; i += 64 * W) {
+            const int row = i >> 5, k = i & 31;
+            float v = 0.0f;
+#pragma unroll
+            for (int j = 0; j < W; j++) v += lds[(j * 16 + row) * kLd + k];
+            if (__shfl(ids[0], row) == id && r0 + k < p.rank) p.h[((int64_t)split * p.entries + first + row) * p.rank + r0 + k] = v * p.scale[id];
+        }
+    }
+}
+
+// Of many rows: of a row tile, of every slots-th of its adapters, as tiles of the products are.
+template <int T, class C>
+__global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) shrink_kernel(ProductDev p) {
+    constexpr int K = C::K;
+    __shared__ __align__(16) uint16_t lds[C::S * C::kStage];
+    const Place<C> at(lds);
+    Acc<T, C> acc;
+                constexpr int kIds = (C::M + 63) / 64;
+                const int n_ranks = (p.rank + C::N - 1) / C::N;
+                int rest = blockIdx.x;
+                const int split = rest % p.h_splits;
+                rest /= p.h_splits;
+                const int n0 = rest % n_ranks * C::N;
+                rest /= n_ranks;
+                const int slot = rest % p.slots, first = rest / p.slots * C::M, count = min(C::M, p.entries - first);
+                int ids[kIds];
+    #pragma unroll
+                for (int i = 0; i < kIds; i++) ids[i] = i * 64 + at.lane < count ? adapter_of(p, first + i * 64 + at.lane) : -1;
+                const int k_lo = split * p.h_k, k_hi = min(p.inputs, k_lo + p.h_k), steps = (k_hi - k_lo) / K, left = (k_hi - k_lo) % K;
+                int id = -1;
+                for (int n = 0;; n++) {
+                    id = next_adapter(ids, id);
+                    if (id == INT32_MAX) return;
+                    if (n % p.slots != slot) continue;
+                    const uint16_t* src[C::Q];
+    #pragma unroll
+                    for (int q = 0; q < C::QW; q++)
+                        src[q] = p.a + ((int64_t)id * p.rank + min(n0 + at.row(q), p.rank - 1)) * p.inputs + k_lo + at.piece;
+    #pragma unroll
+                    for (int q = 0; q < C::QX; q++)
+                        src[C::QW + q] = p.x + (int64_t)(first + min(at.row(q), count - 1)) * p.x_row + k_lo + at.piece;
+                    acc.clear();
+                    barrier();  // an adapter before has been read
+                    begin<C>(at, src, steps);
+                    if (left)
+                        run_alone<T, C>(at, acc, [&](int q, uint16_t* to) {
+                            piece_or_zero(at, at.piece < left, src[q] + (steps - min(C::S - 1, steps)) * K, to);
+                        });
+                    run_stages<T, C>(at, src, steps, at.wm * (C::M / C::WM) < count && n0 + at.wn * (C::N / C::WN) < p.rank, acc);
+                    const float s = p.scale[id];
+    #pragma unroll
+                    for (int j = 0; j < C::FM; j++) {
+                        const int row = at.wm * (C::M / C::WM) + j * 32 + at.col;
+                        if (row >= count || adapter_of(p, first + row) != id) continue;
+                        float* to = p.h + ((int64_t)split * p.entries + first + row) * p.rank;
+    #pragma unroll
+                        for (int i = 0; i < C::FN; i++)
+    #pragma unroll
+                            for (int q = 0; q < 4; q++) {
+                                const int o = n0 + at.wn * (C::N / C::WN) + i * 32 + q * 8 + at.half * 4;
+                                if (o >= p.rank) continue;  // a multiple of 8
+                                const f32x4 v = {acc.sum[i][j][4 * q] * s, acc.sum[i][j][4 * q + 1] * s, acc.sum[i][j][4 * q + 2] * s,
+                                                 acc.sum[i][j][4 * q + 3] * s};
+                                *(f32x4*)(to + o) = v;
+                            }
+                    }
+                }
+}
+
 // ------------------------------------------------------------------ the products
 
 // The groups' tiles summed up, in LDS: sums[g] of the groups before g, and starts[g].  The block's first wave makes it.
@@ -355,7 +478,7 @@ struct Work {
     int n0, split, k_lo, steps, rest;
 };
 
-// EXT: adapters in many rows, as more inputs (h2).  OUT = 0: sums to `part`; the grid's first p.shrink blocks then make h.
+// EXT: adapters in many rows, as more inputs (h2).  OUT = 0: sums to `part`, and the adapters' h in blocks behind p.blocks.
 template <int T, class C, bool GATED, bool EXT, int OUT>
 __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) product_kernel(ProductDev p) {
     constexpr int kOutN = GATED ? C::N / 2 : C::N, K = C::K;
@@ -366,65 +489,17 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
     Acc<T, C> acc;
 
     if constexpr (OUT == 0) {
-        // h = s a x of a row tile, of every slots-th of its adapters
-        if ((int)blockIdx.x < p.shrink) {
-            constexpr int kIds = (C::M + 63) / 64;
-            const int n_ranks = (p.rank + C::N - 1) / C::N;
-            int rest = blockIdx.x;
-            const int split = rest % p.h_splits;
-            rest /= p.h_splits;
-            const int n0 = rest % n_ranks * C::N;
-            rest /= n_ranks;
-            const int slot = rest % p.slots, first = rest / p.slots * C::M, count = min(C::M, p.entries - first);
-            int ids[kIds];
-#pragma unroll
-            for (int i = 0; i < kIds; i++) ids[i] = i * 64 + at.lane < count ? adapter_of(p, first + i * 64 + at.lane) : -1;
-            const int k_lo = split * p.h_k, k_hi = min(p.inputs, k_lo + p.h_k), steps = (k_hi - k_lo) / K, left = (k_hi - k_lo) % K;
-            int id = -1;
-            for (int n = 0;; n++) {
-                id = next_adapter(ids, id);
-                if (id == INT32_MAX) return;
-                if (n % p.slots != slot) continue;
-                const uint16_t* src[C::Q];
-#pragma unroll
-                for (int q = 0; q < C::QW; q++)
-                    src[q] = p.a + ((int64_t)id * p.rank + min(n0 + at.row(q), p.rank - 1)) * p.inputs + k_lo + at.piece;
-#pragma unroll
-                for (int q = 0; q < C::QX; q++)
-                    src[C::QW + q] = p.x + (int64_t)(first + min(at.row(q), count - 1)) * p.x_row + k_lo + at.piece;
-                acc.clear();
-                barrier();  // an adapter before has been read
-                begin<C>(at, src, steps);
-                if (left)
-                    run_alone<T, C>(at, acc, [&](int q, uint16_t* to) {
-                        piece_or_zero(at, at.piece < left, src[q] + (steps - min(C::S - 1, steps)) * K, to);
-                    });
-                run_stages<T, C>(at, src, steps, at.wm * (C::M / C::WM) < count && n0 + at.wn * (C::N / C::WN) < p.rank, acc);
-                const float s = p.scale[id];
-#pragma unroll
-                for (int j = 0; j < C::FM; j++) {
-                    const int row = at.wm * (C::M / C::WM) + j * 32 + at.col;
-                    if (row >= count || adapter_of(p, first + row) != id) continue;
-                    float* to = p.h + ((int64_t)split * p.entries + first + row) * p.rank;
-#pragma unroll
-                    for (int i = 0; i < C::FN; i++)
-#pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            const int o = n0 + at.wn * (C::N / C::WN) + i * 32 + q * 8 + at.half * 4;
-                            if (o >= p.rank) continue;  // a multiple of 8
-                            const f32x4 v = {acc.sum[i][j][4 * q] * s, acc.sum[i][j][4 * q + 1] * s, acc.sum[i][j][4 * q + 2] * s,
-                                             acc.sum[i][j][4 * q + 3] * s};
-                            *(f32x4*)(to + o) = v;
-                        }
-                }
-            }
+        // the adapters' blocks are the last: they run beside the others
+        if ((int)blockIdx.x >= p.blocks) {
+            shrink_few<T, C::kWaves>(p, blockIdx.x - p.blocks, (float*)lds);
+            return;
         }
     }
 
     // A block takes tile after tile.  Blocks go to the 8 XCDs in turn; an XCD takes tiles that follow each other, in strips eight tiles of
     // outputs wide, which share rows of x and matrices in its L2.
     const Groups groups = sum_groups<C::M>(p, more_lds);
-    const int block = blockIdx.x - (OUT == 0 ? p.shrink : 0), blocks = gridDim.x - (OUT == 0 ? p.shrink : 0);
+    const int block = blockIdx.x, blocks = p.blocks;
     const int tall = groups.tiles * p.splits, total = tall * p.tiles_n;
     const int per = (total + 7) / 8, end = min(total, (block % 8 + 1) * per);
     int t = block % 8 * per + block / 8;
@@ -631,97 +706,71 @@ __global__ void __launch_bounds__(256) halves_kernel(ProductDev p) {
     }
 }
 
-// y = the sum of the parts + bias + b h.  A block takes one row and 512 outputs.
+// y = the sum of the parts + bias + b h.  A block takes one row and 256 outputs, whose rows of b follow each other in memory: they are
+// read in 16-byte pieces thread after thread, and the pieces' sums put together through LDS.
 template <int T, int OUT>
-__global__ void __launch_bounds__(128) expand_kernel(ProductDev p) {
-    __shared__ float h[KK_MOST_RANK];
-    const int row = blockIdx.x / p.tiles_n, o = blockIdx.x % p.tiles_n * 512 + threadIdx.x * 4, left = p.outputs - o;
-    const int id = p.adapters ? adapter_of(p, row) : -1;
-    if (id >= 0)
-        for (int k = threadIdx.x; k < p.rank; k += 128) {
+__global__ void __launch_bounds__(256) expand_kernel(ProductDev p) {
+    __shared__ __align__(16) float h[KK_MOST_RANK];
+    __shared__ float sums[256 * (KK_MOST_RANK / 8 + 1)];
+    const int row = blockIdx.x / p.tiles_n, o0 = blockIdx.x % p.tiles_n * 256, o = o0 + threadIdx.x;
+    const int id = p.adapters ? adapter_of(p, row) : -1, pieces = p.rank / 8, ld = pieces | 1;
+    if (id >= 0) {
+        for (int k = threadIdx.x; k < p.rank; k += 256) {
             float v = 0.0f;
             for (int s = 0; s < p.h_splits; s++) v += p.h[((int64_t)s * p.entries + row) * p.rank + k];
             h[k] = v;
         }
-    __syncthreads();
-    if (left <= 0) return;
-    float v[4] = {};
-    const bool whole = p.outputs % 4 == 0;
-    for (int s = 0; s < p.splits; s++) {
-        const float* from = p.part + ((int64_t)s * p.entries + row) * p.outputs + o;
-        if (whole) {
-            const f32x4 q = *(const f32x4*)from;
+        __syncthreads();
+        const uint16_t* b = p.b + ((int64_t)id * p.outputs + o0) * p.rank;
+        const int all = min(256, p.outputs - o0) * pieces;
+        for (int i = threadIdx.x; i < all; i += 256) {
+            const uint4 q = *(const uint4*)(b + (int64_t)i * 8);
+            uint16_t e[8];
+            __builtin_memcpy(e, &q, 16);
+            const int at = i / pieces, piece = i - at * pieces;
+            float v = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; i++) v[i] += q[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++) v[i] += from[min(i, left - 1)];
+            for (int j = 0; j < 8; j++) v = fmaf(ElemOf<T>::load(e[j]), h[piece * 8 + j], v);
+            sums[at * ld + piece] = v;
         }
+        __syncthreads();
     }
-    if (p.bias)
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] += p.bias[o + min(i, left - 1)];
-    if (id >= 0) {
-        const uint16_t* b[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) b[i] = p.b + ((int64_t)id * p.outputs + o + min(i, left - 1)) * p.rank;
-        for (int k = 0; k < p.rank; k += 8) {
-            uint16_t e[4][8];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint4 q = *(const uint4*)(b[i] + k);
-                __builtin_memcpy(e[i], &q, 16);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float x = h[k + j];
-#pragma unroll
-                for (int i = 0; i < 4; i++) v[i] = fmaf(ElemOf<T>::load(e[i][j]), x, v[i]);
-            }
-        }
-    }
-    store4<OUT>(p.y, (int64_t)row * p.y_row + o, p.y_vec, left, v);
+    if (o >= p.outputs) return;
+    float v = p.bias ? p.bias[o] : 0.0f;
+    for (int s = 0; s < p.splits; s++) v += p.part[((int64_t)s * p.entries + row) * p.outputs + o];
+    if (id >= 0)
+        for (int k = 0; k < pieces; k++) v += sums[threadIdx.x * ld + k];
+    ((typename ElemOf<OUT>::type*)p.y)[(int64_t)row * p.y_row + o] = ElemOf<OUT>::store(v);
 }
 
 // ------------------------------------------------------------------ launches
 
-typedef Tile<128, 32, 4, 1, 4, 2> Tile32;
-typedef Tile<128, 32, 2, 1, 4, 2> Tile32Gated;
-typedef Tile<128, 64, 2, 2, 3, 2> Tile64;
-typedef Tile<64, 128, 2, 2, 3, 2> Tile128Narrow;
-typedef Tile<128, 128, 2, 2, 2, 2> Tile128;
-typedef Tile<256, 128, 2, 4, 3, 1> Tile128Wide;
-typedef Tile<256, 256, 2, 4, 2, 1> Tile256;
+typedef Tile<128, 64, 2, 2, 64, 3, 2> Tile64;
+typedef Tile<64, 128, 2, 2, 64, 3, 2> Tile128;
+typedef Tile<256, 128, 2, 4, 64, 3, 1> Tile128Wide;
+typedef Tile<256, 256, 2, 4, 32, 4, 1> Tile256;
 
 template <int T, class C, bool GATED, bool EXT, int OUT>
 hipError_t run_tile(const ProductDev& d, const ProductPlan& p, hipStream_t s) {
     const size_t lds = d.start ? 2 * ((size_t)d.groups + 1) * 4 : 0;
-    return launch(product_kernel<T, C, GATED, EXT, OUT>, dim3((unsigned)p.blocks + d.shrink), dim3(C::kThreads), lds, s, d);
-}
-
-template <int T, bool GATED, bool EXT, int OUT>
-hipError_t run_product(const ProductDev& d, const ProductPlan& p, hipStream_t s) {
-    switch (p.tile) {
-        case k32: return run_tile<T, std::conditional_t<GATED, Tile32Gated, Tile32>, GATED, EXT, OUT>(d, p, s);
-        case k64: return run_tile<T, Tile64, GATED, EXT, OUT>(d, p, s);
-        case k128Narrow: return run_tile<T, std::conditional_t<GATED, Tile128, Tile128Narrow>, GATED, EXT, OUT>(d, p, s);
-        case k128: return run_tile<T, Tile128, GATED, EXT, OUT>(d, p, s);
-        case k128Wide: return run_tile<T, Tile128Wide, GATED, EXT, OUT>(d, p, s);
-        default: return run_tile<T, Tile256, GATED, EXT, OUT>(d, p, s);
-    }
+    return launch(product_kernel<T, C, GATED, EXT, OUT>, dim3((unsigned)(d.blocks + (OUT == 0 ? p.shrink : 0))), dim3(C::kThreads), lds, s, d);
 }
 
 struct TileSize {
     int N, M, per_cu;
 };
-constexpr TileSize kTiles[] = {{128, 32, 2}, {128, 64, 2}, {64, 128, 2}, {128, 128, 2}, {256, 128, 1}, {256, 256, 1}};
+constexpr TileSize kTiles[] = {{128, 64, 2}, {64, 128, 2}, {256, 128, 1}, {256, 256, 1}};
 
 // The grid: as many blocks as tiles or as the device holds at once.
-void size_grid(ProductPlan& p, int64_t row_tiles, int wide, int n_cu) {
+void size_grid(ProductPlan& p, int64_t row_tiles, int64_t wide, int n_cu) {
     const TileSize& z = kTiles[p.tile];
     p.tiles = (int)row_tiles, p.tiles_n = (int)ceil_div(wide, z.N);
     const int64_t all = row_tiles * p.tiles_n * p.splits;
-    p.blocks = (std::min<int64_t>(all, (int64_t)z.per_cu * n_cu) + 7) / 8 * 8;
+    p.blocks = (int)((std::min<int64_t>(all, (int64_t)z.per_cu * n_cu) + 7) / 8 * 8);
+}
+
+void set_grid(ProductDev& d, const ProductPlan& p) {
+    d.splits = p.splits, d.k_split = p.k_split, d.tiles = p.tiles, d.tiles_n = p.tiles_n, d.blocks = p.blocks;
 }
 
 }  // namespace
@@ -729,50 +778,61 @@ void size_grid(ProductPlan& p, int64_t row_tiles, int wide, int n_cu) {
 ProductPlan expert_plan(const kk_expert_product_args& a, int n_cu) {
     ProductPlan p{};
     p.splits = 1, p.k_split = a.inputs;
-    const bool gate = a.gate != KK_GATE_NONE;
     const int64_t mean = a.entries / a.groups;
-    p.tile = mean <= 24 ? k32 : mean <= 64 ? k64 : mean < 384 ? k128Wide : k256;
-    size_grid(p, row_tiles(a.entries, a.groups, kTiles[p.tile].M), a.outputs * (gate ? 2 : 1), n_cu);
+    p.tile = mean <= 40 ? k64 : mean < 450 ? k128Wide : k256;
+    size_grid(p, row_tiles(a.entries, a.groups, kTiles[p.tile].M), (int64_t)a.outputs * (a.gate != KK_GATE_NONE ? 2 : 1), n_cu);
     return p;
 }
 
-ProductPlan adapter_plan(const kk_adapter_product_args& a, int n_cu) {
-    ProductPlan p{};
+AdapterPlan adapter_plan(const kk_adapter_product_args& a, int n_cu) {
+    AdapterPlan r{};
+    ProductPlan& p = r.main;
     p.splits = 1, p.k_split = a.inputs;
-    auto tiles = [&](int tile) { return ceil_div(a.rows, kTiles[tile].M) * ceil_div(a.outputs, kTiles[tile].N); };
-    p.tile = k256;
-    for (int tile : {k256, k128Wide, k128})
-        if (tiles(p.tile) < n_cu) p.tile = tile;
-    const int64_t many = tiles(p.tile);
-    p.joined = many < n_cu;
-    if (p.joined) {
-        p.tile = a.rows <= 32 ? k32 : a.rows <= 64 ? k64 : k128Narrow;
-        p.splits = (int)std::min<int64_t>(ceil_div(n_cu, tiles(p.tile)), std::max<int64_t>(1, a.inputs / 256));
+    auto tiles = [&](int64_t rows, int tile) { return ceil_div(rows, kTiles[tile].M) * ceil_div(a.outputs, kTiles[tile].N); };
+    p.tile = tiles(a.rows, k256) >= n_cu ? k256 : k128Wide;
+    r.joined = tiles(a.rows, p.tile) < n_cu;
+    int64_t rows = a.rows;
+    if (r.joined) {
+        p.tile = a.rows <= 64 ? k64 : k128;
+        const int64_t one = tiles(a.rows, p.tile), room = (int64_t)kTiles[p.tile].per_cu * n_cu;
+        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(room / one, a.inputs / 512));
         p.k_split = (int)ceil_div(ceil_div(a.inputs, p.splits), 64) * 64;
         p.splits = (int)ceil_div(a.inputs, p.k_split);
+    } else if (p.tile == k256) {
+        // Whole rounds of large tiles; the rows of a last round that would leave most of the device idle go to smaller ones.
+        const int64_t wide = ceil_div(a.outputs, 256), all = ceil_div(a.rows, 256) * wide, whole = all / n_cu * n_cu / wide * 256;
+        if ((all - whole / 256 * wide) * 2 < n_cu) rows = std::min<int64_t>(rows, whole);
     }
-    size_grid(p, ceil_div(a.rows, kTiles[p.tile].M), a.outputs, n_cu);
+    size_grid(p, ceil_div(rows, kTiles[p.tile].M), a.outputs, n_cu);
+    r.rows = (int)rows;
+    if (rows < a.rows) {
+        r.rest = p;
+        const int64_t left = a.rows - rows;
+        r.rest.tile = tiles(left, k128Wide) * 2 > n_cu ? k128Wide : k64;
+        size_grid(r.rest, ceil_div(left, kTiles[r.rest.tile].M), a.outputs, n_cu);
+    }
     if (a.adapters) {
-        // h: blocks that take about 512 inputs each
-        p.h_tile = p.joined ? p.tile : k64;
-        const TileSize& z = kTiles[p.h_tile];
-        p.h_k = (int)ceil_div(ceil_div(a.inputs, std::max(1, a.inputs / 512)), 64) * 64;
-        p.h_splits = (int)ceil_div(a.inputs, p.h_k);
-        const int64_t row_tiles = ceil_div(a.rows, z.M);
-        p.slots = (int)std::min<int64_t>(std::min(z.M, a.adapters), std::max<int64_t>(2, 32 / row_tiles));
-        p.shrink = (row_tiles * p.slots * ceil_div(a.rank, z.N) * p.h_splits + 7) / 8 * 8;
+        const int64_t of_rows = ceil_div(a.rows, r.joined ? 16 : kTiles[k128].M), of_ranks = ceil_div(a.rank, r.joined ? 32 : kTiles[k128].N);
+        // blocks that take 1,024 inputs each; in many rows as few as two a CU allow
+        const int64_t most = std::max<int64_t>(1, r.joined ? a.inputs / 1024 : std::min<int64_t>(a.inputs / 512, 2 * n_cu / (of_rows * of_ranks)));
+        r.h_k = (int)ceil_div(ceil_div(a.inputs, most), 64) * 64;
+        r.h_splits = (int)ceil_div(a.inputs, r.h_k);
+        r.slots = (int)std::min<int64_t>(a.adapters, r.joined && a.rows <= 512 ? 16 : 2);
+        p.shrink = of_rows * of_ranks * r.slots * r.h_splits;
     }
     auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
-    p.ws_h2 = a.adapters ? up((int64_t)p.h_splits * a.rows * a.rank * 4) : 0;
-    p.ws_unit = p.ws_h2 + (a.adapters && !p.joined ? up((int64_t)a.rows * a.rank * 4) : 0);
-    p.ws_part = p.ws_unit + (a.adapters && !p.joined ? up((int64_t)a.rows * 4) : 0);
-    p.ws_bytes = p.ws_part + (p.joined ? (int64_t)p.splits * a.rows * a.outputs * 4 : 0);
-    return p;
+    r.ws_h2 = a.adapters ? up((int64_t)r.h_splits * a.rows * a.rank * 4) : 0;
+    r.ws_unit = r.ws_h2 + (a.adapters && !r.joined ? up((int64_t)a.rows * a.rank * 4) : 0);
+    r.ws_part = r.ws_unit + (a.adapters && !r.joined ? up((int64_t)a.rows * 4) : 0);
+    r.ws_bytes = r.ws_part + (r.joined ? (int64_t)p.splits * a.rows * a.outputs * 4 : 0);
+    return r;
 }
 
-template <int T>
+template <int T, bool GATED>
 static hipError_t expert_run(const ProductDev& d, const ProductPlan& p, hipStream_t s) {
-    return d.gate ? run_product<T, true, false, T>(d, p, s) : run_product<T, false, false, T>(d, p, s);
+    if (p.tile == k64) return run_tile<T, Tile64, GATED, false, T>(d, p, s);
+    if (p.tile == k128Wide) return run_tile<T, Tile128Wide, GATED, false, T>(d, p, s);
+    return run_tile<T, Tile256, GATED, false, T>(d, p, s);
 }
 
 hipError_t launch_expert_product(const kk_expert_product_args& a, const ProductPlan& p, hipStream_t s) {
@@ -782,47 +842,61 @@ hipError_t launch_expert_product(const kk_expert_product_args& a, const ProductP
     d.start = a.start, d.x_place = a.x_place, d.y_place = a.y_place, d.fault = a.fault, d.x_inv = 1.0 / std::max(a.x_div, 1);
     d.entries = a.entries, d.groups = a.groups, d.inputs = a.inputs, d.outputs = a.outputs, d.gate = a.gate;
     d.y_vec = (uintptr_t)a.y % 16 == 0 && a.y_row % 8 == 0 ? 2 : (uintptr_t)a.y % 8 == 0 && a.y_row % 4 == 0;
-    d.splits = p.splits, d.k_split = p.k_split, d.tiles = p.tiles, d.tiles_n = p.tiles_n;
-    return a.type == KK_BF16 ? expert_run<KK_BF16>(d, p, s) : expert_run<KK_F16>(d, p, s);
+    set_grid(d, p);
+    if (a.type == KK_BF16) return d.gate ? expert_run<KK_BF16, true>(d, p, s) : expert_run<KK_BF16, false>(d, p, s);
+    return d.gate ? expert_run<KK_F16, true>(d, p, s) : expert_run<KK_F16, false>(d, p, s);
+}
+
+template <int T, bool EXT, int OUT>
+static hipError_t adapter_main(ProductDev d, const ProductPlan& p, hipStream_t s) {
+    set_grid(d, p);
+    if (p.tile == k64) return run_tile<T, Tile64, false, EXT, OUT>(d, p, s);
+    if (p.tile == k128Wide) return run_tile<T, Tile128Wide, false, EXT, OUT>(d, p, s);
+    return run_tile<T, Tile256, false, EXT, OUT>(d, p, s);
 }
 
 template <int T, int OUT>
-static hipError_t adapter_run(ProductDev d, const ProductPlan& p, hipStream_t s) {
+static hipError_t adapter_run(ProductDev d, const AdapterPlan& r, hipStream_t s) {
     hipError_t rc;
-    if (p.joined) {
-        d.shrink = (int)p.shrink;
-        rc = run_product<T, false, false, 0>(d, p, s);
+    if (r.joined) {
+        set_grid(d, r.main);
+        rc = r.main.tile == k64 ? run_tile<T, Tile64, false, false, 0>(d, r.main, s) : run_tile<T, Tile128, false, false, 0>(d, r.main, s);
         if (rc != hipSuccess) return rc;
-        d.tiles_n = (int)ceil_div(d.outputs, 512);
-        return launch(expand_kernel<T, OUT>, dim3((unsigned)((int64_t)d.entries * d.tiles_n)), dim3(128), 0, s, d);
+        d.tiles_n = (int)ceil_div(d.outputs, 256);
+        return launch(expand_kernel<T, OUT>, dim3((unsigned)((int64_t)d.entries * d.tiles_n)), dim3(256), 0, s, d);
     }
-    if (!d.adapters) return run_product<T, false, false, OUT>(d, p, s);
-    ProductDev h = d;
-    ProductPlan hp = p;
-    h.shrink = (int)p.shrink, hp.tile = p.h_tile, hp.blocks = 0;
-    rc = run_product<T, false, false, 0>(h, hp, s);
-    if (rc == hipSuccess) rc = launch(halves_kernel<T>, dim3((unsigned)ceil_div(d.entries, 8)), dim3(256), 0, s, d);
-    return rc == hipSuccess ? run_product<T, false, true, OUT>(d, p, s) : rc;
+    if (d.adapters) {
+        rc = launch(shrink_kernel<T, Tile128>, dim3((unsigned)r.main.shrink), dim3(Tile128::kThreads), 0, s, d);
+        if (rc == hipSuccess) rc = launch(halves_kernel<T>, dim3((unsigned)ceil_div(d.entries, 8)), dim3(256), 0, s, d);
+        if (rc != hipSuccess) return rc;
+    }
+    ProductDev rest = d;
+    d.entries = r.rows;
+    rc = d.adapters ? adapter_main<T, true, OUT>(d, r.main, s) : adapter_main<T, false, OUT>(d, r.main, s);
+    if (rc != hipSuccess || r.rows == rest.entries) return rc;
+    const int e = OUT == KK_F32 ? 4 : 2;
+    rest.x += r.rows * d.x_row, rest.y = (char*)d.y + r.rows * d.y_row * e, rest.entries -= r.rows;
+    if (d.adapters) rest.adapter += r.rows, rest.h2 += (int64_t)r.rows * 2 * d.rank, rest.h_unit += r.rows;
+    return d.adapters ? adapter_main<T, true, OUT>(rest, r.rest, s) : adapter_main<T, false, OUT>(rest, r.rest, s);
 }
 
-hipError_t launch_adapter_product(const kk_adapter_product_args& a, const ProductPlan& p, hipStream_t s) {
+hipError_t launch_adapter_product(const kk_adapter_product_args& a, const AdapterPlan& r, hipStream_t s) {
     ProductDev d{};
     d.x = (const uint16_t*)a.x, d.w = (const uint16_t*)a.w, d.x_row = a.x_row, d.w_row = a.w_row;
     d.x_rows = d.y_rows = a.rows, d.y_row = a.y_row, d.bias = a.bias, d.y = a.y, d.fault = a.fault;
     d.entries = a.rows, d.groups = 1, d.inputs = a.inputs, d.outputs = a.outputs;
     const int e = a.out_type == KK_F32 ? 4 : 2;
     d.y_vec = e == 2 && (uintptr_t)a.y % 16 == 0 && a.y_row % 8 == 0 ? 2 : (uintptr_t)a.y % (4 * e) == 0 && a.y_row % 4 == 0;
-    d.splits = p.splits, d.k_split = p.k_split, d.tiles = p.tiles, d.tiles_n = p.tiles_n;
     char* ws = (char*)a.workspace;
     d.adapters = a.adapters;
     if (a.adapters) {
         d.a = (const uint16_t*)a.a, d.b = (const uint16_t*)a.b, d.scale = a.scale, d.adapter = a.adapter, d.rank = a.rank;
-        d.h = (float*)ws, d.h2 = (uint16_t*)(ws + p.ws_h2), d.h_unit = (float*)(ws + p.ws_unit);
-        d.slots = p.slots, d.h_splits = p.h_splits, d.h_k = p.h_k;
+        d.h = (float*)ws, d.h2 = (uint16_t*)(ws + r.ws_h2), d.h_unit = (float*)(ws + r.ws_unit);
+        d.slots = r.slots, d.h_splits = r.h_splits, d.h_k = r.h_k;
     }
-    d.part = (float*)(ws + p.ws_part);
-    if (a.type == KK_BF16) return a.out_type == KK_F32 ? adapter_run<KK_BF16, KK_F32>(d, p, s) : adapter_run<KK_BF16, KK_BF16>(d, p, s);
-    return a.out_type == KK_F32 ? adapter_run<KK_F16, KK_F32>(d, p, s) : adapter_run<KK_F16, KK_F16>(d, p, s);
+    d.part = (float*)(ws + r.ws_part);
+    if (a.type == KK_BF16) return a.out_type == KK_F32 ? adapter_run<KK_BF16, KK_F32>(d, r, s) : adapter_run<KK_BF16, KK_BF16>(d, r, s);
+    return a.out_type == KK_F32 ? adapter_run<KK_F16, KK_F32>(d, r, s) : adapter_run<KK_F16, KK_F16>(d, r, s);
 }
 
 }  // namespace kk
