@@ -316,7 +316,7 @@ __device__ __forceinline__ void shrink_few(const ProductDev& p, int block, float
     int rest = block / p.h_splits;
     const int r0 = rest % ranks * 32;
     rest /= ranks;
-    const int slot = rest % p.slots, first = rest / p.slots * 16, count = min(16, p.entries - first);
+    const int tiles = (p.entries + 15) / 16, slot = rest / tiles, first = rest % tiles * 16, count = min(16, p.entries - first);
     const int ids[1] = {col < count ? adapter_of(p, first + col) : -1};
     const int share = (p.h_k / W + 31) / 32 * 32;  // of a wave
     const int k_lo = split * p.h_k + wave * share, k_hi = min(min(p.inputs, (split + 1) * p.h_k), k_lo + share);
@@ -374,7 +374,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) shrink
                 rest /= p.h_splits;
                 const int n0 = rest % n_ranks * C::N;
                 rest /= n_ranks;
-                const int slot = rest % p.slots, first = rest / p.slots * C::M, count = min(C::M, p.entries - first);
+                const int tiles = (p.entries + C::M - 1) / C::M, slot = rest / tiles, first = rest % tiles * C::M;
+    const int count = min(C::M, p.entries - first);
                 int ids[kIds];
     #pragma unroll
                 for (int i = 0; i < kIds; i++) ids[i] = i * 64 + at.lane < count ? adapter_of(p, first + i * 64 + at.lane) : -1;
@@ -707,40 +708,56 @@ __global__ void __launch_bounds__(256) halves_kernel(ProductDev p) {
 }
 
 // y = the sum of the parts + bias + b h.  A block takes one row and 256 outputs, whose rows of b follow each other in memory: they are
-// read in 16-byte pieces thread after thread, and the pieces' sums put together through LDS.
+// read in 16-byte pieces thread after thread, and the pieces' sums put together through LDS.  All its time is latency, so every load that
+// waits for nothing is made first.
 template <int T, int OUT>
 __global__ void __launch_bounds__(256) expand_kernel(ProductDev p) {
+    constexpr int kAhead = 4;
     __shared__ __align__(16) float h[KK_MOST_RANK];
-    __shared__ float sums[256 * (KK_MOST_RANK / 8 + 1)];
-    const int row = blockIdx.x / p.tiles_n, o0 = blockIdx.x % p.tiles_n * 256, o = o0 + threadIdx.x;
+    extern __shared__ float sums[];  // [256][rank / 8, made odd]
+    const int row = blockIdx.x / p.tiles_n, o0 = blockIdx.x % p.tiles_n * 256, tid = threadIdx.x;
+    const int o = min(o0 + tid, p.outputs - 1);
     const int id = p.adapters ? adapter_of(p, row) : -1, pieces = p.rank / 8, ld = pieces | 1;
-    if (id >= 0) {
-        for (int k = threadIdx.x; k < p.rank; k += 256) {
-            float v = 0.0f;
-            for (int s = 0; s < p.h_splits; s++) v += p.h[((int64_t)s * p.entries + row) * p.rank + k];
-            h[k] = v;
+    float part[kAhead], own = p.bias ? p.bias[o] : 0.0f, hk = 0.0f;
+    auto load_part = [&](int s) { return p.part[((int64_t)min(s, p.splits - 1) * p.entries + row) * p.outputs + o]; };
+#pragma unroll
+    for (int s = 0; s < kAhead; s++) part[s] = load_part(s);
+    if (tid < p.rank)
+        for (int s = 0; s < p.h_splits; s++) hk += p.h[((int64_t)s * p.entries + row) * p.rank + tid];
+    for (int s = 0; s < p.splits; s += kAhead) {
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            if (s) part[i] = load_part(s + i);
+            if (s + i < p.splits) own += part[i];
         }
-        __syncthreads();
+    }
+    if (id >= 0) {
         const uint16_t* b = p.b + ((int64_t)id * p.outputs + o0) * p.rank;
         const int all = min(256, p.outputs - o0) * pieces;
-        for (int i = threadIdx.x; i < all; i += 256) {
-            const uint4 q = *(const uint4*)(b + (int64_t)i * 8);
-            uint16_t e[8];
-            __builtin_memcpy(e, &q, 16);
-            const int at = i / pieces, piece = i - at * pieces;
-            float v = 0.0f;
+        uint4 q[kAhead];
 #pragma unroll
-            for (int j = 0; j < 8; j++) v = fmaf(ElemOf<T>::load(e[j]), h[piece * 8 + j], v);
-            sums[at * ld + piece] = v;
+        for (int j = 0; j < kAhead; j++) q[j] = *(const uint4*)(b + (int64_t)min(tid + j * 256, all - 1) * 8);
+        if (tid < p.rank) h[tid] = hk;
+        __syncthreads();
+        for (int i0 = tid; i0 < all; i0 += 256 * kAhead) {
+#pragma unroll
+            for (int j = 0; j < kAhead; j++) {
+                const int i = i0 + j * 256;
+                if (i >= all) break;
+                if (i0 != tid) q[j] = *(const uint4*)(b + (int64_t)i * 8);
+                uint16_t e[8];
+                __builtin_memcpy(e, &q[j], 16);
+                const int at = i / pieces, piece = i - at * pieces;
+                float v = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 8; k++) v = fmaf(ElemOf<T>::load(e[k]), h[piece * 8 + k], v);
+                sums[at * ld + piece] = v;
+            }
         }
         __syncthreads();
+        for (int k = 0; k < pieces; k++) own += sums[tid * ld + k];
     }
-    if (o >= p.outputs) return;
-    float v = p.bias ? p.bias[o] : 0.0f;
-    for (int s = 0; s < p.splits; s++) v += p.part[((int64_t)s * p.entries + row) * p.outputs + o];
-    if (id >= 0)
-        for (int k = 0; k < pieces; k++) v += sums[threadIdx.x * ld + k];
-    ((typename ElemOf<OUT>::type*)p.y)[(int64_t)row * p.y_row + o] = ElemOf<OUT>::store(v);
+    if (o0 + tid < p.outputs) ((typename ElemOf<OUT>::type*)p.y)[(int64_t)row * p.y_row + o] = ElemOf<OUT>::store(own);
 }
 
 // ------------------------------------------------------------------ launches
@@ -794,7 +811,8 @@ AdapterPlan adapter_plan(const kk_adapter_product_args& a, int n_cu) {
     int64_t rows = a.rows;
     if (r.joined) {
         p.tile = a.rows <= 64 ? k64 : k128;
-        const int64_t one = tiles(a.rows, p.tile), room = (int64_t)kTiles[p.tile].per_cu * n_cu;
+        // a block for each CU where that splits the inputs, else two: 96 tiles in 2 parts take as long as in 5, with less to sum up
+        const int64_t one = tiles(a.rows, p.tile), room = n_cu / one > 1 ? n_cu : 2 * n_cu;
         p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(room / one, a.inputs / 512));
         p.k_split = (int)ceil_div(ceil_div(a.inputs, p.splits), 64) * 64;
         p.splits = (int)ceil_div(a.inputs, p.k_split);
@@ -863,7 +881,7 @@ static hipError_t adapter_run(ProductDev d, const AdapterPlan& r, hipStream_t s)
         rc = r.main.tile == k64 ? run_tile<T, Tile64, false, false, 0>(d, r.main, s) : run_tile<T, Tile128, false, false, 0>(d, r.main, s);
         if (rc != hipSuccess) return rc;
         d.tiles_n = (int)ceil_div(d.outputs, 256);
-        return launch(expand_kernel<T, OUT>, dim3((unsigned)((int64_t)d.entries * d.tiles_n)), dim3(256), 0, s, d);
+        return launch(expand_kernel<T, OUT>, dim3((unsigned)((int64_t)d.entries * d.tiles_n)), dim3(256), 256 * ((size_t)d.rank / 8 | 1) * 4, s, d);
     }
     if (d.adapters) {
         rc = launch(shrink_kernel<T, Tile128>, dim3((unsigned)r.main.shrink), dim3(Tile128::kThreads), 0, s, d);

@@ -233,11 +233,16 @@ __global__ void __launch_bounds__(kRouteThreads) place_kernel(RouteDev a) {
     const int width = 1 << a.bits, ways = max(1, min(kRouteWaves, kRouteThreads / width)), e = tid & (width - 1), way = tid / width;
     int all = 0, before = 0;
     if (way < ways && e < a.experts) {
-#pragma unroll 8
-        for (int b = way; b < a.blocks; b += ways) {
-            const int c = a.counts[(int64_t)b * a.experts + e];
-            all += c;
-            before += b < (int)blockIdx.x ? c : 0;
+        for (int b0 = way; b0 < a.blocks; b0 += 16 * ways) {
+            int c[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) c[i] = a.counts[min(b0 + i * ways, a.blocks - 1) * a.experts + e];
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int b = b0 + i * ways;
+                all += b < a.blocks ? c[i] : 0;
+                before += b < (int)blockIdx.x ? c[i] : 0;
+            }
         }
         if (ways > 1) parts[way * a.experts + e] = all, parts[(ways + way) * a.experts + e] = before;
     }
@@ -282,59 +287,70 @@ struct JoinDev {
     int64_t y_row, base_row, out_row;
     const int32_t* expert;
     const float* weight;
-    int64_t pieces;  // of V values, of all rows
-    int top, per_row, vec;
+    int waves, top, values, per_row;  // waves of 64 V values a row
 };
 
-// V values of a row a thread (16 bytes, or one).  Bound by memory: every result is read once, kAhead of them in flight a thread.
+// A wave takes 64 V values of a row (V: 16 bytes, or one), so its row, experts and weights are scalars.  Bound by memory: every result is
+// read once, kAhead of them in flight a lane.
 template <int T, int V>
 __global__ void __launch_bounds__(256) join_kernel(JoinDev a) {
     typedef typename ElemOf<T>::type E;
     constexpr int kAhead = 8;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= a.pieces) return;
-    const int64_t row = i / a.per_row;
-    const int at = (int)(i % a.per_row) * V;
-    auto load = [&](const void* p, int64_t from, float (&v)[V]) {
-        const E* x = (const E*)p + from;
-        if constexpr (V > 1) {
-            const uint4 q = *(const uint4*)x;
-            E e[V];
-            __builtin_memcpy(e, &q, 16);
-#pragma unroll
-            for (int k = 0; k < V; k++) v[k] = ElemOf<T>::load(e[k]);
-        } else {
-            v[0] = ElemOf<T>::load(*x);
-        }
+    const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    if (wave >= a.waves) return;
+    const int row = wave / a.per_row, at = (wave - row * a.per_row) * (64 * V) + (threadIdx.x & 63) * V;
+    const bool in = at < a.values;
+    struct Piece {
+        E e[V];
     };
+    auto load = [&](const void* p, int64_t from) {
+        Piece x;
+        const E* q = (const E*)p + from + (in ? at : 0);
+        if constexpr (V > 1) {
+            const uint4 w = stream_load((const uint4*)q);
+            __builtin_memcpy(x.e, &w, 16);
+        } else {
+            x.e[0] = *q;
+        }
+        return x;
+    };
+    const int32_t* expert = a.expert + (int64_t)row * a.top;
+    const float* weight = a.weight + (int64_t)row * a.top;
     float sum[V] = {};
-    if (a.base) load(a.base, row * a.base_row + at, sum);
+    Piece base;
+    if (a.base) base = load(a.base, row * a.base_row);
     for (int j0 = 0; j0 < a.top; j0 += kAhead) {
-        float v[kAhead][V], w[kAhead];
+        Piece x[kAhead];
+        float w[kAhead];
         bool on[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; j++) {
-            on[j] = j0 + j < a.top && a.expert[row * a.top + j0 + j] >= 0;
-            if (!on[j]) continue;
-            w[j] = a.weight[row * a.top + j0 + j];
-            load(a.y, (row * a.top + j0 + j) * a.y_row + at, v[j]);
+            const int k = min(j0 + j, a.top - 1);
+            on[j] = j0 + j < a.top && expert[k] >= 0;
+            w[j] = weight[k];
         }
+#pragma unroll
+        for (int j = 0; j < kAhead; j++)
+            if (on[j]) x[j] = load(a.y, ((int64_t)row * a.top + j0 + j) * a.y_row);
+        if (j0 == 0 && a.base)
+#pragma unroll
+            for (int k = 0; k < V; k++) sum[k] = ElemOf<T>::load(base.e[k]);
 #pragma unroll
         for (int j = 0; j < kAhead; j++)
             if (on[j])
 #pragma unroll
-                for (int k = 0; k < V; k++) sum[k] = fmaf(w[j], v[j][k], sum[k]);
+                for (int k = 0; k < V; k++) sum[k] = fmaf(w[j], ElemOf<T>::load(x[j].e[k]), sum[k]);
     }
-    store_values<T, V>(a.out, row * a.out_row + at, V > 1, sum);
+    if (in) store_values<T, V>(a.out, row * a.out_row + at, V > 1, sum);
 }
 
 template <int T>
-hipError_t run_join(JoinDev d, int values, int64_t rows, hipStream_t s) {
+hipError_t run_join(JoinDev d, bool vec, int64_t rows, hipStream_t s) {
     constexpr int V = T == KK_F32 ? 4 : 8;
-    d.per_row = d.vec ? values / V : values;
-    d.pieces = rows * d.per_row;
-    const dim3 grid((unsigned)ceil_div(d.pieces, 256)), block(256);
-    return d.vec ? launch(join_kernel<T, V>, grid, block, 0, s, d) : launch(join_kernel<T, 1>, grid, block, 0, s, d);
+    d.per_row = (int)ceil_div(d.values, vec ? 64 * V : 64);
+    d.waves = (int)(rows * d.per_row);
+    const dim3 grid((unsigned)ceil_div(d.waves, 4)), block(256);
+    return vec ? launch(join_kernel<T, V>, grid, block, 0, s, d) : launch(join_kernel<T, 1>, grid, block, 0, s, d);
 }
 
 // Rows that a block chooses for, and blocks: few enough that adding up their counts stays short.
@@ -383,13 +399,13 @@ hipError_t launch_route(const kk_expert_route_args& a, hipStream_t s) {
 hipError_t launch_join(const kk_expert_join_args& a, hipStream_t s) {
     JoinDev d{};
     d.y = a.y, d.base = a.base, d.out = a.out, d.y_row = a.y_row, d.base_row = a.base_row, d.out_row = a.out_row;
-    d.expert = a.expert, d.weight = a.weight, d.top = a.top;
+    d.expert = a.expert, d.weight = a.weight, d.top = a.top, d.values = a.values;
     const int e = a.type == KK_F32 ? 4 : 2;
     auto whole = [&](const void* p, int64_t row) { return !p || ((uintptr_t)p % 16 == 0 && row * e % 16 == 0); };
-    d.vec = a.values * e % 16 == 0 && whole(a.y, a.y_row) && whole(a.base, a.base_row) && whole(a.out, a.out_row);
-    if (a.type == KK_BF16) return run_join<KK_BF16>(d, a.values, a.rows, s);
-    if (a.type == KK_F16) return run_join<KK_F16>(d, a.values, a.rows, s);
-    return run_join<KK_F32>(d, a.values, a.rows, s);
+    const bool vec = a.values * (int64_t)e % 16 == 0 && whole(a.y, a.y_row) && whole(a.base, a.base_row) && whole(a.out, a.out_row);
+    if (a.type == KK_BF16) return run_join<KK_BF16>(d, vec, a.rows, s);
+    if (a.type == KK_F16) return run_join<KK_F16>(d, vec, a.rows, s);
+    return run_join<KK_F32>(d, vec, a.rows, s);
 }
 
 }  // namespace kk
