@@ -35,33 +35,27 @@ __device__ __forceinline__ void fault(const ProductDev& p, int bit) {
     if (p.fault) atomicOr(p.fault, bit);
 }
 
-// The row of x of entry e, or -1.
-__device__ __forceinline__ int x_of(const ProductDev& p, int e) {
+// The row of x that entry e's place means, or -1.
+__device__ __forceinline__ int x_of(const ProductDev& p, int e, int place) {
     if (!p.x_place) return e;
-    const int place = p.x_place[e];
     // place / x_div: the half keeps the product's rounding away from whole numbers
     const int row = (int)(((double)place + 0.5) * p.x_inv);
     if (place >= 0 && row < p.x_rows) return row;
     fault(p, KK_PRODUCT_BAD_PLACE);
     return -1;
 }
-// The row of y of entry e, or -1 where it or the row of x is none.
-__device__ __forceinline__ int y_of(const ProductDev& p, int e) {
-    int place = e;
-    if (p.y_place) {
-        place = p.y_place[e];
-        if (place < 0 || place >= p.y_rows) {
-            fault(p, KK_PRODUCT_BAD_PLACE);
-            return -1;
-        }
-    }
-    return p.x_place && x_of(p, e) < 0 ? -1 : place;
+// The row of y, or -1.
+__device__ __forceinline__ int y_of(const ProductDev& p, int e, int place) {
+    if (!p.y_place) return e;
+    if (place >= 0 && place < p.y_rows) return place;
+    fault(p, KK_PRODUCT_BAD_PLACE);
+    return -1;
 }
-__device__ __forceinline__ int adapter_of(const ProductDev& p, int row) {
-    const int id = p.adapter[row];
+__device__ __forceinline__ int adapter_in(const ProductDev& p, int id) {
     if (id >= p.adapters) fault(p, KK_PRODUCT_BAD_ADAPTER);
     return id >= p.adapters || id < 0 ? -1 : id;
 }
+__device__ __forceinline__ int adapter_of(const ProductDev& p, int row) { return adapter_in(p, p.adapter[row]); }
 
 // f(gate) times its partner.  GELU: (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)), which loses nothing where tanh nears -1.
 __device__ __forceinline__ float gated(int kind, float g, float z) {
@@ -115,6 +109,9 @@ __device__ __forceinline__ uint32_t lds_at(const uint16_t* p) {
 }
 __device__ __forceinline__ void to_lds(const uint16_t* from, uint32_t to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory");
+}
+__device__ __forceinline__ void word_to_lds(const int32_t* from, uint32_t to) {  // 4 bytes a lane
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory");
 }
 __device__ __forceinline__ void barrier() {
     asm volatile("" ::: "memory");
@@ -485,6 +482,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
     constexpr int kOutN = GATED ? C::N / 2 : C::N, K = C::K;
     static_assert(!GATED || C::FN % 2 == 0, "a gate and its partner in one wave");
     __shared__ __align__(16) uint16_t lds[C::S * C::kStage];
+    __shared__ __align__(16) int places[2][2][C::M];
     extern __shared__ int more_lds[];  // [2][groups + 1]
     const Place<C> at(lds);
     Acc<T, C> acc;
@@ -516,13 +514,20 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
         w.steps = k / K, w.rest = k % K;
         return w;
     };
-    // the rows of x that this lane loads
-    auto rows_in = [&](const Work& w, int (&row)[C::QX]) {
+    // Where a tile's rows of x and y are (EXT: its rows' adapters): loaded to LDS beside the tile before, so that nothing waits for a load
+    // behind that tile's stores.
+    auto ask = [&](const Work& w, int side) {
+        const int32_t* const from[2] = {EXT ? p.adapter : p.x_place, p.y_place};
 #pragma unroll
-        for (int q = 0; q < C::QX; q++) row[q] = max(x_of(p, w.r.first + min(at.row(q), w.r.count - 1)), 0);
+        for (int i = 0; i < 2 * C::M / 64; i += C::kWaves) {
+            const int piece = i + at.wave, which = piece / (C::M / 64), r0 = piece % (C::M / 64) * 64;
+            if (piece < 2 * C::M / 64 && from[which])
+                word_to_lds(from[which] + w.r.first + min(r0 + at.lane, w.r.count - 1), lds_at((uint16_t*)&places[side][which][r0]));
+        }
     };
+    int to[C::FM];  // this lane's rows of y
     const uint16_t* src[C::Q];
-    auto aim = [&](const Work& w, const int (&x_row)[C::QX]) {
+    auto aim = [&](const Work& w, int side) {
         const uint16_t* wg = p.w + w.r.g * p.w_group + w.k_lo + at.piece;
 #pragma unroll
         for (int q = 0; q < C::QW; q++) {
@@ -535,28 +540,33 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
             src[q] = wg + o * p.w_row;
         }
 #pragma unroll
-        for (int q = 0; q < C::QX; q++) src[C::QW + q] = p.x + x_row[q] * p.x_row + w.k_lo + at.piece;
+        for (int q = 0; q < C::QX; q++) {
+            const int row = min(at.row(q), w.r.count - 1);
+            const int from = EXT ? w.r.first + row : max(x_of(p, w.r.first + row, places[side][0][row]), 0);
+            src[C::QW + q] = p.x + from * p.x_row + w.k_lo + at.piece;
+        }
+#pragma unroll
+        for (int j = 0; j < C::FM; j++) {
+            const int row = at.wm * (C::M / C::WM) + j * 32 + at.col, in = min(row, w.r.count - 1), e = w.r.first + in;
+            to[j] = OUT == 0 || EXT ? e : y_of(p, e, places[side][1][in]);
+            if (row >= w.r.count || (OUT != 0 && !EXT && x_of(p, e, places[side][0][in]) < 0)) to[j] = -1;
+        }
     };
     if (t >= end) return;
     Work w = work_of(t);
-    int x_row[C::QX];
-    rows_in(w, x_row);
-    aim(w, x_row);
+    ask(w, 0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    barrier();
+    aim(w, 0);
     if (!EXT) begin<C>(at, src, w.steps);
-    for (;;) {
-        // while the first stages are on their way: where this tile's results go, and what the next tile is
-        int to[C::FM];
-#pragma unroll
-        for (int j = 0; j < C::FM; j++) {
-            const int row = at.wm * (C::M / C::WM) + j * 32 + at.col;
-            to[j] = row < w.r.count ? OUT == 0 ? w.r.first + row : y_of(p, w.r.first + row) : -1;
-        }
+    for (int side = 0;; side ^= 1) {
+        // while the first stages are on their way: what the next tile is
         const Work now = w;
         t += blocks / 8;
         const bool again = t < end;
         if (again) {
             w = work_of(t);
-            rows_in(w, x_row);
+            ask(w, side ^ 1);
         }
         acc.clear();
         if constexpr (EXT) {
@@ -564,9 +574,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
             constexpr int kIds = (C::M + 63) / 64;
             int ids[kIds], mine[C::QX];  // of the tile's rows, a lane each; and of the rows that this lane loads
 #pragma unroll
-            for (int i = 0; i < kIds; i++) ids[i] = i * 64 + at.lane < now.r.count ? adapter_of(p, now.r.first + i * 64 + at.lane) : -1;
+            for (int i = 0; i < kIds; i++) ids[i] = i * 64 + at.lane < now.r.count ? adapter_in(p, places[side][0][i * 64 + at.lane]) : -1;
 #pragma unroll
-            for (int q = 0; q < C::QX; q++) mine[q] = at.row(q) < now.r.count ? adapter_of(p, now.r.first + at.row(q)) : -1;
+            for (int q = 0; q < C::QX; q++) mine[q] = at.row(q) < now.r.count ? adapter_in(p, places[side][0][at.row(q)]) : -1;
             bool any = false;
             for (int id = next_adapter(ids, -1); id != INT32_MAX; id = next_adapter(ids, id)) {
                 any = true;
@@ -585,8 +595,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
             if (T == KK_F16 && any) {
 #pragma unroll
                 for (int j = 0; j < C::FM; j++) {
-                    const int row = now.r.first + min(at.wm * (C::M / C::WM) + j * 32 + at.col, now.r.count - 1);
-                    const float unit = adapter_of(p, row) < 0 ? 1.0f : p.h_unit[row];
+                    const int row = min(at.wm * (C::M / C::WM) + j * 32 + at.col, now.r.count - 1);
+                    const float unit = adapter_in(p, places[side][0][row]) < 0 ? 1.0f : p.h_unit[now.r.first + row];
 #pragma unroll
                     for (int n = 0; n < C::FN; n++)
 #pragma unroll
@@ -618,9 +628,12 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
         run_stages<T, C>(at, src, now.steps, at.wm * (C::M / C::WM) < now.r.count, acc);
 
         // the next tile's first stages are on their way while this one's results are stored
+        int done[C::FM];
+#pragma unroll
+        for (int j = 0; j < C::FM; j++) done[j] = to[j];
+        barrier();  // all waves have read the last stage, and the next tile's places are there
         if (again) {
-            aim(w, x_row);
-            barrier();  // all waves have read the last stage
+            aim(w, side ^ 1);
             if (!EXT) begin<C>(at, src, w.steps);
         }
 #pragma unroll
@@ -638,8 +651,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
                         if constexpr (GATED) v[q][k] = gated(p.gate, v[q][k], acc.sum[i + 1][j][4 * q + k]);
                     }
                 if constexpr (OUT == 0) {
-                    if (to[j] < 0) continue;
-                    float* part = p.part + ((int64_t)now.split * p.entries + to[j]) * p.outputs;
+                    if (done[j] < 0) continue;
+                    float* part = p.part + ((int64_t)now.split * p.entries + done[j]) * p.outputs;
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
                         const int at_o = o + q * 8 + quad, left = p.outputs - at_o;
@@ -657,13 +670,13 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
                                 s[h][k] = (uint32_t)ElemOf<T>::store(v[q + h][2 * k]) | (uint32_t)ElemOf<T>::store(v[q + h][2 * k + 1]) << 16;
                         const auto a = __builtin_amdgcn_permlane32_swap(s[0][0], s[1][0], false, false);
                         const auto b = __builtin_amdgcn_permlane32_swap(s[0][1], s[1][1], false, false);
-                        if (to[j] >= 0) *(uint4*)((uint16_t*)p.y + to[j] * p.y_row + o + q * 8 + quad * 2) = uint4{a[0], b[0], a[1], b[1]};
+                        if (done[j] >= 0) *(uint4*)((uint16_t*)p.y + done[j] * p.y_row + o + q * 8 + quad * 2) = uint4{a[0], b[0], a[1], b[1]};
                     }
-                } else if (to[j] >= 0) {
+                } else if (done[j] >= 0) {
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
                         const int at_o = o + q * 8 + quad, left = p.outputs - at_o;
-                        if (left > 0) store4<OUT == 0 ? KK_F32 : OUT>(p.y, to[j] * p.y_row + at_o, p.y_vec, left, v[q]);
+                        if (left > 0) store4<OUT == 0 ? KK_F32 : OUT>(p.y, done[j] * p.y_row + at_o, p.y_vec, left, v[q]);
                     }
                 }
             }
