@@ -22,7 +22,8 @@ struct RouteDev {
     int64_t logits_row;
     int32_t *expert, *start, *place, *counts;  // counts: [blocks][experts]
     float* weight;
-    int rows, experts, top, score, renorm, vec, rows_block, blocks, bits;
+    int rows, experts, top, score, renorm, vec, rows_block, blocks;
+    int bits, width;  // bits of experts + 1 numbers; the power of two that holds the experts
     float scale;
 };
 
@@ -218,9 +219,11 @@ __global__ void __launch_bounds__(kRouteThreads) choose_kernel(RouteDev a) {
     if (tid < a.experts) hist[tid] = before, a.start[tid] = before;
     if (tid == a.experts - 1) hist[tid + 1] = before + count, a.start[tid + 1] = before + count;
     __syncthreads();
-    // what this block wrote to `expert` it also reads: the barriers above order that within a block
-    place_choices(a, 0, a.rows * a.top, hist, (uint16_t*)(lds + a.experts + 1),
-                   [&](int i) { return __hip_atomic_load(a.expert + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); });
+    // one block has at most kAtOnce rows, whose choices are all in LDS
+    place_choices(a, 0, a.rows * a.top, hist, (uint16_t*)(lds + a.experts + 1), [&](int i) {
+        const int r = i / a.top;
+        return chosen[r][i - r * a.top];
+    });
 }
 
 __global__ void __launch_bounds__(kRouteThreads) place_kernel(RouteDev a) {
@@ -230,7 +233,7 @@ __global__ void __launch_bounds__(kRouteThreads) place_kernel(RouteDev a) {
     const int tid = threadIdx.x;
     uint16_t* count = (uint16_t*)(base + a.experts + 1);
     // an expert's choices in all blocks, and in those before this one: each of `ways` threads adds up every ways-th block
-    const int width = 1 << a.bits, ways = max(1, min(kRouteWaves, kRouteThreads / width)), e = tid & (width - 1), way = tid / width;
+    const int width = a.width, ways = max(1, min(kRouteWaves, kRouteThreads / width)), e = tid & (width - 1), way = tid / width;
     int all = 0, before = 0;
     if (way < ways && e < a.experts) {
         for (int b0 = way; b0 < a.blocks; b0 += 16 * ways) {
@@ -385,7 +388,8 @@ hipError_t launch_route(const kk_expert_route_args& a, hipStream_t s) {
     d.counts = (int32_t*)a.workspace, d.weight = a.weight, d.rows = a.rows, d.experts = a.experts, d.top = a.top;
     d.score = a.score, d.renorm = a.renorm, d.scale = a.scale;
     route_blocks(a, d.rows_block, d.blocks);
-    while ((1 << d.bits) <= a.experts) d.bits++;  // one number more than experts
+    while ((1 << d.bits) <= a.experts) d.bits++;
+    for (d.width = 1; d.width < a.experts;) d.width *= 2;
     const int e = a.type == KK_F32 ? 4 : 2;
     d.vec = (uintptr_t)a.logits % 16 == 0 && a.logits_row * e % 16 == 0 && a.experts * e % 16 == 0;
     const size_t bins = (size_t)a.experts + 1, lds = bins * 4 + (kRouteWaves + 1) * bins * 2;
