@@ -444,11 +444,12 @@ __device__ __forceinline__ Groups sum_groups(const ProductDev& p, int* lds) {
             }
             if (in) sums[g] = before + sum - own, starts[g] = s0;
             if (g == p.groups - 1) starts[g + 1] = s1, sums[g + 1] = before + sum;
-            before = __builtin_amdgcn_readlane(before + sum, 63);
+            // groups that overlap could have more tiles than the launch was sized by: what is behind those is never asked for
+            before = min(__builtin_amdgcn_readlane(before + sum, 63), p.tiles);
         }
     }
     __syncthreads();
-    return {sums, starts, __builtin_amdgcn_readfirstlane(sums[p.groups])};
+    return {sums, starts, min(__builtin_amdgcn_readfirstlane(sums[p.groups]), p.tiles)};
 }
 template <int M>
 __device__ __forceinline__ Rows rows_of(const ProductDev& p, const Groups& all, int tile) {
@@ -468,6 +469,33 @@ __device__ __forceinline__ Rows rows_of(const ProductDev& p, const Groups& all, 
     const int s0 = __builtin_amdgcn_readfirstlane(all.starts[g]), s1 = __builtin_amdgcn_readfirstlane(all.starts[g + 1]);
     group_rows(s0, s1, g, tile - __builtin_amdgcn_readfirstlane(all.sums[g]), M, r);
     return r;
+}
+
+// The adapters' share of a tile whose rows have several, 32 rows and 32 outputs at a time: each adapter's into sums of its own, of which its
+// rows take theirs.  As more inputs, with h of the other rows zero, an infinity or NaN in one's b would reach them.
+template <int T, class C>
+__device__ __forceinline__ void add_mixed(const ProductDev& p, const Place<C>& at, const Rows& r, int n0, const int* adapters, Acc<T, C>& acc) {
+#pragma unroll
+    for (int j = 0; j < C::FM; j++) {
+        const int in = at.wm * (C::M / C::WM) + j * 32 + at.col, row = r.first + min(in, r.count - 1);
+        const int ids[1] = {in < r.count ? adapter_in(p, adapters[in]) : -1};
+        const uint16_t* h = p.h2 + (int64_t)row * (2 * p.rank) + at.half * 8;
+        const float unit = T == KK_F16 && ids[0] >= 0 ? p.h_unit[row] : 1.0f;
+        for (int id = next_adapter(ids, -1); id != INT32_MAX; id = next_adapter(ids, id)) {
+            const bool own = ids[0] == id;
+#pragma unroll
+            for (int i = 0; i < C::FN; i++) {
+                const uint16_t* b = p.b + ((int64_t)id * p.outputs + min(n0 + i * 32 + at.col, p.outputs - 1)) * p.rank;
+                f32x16 sum;
+#pragma unroll
+                for (int k = 0; k < 16; k++) sum[k] = 0.0f;
+                for (int k0 = 0; k0 < 2 * p.rank; k0 += 16)  // a lane's half of it: first parts, or what these leave
+                    sum = Mat<T>::mul(*(const uint4*)(b + k0 / 2), own ? *(const uint4*)(h + k0) : uint4{0, 0, 0, 0}, sum);
+#pragma unroll
+                for (int k = 0; k < 16; k++) acc.sum[i][j][k] += own ? sum[k] * unit : 0.0f;
+            }
+        }
+    }
 }
 
 // One product tile: rows of x, the outputs from n0 on, inputs from k_lo on.
@@ -569,38 +597,38 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
             ask(w, side ^ 1);
         }
         acc.clear();
+        bool mixed = false;
         if constexpr (EXT) {
-            // each adapter's b beside the rows' h, which is zero in rows of another
+            // A tile whose rows all have one adapter takes it as more inputs: b beside the rows' h.
             constexpr int kIds = (C::M + 63) / 64;
-            int ids[kIds], mine[C::QX];  // of the tile's rows, a lane each; and of the rows that this lane loads
+            int ids[kIds];
+            const int id = adapter_in(p, places[side][0][0]);
+            bool same = true;
 #pragma unroll
-            for (int i = 0; i < kIds; i++) ids[i] = i * 64 + at.lane < now.r.count ? adapter_in(p, places[side][0][i * 64 + at.lane]) : -1;
-#pragma unroll
-            for (int q = 0; q < C::QX; q++) mine[q] = at.row(q) < now.r.count ? adapter_in(p, places[side][0][at.row(q)]) : -1;
-            bool any = false;
-            for (int id = next_adapter(ids, -1); id != INT32_MAX; id = next_adapter(ids, id)) {
-                any = true;
+            for (int i = 0; i < kIds; i++) {
+                const int row = i * 64 + at.lane;
+                ids[i] = row < now.r.count ? adapter_in(p, places[side][0][row]) : id;
+                same = same && ids[i] == id;
+                mixed = mixed || ids[i] >= 0;
+            }
+            const bool one = __ballot(!same) == 0;
+            mixed = !one && __ballot(mixed) != 0;
+            if (one && id >= 0) {
                 for (int k0 = 0; k0 < 2 * p.rank; k0 += K)
                     run_alone<T, C>(at, acc, [&](int q, uint16_t* to) {
                         const int k = k0 + at.piece;  // of a row of h2, whose b lies at half of it
-                        if (q < C::QW) {
-                            const int o = min(now.n0 + at.row(q), p.outputs - 1);
-                            piece_or_zero(at, k < 2 * p.rank, p.b + ((int64_t)id * p.outputs + o) * p.rank + k / 16 * 8, to);
-                        } else {
-                            const int row = now.r.first + min(at.row(q - C::QW), now.r.count - 1);
-                            piece_or_zero(at, k < 2 * p.rank && mine[q - C::QW] == id, p.h2 + (int64_t)row * (2 * p.rank) + k, to);
-                        }
+                        const int o = min(now.n0 + at.row(q), p.outputs - 1), row = now.r.first + min(at.row(q - C::QW), now.r.count - 1);
+                        piece_or_zero(at, k < 2 * p.rank, q < C::QW ? p.b + ((int64_t)id * p.outputs + o) * p.rank + k / 16 * 8 : p.h2 + (int64_t)row * (2 * p.rank) + k, to);
                     });
-            }
-            if (T == KK_F16 && any) {
+                if constexpr (T == KK_F16) {
 #pragma unroll
-                for (int j = 0; j < C::FM; j++) {
-                    const int row = min(at.wm * (C::M / C::WM) + j * 32 + at.col, now.r.count - 1);
-                    const float unit = adapter_in(p, places[side][0][row]) < 0 ? 1.0f : p.h_unit[now.r.first + row];
+                    for (int j = 0; j < C::FM; j++) {
+                        const float unit = p.h_unit[now.r.first + min(at.wm * (C::M / C::WM) + j * 32 + at.col, now.r.count - 1)];
 #pragma unroll
-                    for (int n = 0; n < C::FN; n++)
+                        for (int n = 0; n < C::FN; n++)
 #pragma unroll
-                        for (int k = 0; k < 16; k++) acc.sum[n][j][k] *= unit;
+                            for (int k = 0; k < 16; k++) acc.sum[n][j][k] *= unit;
+                    }
                 }
             }
             barrier();
@@ -628,6 +656,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
         run_stages<T, C>(at, src, now.steps, at.wm * (C::M / C::WM) < now.r.count, acc);
 
         // the next tile's first stages are on their way while this one's results are stored
+        if (EXT && mixed) add_mixed<T, C>(p, at, now.r, n0, places[side][0], acc);
         int done[C::FM];
 #pragma unroll
         for (int j = 0; j < C::FM; j++) done[j] = to[j];
