@@ -124,13 +124,15 @@ __device__ __forceinline__ void barrier() {
 // the order is made by which piece each lane loads.
 template <class C>
 struct Place {
-    int lane, wave, wn, wm, col, half, row_in, piece, turn;
+    int lane, wave, wn, wm, col, half, row_in, piece;
+    int a_row, b_row, turn;  // where this lane's operands lie in a stage
     uint16_t *lds, *in;  // `in`: where this wave's first load of a stage goes
     uint32_t in_at;
     __device__ __forceinline__ explicit Place(uint16_t* l) : lds(l) {
         lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         wn = wave % C::WN, wm = wave / C::WN;
-        col = lane & 31, half = lane >> 5, turn = C::K == 64 ? (col >> 1) & 7 : (col >> 2) & 3;
+        col = lane & 31, half = lane >> 5, turn = half ^ (C::K == 64 ? (col >> 1) & 7 : (col >> 2) & 3);
+        a_row = (wn * (C::N / C::WN) + col) * C::K, b_row = (C::N + wm * (C::M / C::WM) + col) * C::K;
         const int in_load = lane / C::kPieces;
         row_in = wave * C::kRowsIn + in_load;
         piece = ((lane % C::kPieces) ^ (C::K == 64 ? (in_load >> 1) + 4 * (wave & 1) : in_load >> 2)) * 8;
@@ -173,11 +175,11 @@ struct Acc {
     }
     // operand i of the 16 inputs kk of a stage: the matrix's tiles, then the rows'
     __device__ __forceinline__ void read(const Place<C>& at, int set, const uint16_t* stage, int kk, int i) {
-        const int k = ((kk * 2 + at.half) ^ at.turn) * 8;
+        const uint16_t* from = stage + ((kk * 2) ^ at.turn) * 8;
         if (i < C::FN)
-            a[set][i] = *(const uint4*)(stage + (at.wn * (C::N / C::WN) + i * 32 + at.col) * C::K + k);
+            a[set][i] = *(const uint4*)(from + at.a_row + i * 32 * C::K);
         else
-            b[set][i - C::FN] = *(const uint4*)(stage + (C::N + at.wm * (C::M / C::WM) + (i - C::FN) * 32 + at.col) * C::K + k);
+            b[set][i - C::FN] = *(const uint4*)(from + at.b_row + (i - C::FN) * 32 * C::K);
     }
     __device__ __forceinline__ void mul(int set, int m) {
         sum[m % C::FN][m / C::FN] = Mat<T>::mul(a[set][m % C::FN], b[set][m / C::FN], sum[m % C::FN][m / C::FN]);
@@ -187,7 +189,7 @@ struct Acc {
 // The whole stages, whose first S - 1 `begin` has asked for.  The operands of the next 16 inputs are read, and the loads of a later
 // stage made, between the products of these; sched_barrier keeps that order.  A wave without rows only loads.
 template <int T, class C>
-__device__ __forceinline__ void run_stages(const Place<C>& at, const uint16_t* (&src)[C::Q], int steps, bool live, Acc<T, C>& acc) {
+__device__ __forceinline__ void run_stages(const Place<C>& place, const uint16_t* (&src)[C::Q], int steps, bool live, Acc<T, C>& acc) {
     constexpr int S = C::S, Q = C::Q, kMul = C::FN * C::FM, kRead = C::FN + C::FM, kSub = C::K / 16;
     if (!steps) return;
     // all but the last S - 2 stages' loads of this wave have arrived, and then of all; near the end there are fewer: all
@@ -201,6 +203,8 @@ __device__ __forceinline__ void run_stages(const Place<C>& at, const uint16_t* (
     wait(steps < S - 1);
     // whatever the addresses still depend on (a place's load, a register kept in scratch) is waited for here: a wait of the compiler's
     // own inside the loop would be for all loads
+    Place<C> at = place;
+    asm volatile("" : "+v"(at.a_row), "+v"(at.b_row), "+v"(at.turn));
 #pragma unroll
     for (int q = 0; q < Q; q++) asm volatile("" : "+v"(src[q]));
     if (live) {
@@ -471,10 +475,9 @@ __device__ __forceinline__ Rows rows_of(const ProductDev& p, const Groups& all, 
     return r;
 }
 
-// The adapters' share of a tile whose rows have several, 32 rows and 32 outputs at a time: each adapter's into sums of its own, of which its
-// rows take theirs.  As more inputs, with h of the other rows zero, an infinity or NaN in one's b would reach them.
+// The adapters' share of a wave's rows, 32 rows and 32 outputs at a time: each adapter's into sums of its own, of which its rows take theirs.
 template <int T, class C>
-__device__ __forceinline__ void add_mixed(const ProductDev& p, const Place<C>& at, const Rows& r, int n0, const int* adapters, Acc<T, C>& acc) {
+__device__ __forceinline__ void add_apart(const ProductDev& p, const Place<C>& at, const Rows& r, int n0, const int* adapters, Acc<T, C>& acc) {
 #pragma unroll
     for (int j = 0; j < C::FM; j++) {
         const int in = at.wm * (C::M / C::WM) + j * 32 + at.col, row = r.first + min(in, r.count - 1);
@@ -597,39 +600,53 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
             ask(w, side ^ 1);
         }
         acc.clear();
-        bool mixed = false;
+        bool apart = false;
         if constexpr (EXT) {
-            // A tile whose rows all have one adapter takes it as more inputs: b beside the rows' h.
+            // the adapters as more inputs: each one's b beside the rows' h, which is zero in rows of another
             constexpr int kIds = (C::M + 63) / 64;
-            int ids[kIds];
-            const int id = adapter_in(p, places[side][0][0]);
-            bool same = true;
+            int ids[kIds], own[C::QX], seen = 0;  // of the tile's rows, a lane each; and of the rows that this lane loads
 #pragma unroll
             for (int i = 0; i < kIds; i++) {
                 const int row = i * 64 + at.lane;
-                ids[i] = row < now.r.count ? adapter_in(p, places[side][0][row]) : id;
-                same = same && ids[i] == id;
-                mixed = mixed || ids[i] >= 0;
+                ids[i] = adapter_in(p, places[side][0][min(row, now.r.count - 1)]);
+                seen += __ballot(ids[i] < 0) != 0;  // rows without one are another kind
             }
-            const bool one = __ballot(!same) == 0;
-            mixed = !one && __ballot(mixed) != 0;
-            if (one && id >= 0) {
+            seen = seen != 0;
+#pragma unroll
+            for (int q = 0; q < C::QX; q++) own[q] = adapter_in(p, places[side][0][min(at.row(q), now.r.count - 1)]);
+            bool any = false;
+            for (int id = next_adapter(ids, -1); id != INT32_MAX; id = next_adapter(ids, id)) {
+                any = true, seen++;
                 for (int k0 = 0; k0 < 2 * p.rank; k0 += K)
                     run_alone<T, C>(at, acc, [&](int q, uint16_t* to) {
                         const int k = k0 + at.piece;  // of a row of h2, whose b lies at half of it
-                        const int o = min(now.n0 + at.row(q), p.outputs - 1), row = now.r.first + min(at.row(q - C::QW), now.r.count - 1);
-                        piece_or_zero(at, k < 2 * p.rank, q < C::QW ? p.b + ((int64_t)id * p.outputs + o) * p.rank + k / 16 * 8 : p.h2 + (int64_t)row * (2 * p.rank) + k, to);
+                        if (q < C::QW) {
+                            const int o = min(now.n0 + at.row(q), p.outputs - 1);
+                            piece_or_zero(at, k < 2 * p.rank, p.b + ((int64_t)id * p.outputs + o) * p.rank + k / 16 * 8, to);
+                        } else {
+                            const int row = now.r.first + min(at.row(q - C::QW), now.r.count - 1);
+                            piece_or_zero(at, k < 2 * p.rank && own[q - C::QW] == id, p.h2 + (int64_t)row * (2 * p.rank) + k, to);
+                        }
                     });
-                if constexpr (T == KK_F16) {
+            }
+            if (any) {
+                float size = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < C::FM; j++) {
-                        const float unit = p.h_unit[now.r.first + min(at.wm * (C::M / C::WM) + j * 32 + at.col, now.r.count - 1)];
+                for (int j = 0; j < C::FM; j++) {
+                    const int row = min(at.wm * (C::M / C::WM) + j * 32 + at.col, now.r.count - 1);
+                    const float unit = T == KK_F16 && adapter_in(p, places[side][0][row]) >= 0 ? p.h_unit[now.r.first + row] : 1.0f;
 #pragma unroll
-                        for (int n = 0; n < C::FN; n++)
+                    for (int n = 0; n < C::FN; n++)
 #pragma unroll
-                            for (int k = 0; k < 16; k++) acc.sum[n][j][k] *= unit;
-                    }
+                        for (int k = 0; k < 16; k++) {
+                            size += acc.sum[n][j][k] * 0.0f;
+                            if constexpr (T == KK_F16) acc.sum[n][j][k] *= unit;
+                        }
                 }
+                // Zero times an infinity or NaN of one adapter's b is not zero in the rows of another: where something is not finite in a tile
+                // of several kinds, the wave adds the shares apart.
+                apart = seen > 1 && __ballot(size != 0.0f) != 0;
+                if (apart) acc.clear();
             }
             barrier();
             begin<C>(at, src, now.steps);
@@ -656,7 +673,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
         run_stages<T, C>(at, src, now.steps, at.wm * (C::M / C::WM) < now.r.count, acc);
 
         // the next tile's first stages are on their way while this one's results are stored
-        if (EXT && mixed) add_mixed<T, C>(p, at, now.r, n0, places[side][0], acc);
+        if (EXT && apart) add_apart<T, C>(p, at, now.r, n0, places[side][0], acc);
         int done[C::FM];
 #pragma unroll
         for (int j = 0; j < C::FM; j++) done[j] = to[j];
@@ -848,7 +865,7 @@ AdapterPlan adapter_plan(const kk_adapter_product_args& a, int n_cu) {
     ProductPlan& p = r.main;
     p.splits = 1, p.k_split = a.inputs;
     auto tiles = [&](int64_t rows, int tile) { return ceil_div(rows, kTiles[tile].M) * ceil_div(a.outputs, kTiles[tile].N); };
-    p.tile = tiles(a.rows, k256) >= n_cu ? k256 : k128Wide;
+    p.tile = k128Wide;
     r.joined = tiles(a.rows, p.tile) < n_cu;
     int64_t rows = a.rows;
     if (r.joined) {
@@ -858,17 +875,17 @@ AdapterPlan adapter_plan(const kk_adapter_product_args& a, int n_cu) {
         p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(room / one, a.inputs / 512));
         p.k_split = (int)ceil_div(ceil_div(a.inputs, p.splits), 64) * 64;
         p.splits = (int)ceil_div(a.inputs, p.k_split);
-    } else if (p.tile == k256) {
+    } else {
         // Whole rounds of large tiles; the rows of a last round that would leave most of the device idle go to smaller ones.
-        const int64_t wide = ceil_div(a.outputs, 256), all = ceil_div(a.rows, 256) * wide, whole = all / n_cu * n_cu / wide * 256;
-        if ((all - whole / 256 * wide) * 2 < n_cu) rows = std::min<int64_t>(rows, whole);
+        const int64_t wide = ceil_div(a.outputs, kTiles[k128Wide].N), all = tiles(a.rows, k128Wide), whole = all / n_cu * n_cu / wide;
+        if (whole && (all - whole * wide) * 2 < n_cu) rows = std::min<int64_t>(rows, whole * kTiles[k128Wide].M);
     }
     size_grid(p, ceil_div(rows, kTiles[p.tile].M), a.outputs, n_cu);
     r.rows = (int)rows;
     if (rows < a.rows) {
         r.rest = p;
         const int64_t left = a.rows - rows;
-        r.rest.tile = tiles(left, k128Wide) * 2 > n_cu ? k128Wide : k64;
+        r.rest.tile = k64;
         size_grid(r.rest, ceil_div(left, kTiles[r.rest.tile].M), a.outputs, n_cu);
     }
     if (a.adapters) {
@@ -910,9 +927,7 @@ hipError_t launch_expert_product(const kk_expert_product_args& a, const ProductP
 template <int T, bool EXT, int OUT>
 static hipError_t adapter_main(ProductDev d, const ProductPlan& p, hipStream_t s) {
     set_grid(d, p);
-    if (p.tile == k64) return run_tile<T, Tile64, false, EXT, OUT>(d, p, s);
-    if (p.tile == k128Wide) return run_tile<T, Tile128Wide, false, EXT, OUT>(d, p, s);
-    return run_tile<T, Tile256, false, EXT, OUT>(d, p, s);
+    return p.tile == k64 ? run_tile<T, Tile64, false, EXT, OUT>(d, p, s) : run_tile<T, Tile128Wide, false, EXT, OUT>(d, p, s);
 }
 
 template <int T, int OUT>
