@@ -865,8 +865,8 @@ AdapterPlan adapter_plan(const kk_adapter_product_args& a, int n_cu) {
     ProductPlan& p = r.main;
     p.splits = 1, p.k_split = a.inputs;
     auto tiles = [&](int64_t rows, int tile) { return ceil_div(rows, kTiles[tile].M) * ceil_div(a.outputs, kTiles[tile].N); };
-    p.tile = k128Wide;
-    r.joined = tiles(a.rows, p.tile) < n_cu;
+    p.tile = tiles(a.rows, k128Wide) * 4 >= 3 * n_cu ? k128Wide : k64;
+    r.joined = tiles(a.rows, k64) < n_cu;
     int64_t rows = a.rows;
     if (r.joined) {
         p.tile = a.rows <= 64 ? k64 : k128;
@@ -875,7 +875,7 @@ AdapterPlan adapter_plan(const kk_adapter_product_args& a, int n_cu) {
         p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(room / one, a.inputs / 512));
         p.k_split = (int)ceil_div(ceil_div(a.inputs, p.splits), 64) * 64;
         p.splits = (int)ceil_div(a.inputs, p.k_split);
-    } else {
+    } else if (p.tile == k128Wide) {
         // Whole rounds of large tiles; the rows of a last round that would leave most of the device idle go to smaller ones.
         const int64_t wide = ceil_div(a.outputs, kTiles[k128Wide].N), all = tiles(a.rows, k128Wide), whole = all / n_cu * n_cu / wide;
         if (whole && (all - whole * wide) * 2 < n_cu) rows = std::min<int64_t>(rows, whole * kTiles[k128Wide].M);
