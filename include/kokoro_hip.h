@@ -475,8 +475,8 @@ typedef struct {
     void* workspace;        /* 16-byte aligned, kk_expert_route_workspace bytes or more; need not be cleared */
     size_t workspace_bytes;
 } kk_expert_route_args;
-/* The workspace that kk_expert_route needs (0: none), or negative KK_ERR_* for arguments that it would refuse.  It depends on rows,
- * experts and top alone. */
+/* The workspace that kk_expert_route needs (0: none), or negative KK_ERR_* for arguments that it would refuse.  It depends on rows and
+ * experts alone. */
 int64_t kk_expert_route_workspace(kk_ctx* ctx, const kk_expert_route_args* args, char* err, size_t errlen);
 int kk_expert_route(kk_ctx* ctx, const kk_expert_route_args* args, void* stream, char* err, size_t errlen);
 
@@ -488,7 +488,9 @@ int kk_expert_route(kk_ctx* ctx, const kk_expert_route_args* args, void* stream,
  * The layer's first product takes kk_expert_route's `place` as x_place with x_div = top (rows of the layer's input to
  * entries), its second as y_place (entries to rows of y by row and choice, as kk_expert_join reads them).  Rows of y that no
  * entry goes to are left as they were; two entries with one place write the same row, in no order.  y overlaps no input.
- * The result of an entry depends on `entries` and `groups` (by which a kernel is chosen: the order of f32 sums), not on the others. */
+ * The result of an entry depends on `entries` and `groups` (by which a tile is chosen: the order of f32 sums), not on the others.
+ * One choice is made for the whole call, by entries / groups: where some groups have hundreds of rows and most have few, two calls can
+ * take less time. */
 #define KK_GATE_NONE 0
 #define KK_GATE_SILU 1
 #define KK_GATE_GELU 2
@@ -534,7 +536,7 @@ int kk_expert_join(kk_ctx* ctx, const kk_expert_join_args* args, void* stream, c
 
 /* y[r] = w x[r] + bias + scale[i] b_i (a_i x[r]) with i = adapter[r]; a row whose adapter is negative has no third term.  The rows
  * may be in any order; those of one request next to each other are the fast case.  a_i x is kept with 16 bits or more before
- * b_i.  With adapters = 0 it is the projection alone. */
+ * b_i.  A matrix that is not finite reaches the rows of its own adapter alone.  With adapters = 0 it is the projection alone. */
 typedef struct {
     int32_t type;           /* KK_BF16 or KK_F16: x, w, a, b */
     int32_t out_type;       /* `type` or KK_F32: y */
@@ -558,7 +560,8 @@ typedef struct {
     void* workspace;        /* 16-byte aligned, kk_adapter_product_workspace bytes or more; need not be cleared */
     size_t workspace_bytes;
 } kk_adapter_product_args;
-/* As kk_expert_route_workspace.  It depends on rows, inputs, outputs, adapters, rank and the device's compute units alone. */
+/* As kk_expert_route_workspace.  It depends on rows, inputs, outputs, adapters, rank and the device's compute units alone, and does
+ * not always grow with them (fewer rows may be split into more parts). */
 int64_t kk_adapter_product_workspace(kk_ctx* ctx, const kk_adapter_product_args* args, char* err, size_t errlen);
 int kk_adapter_product(kk_ctx* ctx, const kk_adapter_product_args* args, void* stream, char* err, size_t errlen);
 

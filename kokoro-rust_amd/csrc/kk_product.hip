@@ -87,8 +87,8 @@ __device__ __forceinline__ void store4(void* base, int64_t at, int vec, int left
 
 // ------------------------------------------------------------------ a tile
 
-// N rows of the matrix (outputs) and M rows of x, held by WN x WM waves in 32 x 32 tiles of the matrix cores, through LDS in stages of
-// 64 inputs, S of them in flight.
+// N rows of the matrix (outputs) and M rows of x, held by WN x WM waves in 32 x 32 tiles of the matrix cores, through LDS in S stages of
+// K inputs each.
 template <int N_, int M_, int WN_, int WM_, int K_, int S_, int PER_CU_>
 struct Tile {
     static constexpr int N = N_, M = M_, WN = WN_, WM = WM_, K = K_, S = S_, kPerCu = PER_CU_;
@@ -120,8 +120,9 @@ __device__ __forceinline__ void barrier() {
 }
 
 // What a wave and a lane are in a tile.  A stage's rows are 64 inputs, eight pieces of 16 bytes, in an order that their row number turns
-// (by XOR with its bits 1 to 3; rows of 32 inputs, four pieces: bits 2 and 3), so that the 16 rows that LDS reads at once lie on all 64 banks; since the loads store lane after lane,
-// the order is made by which piece each lane loads.
+// (by XOR with its bits 1 to 3; rows of 32 inputs, four pieces: bits 2 and 3), so that the 16 rows that LDS reads at once lie on all 64
+// banks (with bits 0 to 2 half of its time were conflicts); since the loads store lane after lane, the order is made by which piece each
+// lane loads.
 template <class C>
 struct Place {
     int lane, wave, wn, wm, col, half, row_in, piece;
@@ -147,7 +148,7 @@ __device__ __forceinline__ void load(const Place<C>& at, const uint16_t* const (
     to_lds(src[q], at.in_at + side * (2 * C::kStage) + q * (2 * C::kNext));
 }
 
-// The first stages' loads: `steps` stages of 64 inputs follow.
+// The first of `steps` stages' loads, as many as are in flight at a time.
 template <class C>
 __device__ __forceinline__ void begin(const Place<C>& at, const uint16_t* (&src)[C::Q], int steps) {
 #pragma unroll
@@ -368,57 +369,57 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) shrink
     __shared__ __align__(16) uint16_t lds[C::S * C::kStage];
     const Place<C> at(lds);
     Acc<T, C> acc;
-                constexpr int kIds = (C::M + 63) / 64;
-                const int n_ranks = (p.rank + C::N - 1) / C::N;
-                int rest = blockIdx.x;
-                const int split = rest % p.h_splits;
-                rest /= p.h_splits;
-                const int n0 = rest % n_ranks * C::N;
-                rest /= n_ranks;
-                const int tiles = (p.entries + C::M - 1) / C::M, slot = rest / tiles, first = rest % tiles * C::M;
+    constexpr int kIds = (C::M + 63) / 64;
+    const int n_ranks = (p.rank + C::N - 1) / C::N;
+    int rest = blockIdx.x;
+    const int split = rest % p.h_splits;
+    rest /= p.h_splits;
+    const int n0 = rest % n_ranks * C::N;
+    rest /= n_ranks;
+    const int tiles = (p.entries + C::M - 1) / C::M, slot = rest / tiles, first = rest % tiles * C::M;
     const int count = min(C::M, p.entries - first);
-                int ids[kIds];
-    #pragma unroll
-                for (int i = 0; i < kIds; i++) ids[i] = i * 64 + at.lane < count ? adapter_of(p, first + i * 64 + at.lane) : -1;
-                const int k_lo = split * p.h_k, k_hi = min(p.inputs, k_lo + p.h_k), steps = (k_hi - k_lo) / K, left = (k_hi - k_lo) % K;
-                int id = -1;
-                for (int n = 0;; n++) {
-                    id = next_adapter(ids, id);
-                    if (id == INT32_MAX) return;
-                    if (n % p.slots != slot) continue;
-                    const uint16_t* src[C::Q];
-    #pragma unroll
-                    for (int q = 0; q < C::QW; q++)
-                        src[q] = p.a + ((int64_t)id * p.rank + min(n0 + at.row(q), p.rank - 1)) * p.inputs + k_lo + at.piece;
-    #pragma unroll
-                    for (int q = 0; q < C::QX; q++)
-                        src[C::QW + q] = p.x + (int64_t)(first + min(at.row(q), count - 1)) * p.x_row + k_lo + at.piece;
-                    acc.clear();
-                    barrier();  // an adapter before has been read
-                    begin<C>(at, src, steps);
-                    if (left)
-                        run_alone<T, C>(at, acc, [&](int q, uint16_t* to) {
-                            piece_or_zero(at, at.piece < left, src[q] + (steps - min(C::S - 1, steps)) * K, to);
-                        });
-                    run_stages<T, C>(at, src, steps, at.wm * (C::M / C::WM) < count && n0 + at.wn * (C::N / C::WN) < p.rank, acc);
-                    const float s = p.scale[id];
-    #pragma unroll
-                    for (int j = 0; j < C::FM; j++) {
-                        const int row = at.wm * (C::M / C::WM) + j * 32 + at.col;
-                        if (row >= count || adapter_of(p, first + row) != id) continue;
-                        float* to = p.h + ((int64_t)split * p.entries + first + row) * p.rank;
-    #pragma unroll
-                        for (int i = 0; i < C::FN; i++)
-    #pragma unroll
-                            for (int q = 0; q < 4; q++) {
-                                const int o = n0 + at.wn * (C::N / C::WN) + i * 32 + q * 8 + at.half * 4;
-                                if (o >= p.rank) continue;  // a multiple of 8
-                                const f32x4 v = {acc.sum[i][j][4 * q] * s, acc.sum[i][j][4 * q + 1] * s, acc.sum[i][j][4 * q + 2] * s,
-                                                 acc.sum[i][j][4 * q + 3] * s};
-                                *(f32x4*)(to + o) = v;
-                            }
-                    }
+    int ids[kIds];
+#pragma unroll
+    for (int i = 0; i < kIds; i++) ids[i] = i * 64 + at.lane < count ? adapter_of(p, first + i * 64 + at.lane) : -1;
+    const int k_lo = split * p.h_k, k_hi = min(p.inputs, k_lo + p.h_k), steps = (k_hi - k_lo) / K, left = (k_hi - k_lo) % K;
+    int id = -1;
+    for (int n = 0;; n++) {
+        id = next_adapter(ids, id);
+        if (id == INT32_MAX) return;
+        if (n % p.slots != slot) continue;
+        const uint16_t* src[C::Q];
+#pragma unroll
+        for (int q = 0; q < C::QW; q++)
+            src[q] = p.a + ((int64_t)id * p.rank + min(n0 + at.row(q), p.rank - 1)) * p.inputs + k_lo + at.piece;
+#pragma unroll
+        for (int q = 0; q < C::QX; q++)
+            src[C::QW + q] = p.x + (int64_t)(first + min(at.row(q), count - 1)) * p.x_row + k_lo + at.piece;
+        acc.clear();
+        barrier();  // an adapter before has been read
+        begin<C>(at, src, steps);
+        if (left)
+            run_alone<T, C>(at, acc, [&](int q, uint16_t* to) {
+                piece_or_zero(at, at.piece < left, src[q] + (steps - min(C::S - 1, steps)) * K, to);
+            });
+        run_stages<T, C>(at, src, steps, at.wm * (C::M / C::WM) < count && n0 + at.wn * (C::N / C::WN) < p.rank, acc);
+        const float s = p.scale[id];
+#pragma unroll
+        for (int j = 0; j < C::FM; j++) {
+            const int row = at.wm * (C::M / C::WM) + j * 32 + at.col;
+            if (row >= count || adapter_of(p, first + row) != id) continue;
+            float* to = p.h + ((int64_t)split * p.entries + first + row) * p.rank;
+#pragma unroll
+            for (int i = 0; i < C::FN; i++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const int o = n0 + at.wn * (C::N / C::WN) + i * 32 + q * 8 + at.half * 4;
+                    if (o >= p.rank) continue;  // a multiple of 8
+                    const f32x4 v = {acc.sum[i][j][4 * q] * s, acc.sum[i][j][4 * q + 1] * s, acc.sum[i][j][4 * q + 2] * s,
+                                     acc.sum[i][j][4 * q + 3] * s};
+                    *(f32x4*)(to + o) = v;
                 }
+        }
+    }
 }
 
 // ------------------------------------------------------------------ the products
@@ -507,6 +508,15 @@ struct Work {
     int n0, split, k_lo, steps, rest;
 };
 
+// Bound by the matrix cores where a group has many rows, and then by the power they draw: 63,352 entries over 64 groups, 2,048 inputs to
+// 2 x 1,024 outputs (531 GFLOP) 548-650 us by the device's clock, 820-970 TFLOP/s; one group of 8,192 x 8,192 x 8,192 1,200, of zeros 1,430
+// (a library product 1,525 and 2,125).  11% of the tiles' rows are empty, 9 rounds of tiles are 8.7 full ones, and each tile costs 12 us beside
+// its stages: the stores of all CUs come together and wait for memory (50 us of such a call).  Without its loads a stage of 64 inputs takes
+// 1.5 us of 1.85, without its products 1.4.  Where groups have few rows, bound by the matrices' bytes: 512 entries over 64 groups of
+// 2,048 x 1,024 (268 MB) 50 us, 5.4 TB/s; eight entries with a group each (67 MB) 14 us.
+// Tried: four waves with 128 x 128 each (stages 7% shorter, tiles' ends 30% longer), five stages of 32 inputs and two of 64, loads spread
+// over a whole stage or reads all in its first half (no change), blocks started apart in time so that their stores do not meet (no change),
+// stores that pass the caches (a third slower), matrices straight to registers for few rows (15-20% slower: 64 bytes of each row a load).
 // EXT: adapters in many rows, as more inputs (h2).  OUT = 0: sums to `part`, and the adapters' h in blocks behind p.blocks.
 template <int T, class C, bool GATED, bool EXT, int OUT>
 __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) product_kernel(ProductDev p) {
@@ -526,17 +536,16 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
         }
     }
 
-    // A block takes tile after tile.  Blocks go to the 8 XCDs in turn; an XCD takes tiles that follow each other, in strips eight tiles of
-    // outputs wide, which share rows of x and matrices in its L2.
+    // a block takes tile after tile
     const Groups groups = sum_groups<C::M>(p, more_lds);
-    const int block = blockIdx.x, blocks = p.blocks;
-    const int tall = groups.tiles * p.splits, total = tall * p.tiles_n;
-    const int per = (total + 7) / 8, end = min(total, (block % 8 + 1) * per);
-    int t = block % 8 * per + block / 8;
+    const int tall = groups.tiles * p.splits;
+    const TileWalk walk = tile_walk(blockIdx.x, p.blocks, tall * p.tiles_n);
+    int t = walk.first;
     auto work_of = [&](int t) {
         Work w;
-        const int strip = t / (8 * tall), wide = min(8, p.tiles_n - 8 * strip), in = t - strip * (8 * tall), rest = in / wide;
-        w.n0 = (8 * strip + (in - rest * wide)) * kOutN;
+        const TileAt on = tile_at(t, tall, p.tiles_n);
+        w.n0 = on.n * kOutN;
+        const int rest = on.row;
         const int tile = rest / p.splits;
         w.split = rest - tile * p.splits;
         w.r = rows_of<C::M>(p, groups, tile);
@@ -583,7 +592,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
             if (row >= w.r.count || (OUT != 0 && !EXT && x_of(p, e, places[side][0][in]) < 0)) to[j] = -1;
         }
     };
-    if (t >= end) return;
+    if (t >= walk.end) return;
     Work w = work_of(t);
     ask(w, 0);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -593,8 +602,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
     for (int side = 0;; side ^= 1) {
         // while the first stages are on their way: what the next tile is
         const Work now = w;
-        t += blocks / 8;
-        const bool again = t < end;
+        t += walk.step;
+        const bool again = t < walk.end;
         if (again) {
             w = work_of(t);
             ask(w, side ^ 1);
@@ -832,78 +841,11 @@ hipError_t run_tile(const ProductDev& d, const ProductPlan& p, hipStream_t s) {
     return launch(product_kernel<T, C, GATED, EXT, OUT>, dim3((unsigned)(d.blocks + (OUT == 0 ? p.shrink : 0))), dim3(C::kThreads), lds, s, d);
 }
 
-struct TileSize {
-    int N, M, per_cu;
-};
-constexpr TileSize kTiles[] = {{128, 64, 2}, {64, 128, 2}, {256, 128, 1}, {256, 256, 1}};
-
-// The grid: as many blocks as tiles or as the device holds at once.
-void size_grid(ProductPlan& p, int64_t row_tiles, int64_t wide, int n_cu) {
-    const TileSize& z = kTiles[p.tile];
-    p.tiles = (int)row_tiles, p.tiles_n = (int)ceil_div(wide, z.N);
-    const int64_t all = row_tiles * p.tiles_n * p.splits;
-    p.blocks = (int)((std::min<int64_t>(all, (int64_t)z.per_cu * n_cu) + 7) / 8 * 8);
-}
-
 void set_grid(ProductDev& d, const ProductPlan& p) {
     d.splits = p.splits, d.k_split = p.k_split, d.tiles = p.tiles, d.tiles_n = p.tiles_n, d.blocks = p.blocks;
 }
 
 }  // namespace
-
-ProductPlan expert_plan(const kk_expert_product_args& a, int n_cu) {
-    ProductPlan p{};
-    p.splits = 1, p.k_split = a.inputs;
-    const int64_t mean = a.entries / a.groups;
-    p.tile = mean <= 40 ? k64 : mean < 450 ? k128Wide : k256;
-    size_grid(p, row_tiles(a.entries, a.groups, kTiles[p.tile].M), (int64_t)a.outputs * (a.gate != KK_GATE_NONE ? 2 : 1), n_cu);
-    return p;
-}
-
-AdapterPlan adapter_plan(const kk_adapter_product_args& a, int n_cu) {
-    AdapterPlan r{};
-    ProductPlan& p = r.main;
-    p.splits = 1, p.k_split = a.inputs;
-    auto tiles = [&](int64_t rows, int tile) { return ceil_div(rows, kTiles[tile].M) * ceil_div(a.outputs, kTiles[tile].N); };
-    p.tile = tiles(a.rows, k128Wide) * 4 >= 3 * n_cu ? k128Wide : k64;
-    r.joined = tiles(a.rows, k64) < n_cu;
-    int64_t rows = a.rows;
-    if (r.joined) {
-        p.tile = a.rows <= 64 ? k64 : k128;
-        // a block for each CU where that splits the inputs, else two: 96 tiles in 2 parts take as long as in 5, with less to sum up
-        const int64_t one = tiles(a.rows, p.tile), room = n_cu / one > 1 ? n_cu : 2 * n_cu;
-        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(room / one, a.inputs / 512));
-        p.k_split = (int)ceil_div(ceil_div(a.inputs, p.splits), 64) * 64;
-        p.splits = (int)ceil_div(a.inputs, p.k_split);
-    } else if (p.tile == k128Wide) {
-        // Whole rounds of large tiles; the rows of a last round that would leave most of the device idle go to smaller ones.
-        const int64_t wide = ceil_div(a.outputs, kTiles[k128Wide].N), all = tiles(a.rows, k128Wide), whole = all / n_cu * n_cu / wide;
-        if (whole && (all - whole * wide) * 2 < n_cu) rows = std::min<int64_t>(rows, whole * kTiles[k128Wide].M);
-    }
-    size_grid(p, ceil_div(rows, kTiles[p.tile].M), a.outputs, n_cu);
-    r.rows = (int)rows;
-    if (rows < a.rows) {
-        r.rest = p;
-        const int64_t left = a.rows - rows;
-        r.rest.tile = k64;
-        size_grid(r.rest, ceil_div(left, kTiles[r.rest.tile].M), a.outputs, n_cu);
-    }
-    if (a.adapters) {
-        const int64_t of_rows = ceil_div(a.rows, r.joined ? 16 : kTiles[k128].M), of_ranks = ceil_div(a.rank, r.joined ? 32 : kTiles[k128].N);
-        // blocks that take 1,024 inputs each; in many rows as few as two a CU allow
-        const int64_t most = std::max<int64_t>(1, r.joined ? a.inputs / 1024 : std::min<int64_t>(a.inputs / 512, 2 * n_cu / (of_rows * of_ranks)));
-        r.h_k = (int)ceil_div(ceil_div(a.inputs, most), 64) * 64;
-        r.h_splits = (int)ceil_div(a.inputs, r.h_k);
-        r.slots = (int)std::min<int64_t>(a.adapters, r.joined && a.rows <= 512 ? 16 : 2);
-        p.shrink = of_rows * of_ranks * r.slots * r.h_splits;
-    }
-    auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
-    r.ws_h2 = a.adapters ? up((int64_t)r.h_splits * a.rows * a.rank * 4) : 0;
-    r.ws_unit = r.ws_h2 + (a.adapters && !r.joined ? up((int64_t)a.rows * a.rank * 4) : 0);
-    r.ws_part = r.ws_unit + (a.adapters && !r.joined ? up((int64_t)a.rows * 4) : 0);
-    r.ws_bytes = r.ws_part + (r.joined ? (int64_t)p.splits * a.rows * a.outputs * 4 : 0);
-    return r;
-}
 
 template <int T, bool GATED>
 static hipError_t expert_run(const ProductDev& d, const ProductPlan& p, hipStream_t s) {

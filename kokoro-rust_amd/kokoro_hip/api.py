@@ -30,6 +30,8 @@ EXPORTS = [
     "kk_checkpoint_entry", "kk_checkpoint_free", "kk_upload_checkpoint", "kk_weight_norm", "kk_voice_load",
     "kk_voice_free", "kk_voice_ref_s", "kk_forward_batch", "kk_result_free", "kk_plan_create_full",
     "kk_plan_durations", "kk_qk_norm_rope", "kk_kv_write", "kk_kv_read", "kk_kv_attention", "kk_kv_attention_workspace",
+    "kk_expert_route", "kk_expert_route_workspace", "kk_expert_product", "kk_expert_join", "kk_adapter_product",
+    "kk_adapter_product_workspace",
 ]
 BF16, F16, F32 = 1, 2, 3
 KV_PAGE, KV_INT8, KV_E4M3 = 64, 1, 2
