@@ -1,4 +1,5 @@
-// kk_ops.hip -- the C entries of a language model's operators (attention over an 8-bit cache, products of ragged rows): checks, the context's device, the launch.
+// kk_ops.hip -- the C entries of a language model's operators (attention over an 8-bit cache, products of ragged rows): checks, the
+// context's device, the launch.
 // They enqueue on the caller's stream, allocate nothing and touch nothing of the context but its device.
 #include <cstdio>
 #include <new>

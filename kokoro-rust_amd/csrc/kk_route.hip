@@ -6,7 +6,9 @@
 // Grouping.  A stable counting sort by expert.  Within 64 choices a lane's rank among those of its expert comes from one ballot for each
 // bit of the expert's number; over a block's waves and over blocks from counts.  Nothing depends on the order of atomics.
 //
-// Few rows take one launch of one block, which is all latency; many take one that chooses and counts and one that places.
+// Few rows take one launch of one block, which is all latency (a row of 64 experts, top 8: 7-8 us);
+// many take one that chooses and counts and one that places: 16,384 rows of 128 experts 7.3-8.8 and 7.8-8.6 us, for 5.8 MB.  Both are chains
+// of reductions and barriers, not bytes: eight rounds of a row's largest key, and for each 1,024 choices of a block five barriers.
 #include <algorithm>
 
 #include "kk_product.h"
@@ -294,7 +296,7 @@ struct JoinDev {
 };
 
 // A wave takes 64 V values of a row (V: 16 bytes, or one), so its row, experts and weights are scalars.  Bound by memory: every result is
-// read once, kAhead of them in flight a lane.
+// read once, kAhead of them in flight a lane: 8,192 rows of 2,048 values, top 8 (327 MB) 54-57 us, 5.7-6.1 TB/s; 64 rows 4.2 us.
 template <int T, int V>
 __global__ void __launch_bounds__(256) join_kernel(JoinDev a) {
     typedef typename ElemOf<T>::type E;

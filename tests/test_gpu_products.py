@@ -308,6 +308,27 @@ def test_adapter_product_keeps_requests_apart(ctx, kind, rows, n):
     assert not torch.isfinite(y[ids == 2][:, :2]).any() and not torch.isfinite(y[ids == 3]).any()
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("rows, n", [(40, 100), (6000, 2000)])
+def test_adapter_product_infinite_rows(ctx, kind, rows, n):
+    """An infinity in a row of x stays one where every term has its sign, whether the adapter's share goes through 16-bit parts or not,
+    and is NaN where they differ; the other rows are as without it."""
+    k, rank = 72, 16
+    x, w = _randn((rows, k), 1, kind), _randn((n, k), 2, kind).abs() + 0.5
+    a, b, scale = _randn((2, rank, k), 3, kind).abs() + 0.5, _randn((2, n, rank), 4, kind).abs() + 0.5, torch.ones(2, device="cuda")
+    ids = (torch.arange(rows, device="cuda") % 3 - 1).int()
+    ids[rows // 2:] = 1
+    want, bound = R.adapter_ref(x, w, None, a, b, scale, ids)
+    up, down, both = [torch.tensor(i, device="cuda") for i in ((1, rows - 3), (5, rows - 4), (7, rows - 5))]
+    x[up, 3], x[down, 70], x[both, 5], x[both, 6] = torch.inf, -torch.inf, torch.inf, -torch.inf
+    y = torch.empty(rows, n, dtype=R.TYPES[kind], device="cuda")
+    R.adapter_run(ctx, R.adapter_args(x, w, y, None, a, b, scale, ids))
+    good = torch.ones(rows, dtype=torch.bool, device="cuda")
+    good[torch.cat([up, down, both])] = False
+    R.close(y[good], want[good], bound[good])
+    assert (y[up] == torch.inf).all() and (y[down] == -torch.inf).all() and torch.isnan(y[both]).all()
+
+
 @pytest.mark.parametrize("rows", [3, 300, 6000])
 def test_adapter_product_sizes_out_of_f16(ctx, rows):
     """a x beyond f16's range, with b small: neither overflows on the way."""
