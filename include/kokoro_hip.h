@@ -536,7 +536,7 @@ int kk_expert_join(kk_ctx* ctx, const kk_expert_join_args* args, void* stream, c
 
 /* y[r] = w x[r] + bias + scale[i] b_i (a_i x[r]) with i = adapter[r]; a row whose adapter is negative has no third term.  The rows
  * may be in any order; those of one request next to each other are the fast case.  a_i x is kept with 16 bits or more before
- * b_i.  A matrix that is not finite reaches the rows of its own adapter alone.  With adapters = 0 it is the projection alone. */
+ * b_i, where y is f32 with 22.  A matrix that is not finite reaches the rows of its own adapter alone.  With adapters = 0 it is the projection alone. */
 typedef struct {
     int32_t type;           /* KK_BF16 or KK_F16: x, w, a, b */
     int32_t out_type;       /* `type` or KK_F32: y */

@@ -26,7 +26,7 @@ struct ProductDev {
     int adapters, rank;
     int slots, h_splits, h_k;  // blocks that share a row tile's adapters, and its inputs
     float* h;        // [h_splits][rows][rank], times the adapter's scale
-    uint16_t* h2;    // [rows][2 rank]: each 8 values' first 16 bits and then what these leave, in units of h_unit[row]
+    uint16_t* h2;    // [rows][parts * rank]: each 8 values' first 16 bits, what these leave, and so on, in units of h_unit[row]
     float* h_unit;   // [rows]
     float* part;     // [splits][entries][outputs]
     int splits, k_split;

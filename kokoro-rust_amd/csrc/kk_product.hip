@@ -479,14 +479,20 @@ __device__ __forceinline__ Rows rows_of(const ProductDev& p, const Groups& all, 
     return r;
 }
 
+// Parts of 16 bits that h of many rows is kept in: of f16 (11 bits each) two; of bf16 (8) two, to 2^-17, where y has 16 bits, and three where it
+// has 32: with two, f32 results were off by 1.1e-6 in place of 2.3e-7.
+template <int T, int OUT>
+constexpr int kHParts = T == KK_BF16 && OUT == KK_F32 ? 3 : 2;
+
 // The adapters' share of a wave's rows, 32 rows and 32 outputs at a time: each adapter's into sums of its own, of which its rows take theirs.
-template <int T, class C>
+template <int T, int PARTS, class C>
 __device__ __forceinline__ void add_apart(const ProductDev& p, const Place<C>& at, const Rows& r, int n0, const int* adapters, Acc<T, C>& acc) {
 #pragma unroll
     for (int j = 0; j < C::FM; j++) {
         const int in = at.wm * (C::M / C::WM) + j * 32 + at.col, row = r.first + min(in, r.count - 1);
         const int ids[1] = {in < r.count ? adapter_in(p, adapters[in]) : -1};
-        const uint16_t* h = p.h2 + (int64_t)row * (2 * p.rank) + at.half * 8;
+        const int all = PARTS * p.rank;
+        const uint16_t* h = p.h2 + (int64_t)row * all;
         const float unit = T == KK_F16 && ids[0] >= 0 ? p.h_unit[row] : 1.0f;
         for (int id = next_adapter(ids, -1); id != INT32_MAX; id = next_adapter(ids, id)) {
             const bool own = ids[0] == id;
@@ -496,8 +502,11 @@ __device__ __forceinline__ void add_apart(const ProductDev& p, const Place<C>& a
                 f32x16 sum;
 #pragma unroll
                 for (int k = 0; k < 16; k++) sum[k] = 0.0f;
-                for (int k0 = 0; k0 < 2 * p.rank; k0 += 16)  // a lane's half of it: first parts, or what these leave
-                    sum = Mat<T>::mul(*(const uint4*)(b + k0 / 2), own ? *(const uint4*)(h + k0) : uint4{0, 0, 0, 0}, sum);
+                for (int k = at.half * 8; k < all + at.half * 8; k += 16) {  // a lane takes every other piece, and zeros behind the last
+                    const uint4 zero = {0, 0, 0, 0};
+                    const bool in = k < all;
+                    sum = Mat<T>::mul(in ? *(const uint4*)(b + k / (8 * PARTS) * 8) : zero, in && own ? *(const uint4*)(h + k) : zero, sum);
+                }
 #pragma unroll
                 for (int k = 0; k < 16; k++) acc.sum[i][j][k] += own ? sum[k] * unit : 0.0f;
             }
@@ -615,7 +624,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
         bool apart = false;
         if constexpr (EXT) {
             // the adapters as more inputs: each one's b beside the rows' h, which is zero in rows of another
-            constexpr int kIds = (C::M + 63) / 64;
+            constexpr int kIds = (C::M + 63) / 64, kParts = kHParts<T, OUT>;
             int ids[kIds], own[C::QX], seen = 0;  // of the tile's rows, a lane each; and of the rows that this lane loads
 #pragma unroll
             for (int i = 0; i < kIds; i++) {
@@ -629,15 +638,15 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
             bool any = false;
             for (int id = next_adapter(ids, -1); id != INT32_MAX; id = next_adapter(ids, id)) {
                 any = true, seen++;
-                for (int k0 = 0; k0 < 2 * p.rank; k0 += K)
+                for (int k0 = 0; k0 < kParts * p.rank; k0 += K)
                     run_alone<T, C>(at, acc, [&](int q, uint16_t* to) {
-                        const int k = k0 + at.piece;  // of a row of h2, whose b lies at half of it
+                        const int k = k0 + at.piece;  // of a row of h2: each eight of b meet all their parts
                         if (q < C::QW) {
                             const int o = min(now.n0 + at.row(q), p.outputs - 1);
-                            piece_or_zero(at, k < 2 * p.rank, p.b + ((int64_t)id * p.outputs + o) * p.rank + k / 16 * 8, to);
+                            piece_or_zero(at, k < kParts * p.rank, p.b + ((int64_t)id * p.outputs + o) * p.rank + k / (8 * kParts) * 8, to);
                         } else {
                             const int row = now.r.first + min(at.row(q - C::QW), now.r.count - 1);
-                            piece_or_zero(at, k < 2 * p.rank && own[q - C::QW] == id, p.h2 + (int64_t)row * (2 * p.rank) + k, to);
+                            piece_or_zero(at, k < kParts * p.rank && own[q - C::QW] == id, p.h2 + (int64_t)row * (kParts * p.rank) + k, to);
                         }
                     });
             }
@@ -685,7 +694,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
         run_stages<T, C>(at, src, now.steps, at.wm * (C::M / C::WM) < now.r.count, acc);
 
         // the next tile's first stages are on their way while this one's results are stored
-        if (EXT && apart) add_apart<T, C>(p, at, now.r, n0, places[side][0], acc);
+        if (EXT && apart) add_apart<T, kHParts<T, OUT>, C>(p, at, now.r, n0, places[side][0], acc);
         int done[C::FM];
 #pragma unroll
         for (int j = 0; j < C::FM; j++) done[j] = to[j];
@@ -745,10 +754,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
 
 // ------------------------------------------------------------------ adapters
 
-// h of many rows, summed over its parts, as two parts of 16 bits each: 32 lanes a row.  One part alone would lose up to 2^-8 of h (bf16);
-// two keep 2^-17, about what f32 sums over thousands of inputs are off by, and the products stay those of 16-bit operands.  6 us
-// for 12,661 rows of 64.
-template <int T>
+// h of many rows, summed over its parts of the inputs, as parts of 16 bits: 32 lanes a row.  The products stay those of 16-bit operands; one
+// part alone would lose up to 2^-8 of h.  6 us for 12,661 rows of 64.
+template <int T, int PARTS>
 __global__ void __launch_bounds__(256) halves_kernel(ProductDev p) {
     const int row = blockIdx.x * 8 + (threadIdx.x >> 5), sub = threadIdx.x & 31;
     if (row >= p.entries || adapter_of(p, row) < 0) return;  // 32 lanes together
@@ -773,11 +781,14 @@ __global__ void __launch_bounds__(256) halves_kernel(ProductDev p) {
     for (int i = 0; i < KK_MOST_RANK / 32; i++) {
         const int k = sub + 32 * i;
         if (k >= p.rank) continue;
-        const uint16_t hi = ElemOf<T>::store(v[i] * down);
-        uint16_t* to = p.h2 + (int64_t)row * (2 * p.rank) + k / 8 * 16 + k % 8;
-        const float lo = v[i] * down - ElemOf<T>::load(hi);
-        to[0] = hi;
-        to[8] = ElemOf<T>::store(fabsf(lo) < INFINITY ? lo : 0.0f);  // behind an infinity nothing is left, and not inf - inf
+        uint16_t* to = p.h2 + (int64_t)row * (PARTS * p.rank) + k / 8 * (8 * PARTS) + k % 8;
+        float left = v[i] * down;
+#pragma unroll
+        for (int n = 0; n < PARTS; n++) {
+            to[8 * n] = ElemOf<T>::store(left);
+            left -= ElemOf<T>::load(to[8 * n]);
+            if (!(fabsf(left) < INFINITY)) left = 0.0f;  // behind an infinity nothing is left, and not inf - inf
+        }
     }
 }
 
@@ -891,7 +902,7 @@ static hipError_t adapter_run(ProductDev d, const AdapterPlan& r, hipStream_t s)
     }
     if (d.adapters) {
         rc = launch(shrink_kernel<T, Tile128>, dim3((unsigned)r.main.shrink), dim3(Tile128::kThreads), 0, s, d);
-        if (rc == hipSuccess) rc = launch(halves_kernel<T>, dim3((unsigned)ceil_div(d.entries, 8)), dim3(256), 0, s, d);
+        if (rc == hipSuccess) rc = launch(halves_kernel<T, kHParts<T, OUT>>, dim3((unsigned)ceil_div(d.entries, 8)), dim3(256), 0, s, d);
         if (rc != hipSuccess) return rc;
     }
     ProductDev rest = d;
@@ -900,7 +911,7 @@ static hipError_t adapter_run(ProductDev d, const AdapterPlan& r, hipStream_t s)
     if (rc != hipSuccess || r.rows == rest.entries) return rc;
     const int e = OUT == KK_F32 ? 4 : 2;
     rest.x += r.rows * d.x_row, rest.y = (char*)d.y + r.rows * d.y_row * e, rest.entries -= r.rows;
-    if (d.adapters) rest.adapter += r.rows, rest.h2 += (int64_t)r.rows * 2 * d.rank, rest.h_unit += r.rows;
+    if (d.adapters) rest.adapter += r.rows, rest.h2 += (int64_t)r.rows * kHParts<T, OUT> * d.rank, rest.h_unit += r.rows;
     return d.adapters ? adapter_main<T, true, OUT>(rest, r.rest, s) : adapter_main<T, false, OUT>(rest, r.rest, s);
 }
 

@@ -132,7 +132,7 @@ inline AdapterPlan adapter_plan(const kk_adapter_product_args& a, int n_cu) {
     }
     auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
     r.ws_h2 = a.adapters ? up((int64_t)r.h_splits * a.rows * a.rank * 4) : 0;
-    r.ws_unit = r.ws_h2 + (a.adapters && !r.joined ? up((int64_t)a.rows * a.rank * 4) : 0);
+    r.ws_unit = r.ws_h2 + (a.adapters && !r.joined ? up((int64_t)a.rows * a.rank * 6) : 0);  // up to three parts
     r.ws_part = r.ws_unit + (a.adapters && !r.joined ? up((int64_t)a.rows * 4) : 0);
     r.ws_bytes = r.ws_part + (r.joined ? (int64_t)p.splits * a.rows * a.outputs * 4 : 0);
     return r;

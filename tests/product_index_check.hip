@@ -107,7 +107,7 @@ static int plan() {
         if (r.joined && r.rows != a.rows) return fail("parts of some rows");
         if (a.adapters && ((int64_t)(r.h_splits - 1) * r.h_k >= a.inputs || (int64_t)r.h_splits * r.h_k < a.inputs || r.h_k % 64 || r.slots < 1))
             return fail("the adapters' parts");
-        const int64_t h = a.adapters ? (int64_t)r.h_splits * a.rows * a.rank * 4 : 0, h2 = a.adapters && !r.joined ? (int64_t)a.rows * a.rank * 4 : 0;
+        const int64_t h = a.adapters ? (int64_t)r.h_splits * a.rows * a.rank * 4 : 0, h2 = a.adapters && !r.joined ? (int64_t)a.rows * a.rank * 6 : 0;
         if (h > r.ws_h2 || r.ws_h2 + h2 > r.ws_unit || r.ws_unit + (h2 ? (int64_t)a.rows * 4 : 0) > r.ws_part ||
             r.ws_part + (r.joined ? (int64_t)r.main.splits * a.rows * a.outputs * 4 : 0) > r.ws_bytes || r.ws_h2 % 256 || r.ws_unit % 256 || r.ws_part % 256)
             return fail("the workspace");

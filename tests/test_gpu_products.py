@@ -309,6 +309,26 @@ def test_adapter_product_keeps_requests_apart(ctx, kind, rows, n):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("rows, n, rank", [(40, 100, 24), (6000, 2000, 24), (8300, 2111, 8), (4200, 4096, 40)])
+def test_adapter_product_keeps_f32(ctx, kind, rows, n, rank):
+    """Where y is f32 nothing of a x is lost: whole numbers below 2^24, whose sums in any order are exact, come out as they are."""
+    k, many = 64, 7
+    g = torch.Generator(device="cuda").manual_seed(rank)
+
+    def whole(shape, most):
+        return torch.randint(-most, most + 1, shape, generator=g, device="cuda").to(R.TYPES[kind])
+    x, w = whole((rows, k), 127), whole((n, k), 1)
+    a, b, scale = whole((many, rank, k), 63), whole((many, n, rank), 1), torch.tensor([1.0, -1.0, 0.5, 2.0, 1.0, 0.0, -0.25], device="cuda")
+    ids = torch.sort(torch.randint(-1, many, (rows,), generator=g, device="cuda", dtype=torch.int32)).values
+    want, _ = R.adapter_ref(x, w, None, a, b, scale, ids)
+    size = max((x.float() @ a[i].float().t()).abs().sum(1).max().item() for i in range(many))
+    assert 2 * size + 127 * k < 2 ** 22  # in quarters
+    y = torch.empty(rows, n, device="cuda")
+    R.adapter_run(ctx, R.adapter_args(x, w, y, None, a, b, scale, ids))
+    assert torch.equal(y.double(), want)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
 @pytest.mark.parametrize("rows, n", [(40, 100), (6000, 2000)])
 def test_adapter_product_infinite_rows(ctx, kind, rows, n):
     """An infinity in a row of x stays one where every term has its sign, whether the adapter's share goes through 16-bit parts or not,
@@ -321,12 +341,13 @@ def test_adapter_product_infinite_rows(ctx, kind, rows, n):
     want, bound = R.adapter_ref(x, w, None, a, b, scale, ids)
     up, down, both = [torch.tensor(i, device="cuda") for i in ((1, rows - 3), (5, rows - 4), (7, rows - 5))]
     x[up, 3], x[down, 70], x[both, 5], x[both, 6] = torch.inf, -torch.inf, torch.inf, -torch.inf
-    y = torch.empty(rows, n, dtype=R.TYPES[kind], device="cuda")
-    R.adapter_run(ctx, R.adapter_args(x, w, y, None, a, b, scale, ids))
     good = torch.ones(rows, dtype=torch.bool, device="cuda")
     good[torch.cat([up, down, both])] = False
-    R.close(y[good], want[good], bound[good])
-    assert (y[up] == torch.inf).all() and (y[down] == -torch.inf).all() and torch.isnan(y[both]).all()
+    for out in (kind, "f32"):
+        y = torch.empty(rows, n, dtype=R.TYPES[out], device="cuda")
+        R.adapter_run(ctx, R.adapter_args(x, w, y, None, a, b, scale, ids))
+        R.close(y[good], want[good], bound[good])
+        assert (y[up] == torch.inf).all() and (y[down] == -torch.inf).all() and torch.isnan(y[both]).all()
 
 
 @pytest.mark.parametrize("rows", [3, 300, 6000])
