@@ -488,9 +488,9 @@ int kk_expert_route(kk_ctx* ctx, const kk_expert_route_args* args, void* stream,
  * The layer's first product takes kk_expert_route's `place` as x_place with x_div = top (rows of the layer's input to
  * entries), its second as y_place (entries to rows of y by row and choice, as kk_expert_join reads them).  Rows of y that no
  * entry goes to are left as they were; two entries with one place write the same row, in no order.  y overlaps no input.
- * The result of an entry depends on `entries` and `groups` (by which a tile is chosen: the order of f32 sums), not on the others.
- * One choice is made for the whole call, by entries / groups: where some groups have hundreds of rows and most have few, two calls can
- * take less time. */
+ * The result of an entry depends on `entries`, `groups`, the sizes and the device's compute units (by which a tile is chosen: the
+ * order of f32 sums), not on the other entries.  One choice is made for the whole call, by entries / groups: where some groups have
+ * hundreds of rows and most have few, two calls can take less time. */
 #define KK_GATE_NONE 0
 #define KK_GATE_SILU 1
 #define KK_GATE_GELU 2

@@ -87,8 +87,14 @@ inline ProductPlan expert_plan(const kk_expert_product_args& a, int n_cu) {
     const int64_t mean = a.entries / a.groups;
     // Measured, us, tiles of 64, 128 and 256 rows: 64 groups of 1,024 x 2,048 with 8 rows each 50, 51, 57; 32: 57, 57, 63; 62: 64, 70, 70;
     // 125: 88, 79, 104; 250: 146, 113, 118; 500: 273, 210, 199.  (Tiles of 32 rows: 53, 64, 88.)
-    p.tile = mean <= 40 ? k64 : mean < 450 ? k128Wide : k256;
-    size_grid(p, row_tiles(a.entries, a.groups, kTiles[p.tile].M), (int64_t)a.outputs * (a.gate != KK_GATE_NONE ? 2 : 1), n_cu);
+    const int64_t wide = (int64_t)a.outputs * (a.gate != KK_GATE_NONE ? 2 : 1);
+    auto tiles = [&](int tile) { return a.groups * ceil_div(mean, kTiles[tile].M) * ceil_div(wide, kTiles[tile].N); };
+    // Where the device holds all tiles of 64 rows at once, they leave the fewest CUs idle: 8 groups of 2 x 1,024 x 2,048 with 60 rows each 16
+    // us (of 128 rows 27), 150: 23 (27), 200: 24 (28); 16 groups with 100: 45 (44).  Tiles of 256 rows where their rounds are full: 8 groups
+    // of 4,096 x 4,096 with 900 rows (2 rounds) 267 (of 128 rows 281), with 600 (1.5) 230 (202); 16 of 2 x 1,024 x 2,048 131 (140), 116 (105).
+    const int64_t large = tiles(k256), room = ceil_div(large, n_cu) * n_cu;
+    p.tile = mean <= 40 || tiles(k64) <= 2 * n_cu ? k64 : mean < 450 || large * 10 < room * 9 ? k128Wide : k256;
+    size_grid(p, row_tiles(a.entries, a.groups, kTiles[p.tile].M), wide, n_cu);
     return p;
 }
 

@@ -128,6 +128,13 @@ def test_expert_product(ctx, kind, sizes, k, n):
         assert (y[~written] == 7.0).all() and (room[:, 0] == 7.0).all() and (room[:, n + 1:] == 7.0).all()
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("sizes, k, n", [("many", 72, 4500), ("many", 136, 4613), ("most", 64, 3333), ("largest", 104, 5301), ("largest", 1032, 5312), ("largest", 72, 10611)])
+def test_expert_product_larger_tiles(ctx, kind, sizes, k, n):
+    """The same where there are enough outputs for tiles of 128 and 256 rows."""
+    test_expert_product(ctx, kind, sizes, k, n)
+
+
 @pytest.mark.parametrize("sizes, k, n", [([30, 0, 1, 64, 65] * 20, 72, 1500), ([300, 128, 0, 129] * 5, 200, 5000), ([1900, 0, 700], 64, 16400)])
 def test_expert_product_tile_after_tile(ctx, sizes, k, n):
     """More tiles than the device holds at once, so that blocks go on to others, with places in and out."""
