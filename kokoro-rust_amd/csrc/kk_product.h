@@ -25,7 +25,8 @@ struct ProductDev {
     const int32_t* adapter;
     int adapters, rank;
     int slots, h_splits, h_k;  // blocks that share a row tile's adapters, and its inputs
-    float* h;        // [h_splits][rows][rank], times the adapter's scale
+    int h_rows;      // of the whole call, where a launch takes some
+    float* h;        // [h_splits][h_rows][rank], times the adapter's scale
     uint16_t* h2;    // [rows][parts * rank]: each 8 values' first 16 bits, what these leave, and so on, in units of h_unit[row]
     float* h_unit;   // [rows]
     float* part;     // [splits][entries][outputs]

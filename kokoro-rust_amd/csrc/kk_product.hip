@@ -484,32 +484,39 @@ __device__ __forceinline__ Rows rows_of(const ProductDev& p, const Groups& all, 
 template <int T, int OUT>
 constexpr int kHParts = T == KK_BF16 && OUT == KK_F32 ? 3 : 2;
 
-// The adapters' share of a wave's rows, 32 rows and 32 outputs at a time: each adapter's into sums of its own, of which its rows take theirs.
-template <int T, int PARTS, class C>
+// The adapters' share of a wave's rows once more, each row's from its own adapter's b and h as it was before it was split.
+template <int T, class C>
 __device__ __forceinline__ void add_apart(const ProductDev& p, const Place<C>& at, const Rows& r, int n0, const int* adapters, Acc<T, C>& acc) {
 #pragma unroll
     for (int j = 0; j < C::FM; j++) {
-        const int in = at.wm * (C::M / C::WM) + j * 32 + at.col, row = r.first + min(in, r.count - 1);
-        const int ids[1] = {in < r.count ? adapter_in(p, adapters[in]) : -1};
-        const int all = PARTS * p.rank;
-        const uint16_t* h = p.h2 + (int64_t)row * all;
-        const float unit = T == KK_F16 && ids[0] >= 0 ? p.h_unit[row] : 1.0f;
-        for (int id = next_adapter(ids, -1); id != INT32_MAX; id = next_adapter(ids, id)) {
-            const bool own = ids[0] == id;
+        const int in = at.wm * (C::M / C::WM) + j * 32 + at.col;
+        const int id = in < r.count ? adapter_in(p, adapters[in]) : -1;
+        if (id < 0) continue;
+        const float* h = p.h + (int64_t)(r.first + in) * p.rank;
 #pragma unroll
-            for (int i = 0; i < C::FN; i++) {
-                const uint16_t* b = p.b + ((int64_t)id * p.outputs + min(n0 + i * 32 + at.col, p.outputs - 1)) * p.rank;
-                f32x16 sum;
+        for (int n = 0; n < 4 * C::FN; n++) {  // four outputs at a time: the sums of the whole tile fill the registers
+            int o0 = n0 + n * 8 + at.half * 4;
+            asm volatile("" : "+v"(o0));
+            float sum[4] = {};
+            for (int k0 = 0; k0 < p.rank; k0 += 8) {
+                float v[8] = {};
+                for (int s = 0; s < p.h_splits; s++)
 #pragma unroll
-                for (int k = 0; k < 16; k++) sum[k] = 0.0f;
-                for (int k = at.half * 8; k < all + at.half * 8; k += 16) {  // a lane takes every other piece, and zeros behind the last
-                    const uint4 zero = {0, 0, 0, 0};
-                    const bool in = k < all;
-                    sum = Mat<T>::mul(in ? *(const uint4*)(b + k / (8 * PARTS) * 8) : zero, in && own ? *(const uint4*)(h + k) : zero, sum);
+                    for (int k = 0; k < 8; k++) v[k] += h[(int64_t)s * p.h_rows * p.rank + k0 + k];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    uint16_t b[8];
+                    const uint4 q = *(const uint4*)(p.b + ((int64_t)id * p.outputs + min(o0 + e, p.outputs - 1)) * p.rank + k0);
+                    __builtin_memcpy(b, &q, 16);
+                    float own = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 8; k++) own = fmaf(ElemOf<T>::load(b[k]), v[k], own);
+                    sum[e] += own;
                 }
-#pragma unroll
-                for (int k = 0; k < 16; k++) acc.sum[i][j][k] += own ? sum[k] * unit : 0.0f;
             }
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc.sum[n / 4][j][n % 4 * 4 + e] += sum[e];
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 }
@@ -625,19 +632,17 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
         if constexpr (EXT) {
             // the adapters as more inputs: each one's b beside the rows' h, which is zero in rows of another
             constexpr int kIds = (C::M + 63) / 64, kParts = kHParts<T, OUT>;
-            int ids[kIds], own[C::QX], seen = 0;  // of the tile's rows, a lane each; and of the rows that this lane loads
+            int ids[kIds], own[C::QX];  // of the tile's rows, a lane each; and of the rows that this lane loads
 #pragma unroll
             for (int i = 0; i < kIds; i++) {
                 const int row = i * 64 + at.lane;
                 ids[i] = adapter_in(p, places[side][0][min(row, now.r.count - 1)]);
-                seen += __ballot(ids[i] < 0) != 0;  // rows without one are another kind
             }
-            seen = seen != 0;
 #pragma unroll
             for (int q = 0; q < C::QX; q++) own[q] = adapter_in(p, places[side][0][min(at.row(q), now.r.count - 1)]);
             bool any = false;
             for (int id = next_adapter(ids, -1); id != INT32_MAX; id = next_adapter(ids, id)) {
-                any = true, seen++;
+                any = true;
                 for (int k0 = 0; k0 < kParts * p.rank; k0 += K)
                     run_alone<T, C>(at, acc, [&](int q, uint16_t* to) {
                         const int k = k0 + at.piece;  // of a row of h2: each eight of b meet all their parts
@@ -664,9 +669,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
                             if constexpr (T == KK_F16) acc.sum[n][j][k] *= unit;
                         }
                 }
-                // Zero times an infinity or NaN of one adapter's b is not zero in the rows of another: where something is not finite in a tile
-                // of several kinds, the wave adds the shares apart.
-                apart = seen > 1 && __ballot(size != 0.0f) != 0;
+                // Zero times an infinity or NaN of one adapter's b is not zero in the rows of another, and an infinity of b times the parts of
+                // an h, of which one is zero or of the other sign, is NaN: where something is not finite, the wave adds the shares apart.
+                apart = __ballot(size != 0.0f) != 0;
                 if (apart) acc.clear();
             }
             barrier();
@@ -694,7 +699,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) produc
         run_stages<T, C>(at, src, now.steps, at.wm * (C::M / C::WM) < now.r.count, acc);
 
         // the next tile's first stages are on their way while this one's results are stored
-        if (EXT && apart) add_apart<T, kHParts<T, OUT>, C>(p, at, now.r, n0, places[side][0], acc);
+        if (EXT && apart) add_apart<T, C>(p, at, now.r, n0, places[side][0], acc);
         int done[C::FM];
 #pragma unroll
         for (int j = 0; j < C::FM; j++) done[j] = to[j];
@@ -911,7 +916,7 @@ static hipError_t adapter_run(ProductDev d, const AdapterPlan& r, hipStream_t s)
     if (rc != hipSuccess || r.rows == rest.entries) return rc;
     const int e = OUT == KK_F32 ? 4 : 2;
     rest.x += r.rows * d.x_row, rest.y = (char*)d.y + r.rows * d.y_row * e, rest.entries -= r.rows;
-    if (d.adapters) rest.adapter += r.rows, rest.h2 += (int64_t)r.rows * kHParts<T, OUT> * d.rank, rest.h_unit += r.rows;
+    if (d.adapters) rest.adapter += r.rows, rest.h += (int64_t)r.rows * d.rank, rest.h2 += (int64_t)r.rows * kHParts<T, OUT> * d.rank, rest.h_unit += r.rows;
     return d.adapters ? adapter_main<T, true, OUT>(rest, r.rest, s) : adapter_main<T, false, OUT>(rest, r.rest, s);
 }
 
@@ -927,7 +932,7 @@ hipError_t launch_adapter_product(const kk_adapter_product_args& a, const Adapte
     if (a.adapters) {
         d.a = (const uint16_t*)a.a, d.b = (const uint16_t*)a.b, d.scale = a.scale, d.adapter = a.adapter, d.rank = a.rank;
         d.h = (float*)ws, d.h2 = (uint16_t*)(ws + r.ws_h2), d.h_unit = (float*)(ws + r.ws_unit);
-        d.slots = r.slots, d.h_splits = r.h_splits, d.h_k = r.h_k;
+        d.slots = r.slots, d.h_splits = r.h_splits, d.h_k = r.h_k, d.h_rows = a.rows;
     }
     d.part = (float*)(ws + r.ws_part);
     if (a.type == KK_BF16) return a.out_type == KK_F32 ? adapter_run<KK_BF16, KK_F32>(d, r, s) : adapter_run<KK_BF16, KK_BF16>(d, r, s);
