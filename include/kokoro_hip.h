@@ -454,7 +454,8 @@ int kk_kv_attention(kk_ctx* ctx, const kk_kv_cache* cache, const kk_kv_batch* ba
  *  - An expert whose logit is -inf or NaN is never chosen; +inf counts as the largest finite number.  A row with fewer than
  *    `top` others (padding: none) has expert -1 and weight 0 in the rest.
  *  - weight: KK_SCORE_SOFTMAX, the softmax over all experts of the row; KK_SCORE_SIGMOID, 1 / (1 + exp(-logit)).  With `renorm`
- *    divided by their sum over the row's choices; then times `scale`.  Computed in f32.
+ *    divided by their sum over the row's choices; then times `scale`.  Computed in f32: sigmoids of a row whose largest logit is
+ *    below -780 may be 0 (of a row masked by a type's lowest value they are), and with `renorm` its weights too.
  *  - choice j of row r has the number r * top + j.  start[e]..start[e + 1] are the places of expert e's choices in `place`, which
  *    lists their numbers in rising order; start[experts] of them in all, and -1 behind. */
 #define KK_SCORE_SOFTMAX 0

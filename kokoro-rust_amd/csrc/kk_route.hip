@@ -167,8 +167,8 @@ __global__ void __launch_bounds__(kRouteThreads) choose_kernel(RouteDev a) {
             const uint32_t m = lanes_max<L>(own);
             uint64_t who = __ballot(own == m);
             if constexpr (L == 16) who = who >> (lane & 48) & 0xffff;
+            if (k == 0) most = m ? of_key(m) : 0.0f;
             if (k == 0 && a.score == KK_SCORE_SOFTMAX) {
-                most = m ? of_key(m) : 0.0f;
 #pragma unroll
                 for (int j = 0; j < J; j++) sum += key[j] ? expf(of_key(key[j]) - most) : 0.0f;
                 sum = lanes_sum<L>(sum);
@@ -187,6 +187,15 @@ __global__ void __launch_bounds__(kRouteThreads) choose_kernel(RouteDev a) {
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
+        // Scores in units of exp(unit).  Sigmoids that are divided by their sum have one too, or a row of logits below -88 would have 0 / 0;
+        // it ends at -700, about where 64 bits end: a row masked by a type's lowest value has scores, and weights, of 0.
+        const bool soft = a.score == KK_SCORE_SOFTMAX;
+        const float unit = soft ? most : a.renorm ? fminf(fmaxf(most, -700.0f), 0.0f) : 0.0f;
+        auto score = [&](float v) {
+            if (!soft && v >= 0.0f) return 1.0f / (1.0f + expf(-v));
+            const float x = expf(v - unit);
+            return soft ? x : x / (1.0f + expf(v));
+        };
         float w[kPer], total = 0.0f;
         int e[kPer];
 #pragma unroll
@@ -194,11 +203,11 @@ __global__ void __launch_bounds__(kRouteThreads) choose_kernel(RouteDev a) {
             const int k = sub + i * L;
             e[i] = k < a.top ? chosen[slot][k] : -1;
             const float v = e[i] >= 0 ? value[slot][k] : 0.0f;
-            w[i] = e[i] < 0 ? 0.0f : a.score == KK_SCORE_SOFTMAX ? expf(v - most) : 1.0f / (1.0f + expf(-v));
+            w[i] = e[i] < 0 ? 0.0f : score(v);
             total += w[i];
         }
         total = lanes_sum<L>(total);
-        const float by = a.renorm ? total : a.score == KK_SCORE_SOFTMAX ? sum : 1.0f;
+        const float by = a.renorm ? total : soft ? sum : 1.0f;
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
             const int k = sub + i * L;
