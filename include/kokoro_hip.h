@@ -441,7 +441,8 @@ int kk_kv_attention(kk_ctx* ctx, const kk_kv_cache* cache, const kk_kv_batch* ba
  * twice, kk_expert_join), and projections that all requests share with a low-rank adapter (a voice's, a persona's) for each
  * (kk_adapter_product).  Matrices are [outputs][inputs], inputs next to each other; strides are in values.  Products are of
  * 16-bit operands with f32 sums, rounded once.  What only the device knows (start, places, adapters) is checked by
- * the kernels: `fault` is one word, or NULL, where a kernel that meets a bad one sets KK_PRODUCT_BAD_* bits. */
+ * the kernels: `fault` is one word, or NULL, where a kernel that meets a bad one sets KK_PRODUCT_BAD_* bits.  A call of sizes that are
+ * each within their range is refused all the same (KK_ERR_INVALID) where one launch would have 2^32 threads or more than 2^27 tiles. */
 #define KK_PRODUCT_BAD_START 1   /* a group that leaves [0, entries] or ends before it begins: left out */
 #define KK_PRODUCT_BAD_PLACE 2   /* a place outside x_rows or y_rows: nothing is read or written for its entry */
 #define KK_PRODUCT_BAD_ADAPTER 4 /* an adapter number of `adapters` or more: the row's result is that of a row without one */
@@ -499,8 +500,8 @@ typedef struct {
     int32_t type;           /* KK_BF16 or KK_F16: x, w, y */
     int32_t groups;         /* 1..KK_MOST_EXPERTS */
     int32_t entries;        /* >= 0: start[groups] at most, by which the launch is sized; at most 2^28 */
-    int32_t inputs;         /* a multiple of 8 */
-    int32_t outputs;        /* >= 1 */
+    int32_t inputs;         /* a multiple of 8, at most 2^28 */
+    int32_t outputs;        /* >= 1, at most 2^28 */
     const int32_t* start;   /* [groups + 1], not falling */
     const void* x;          /* 16-byte aligned, as are w and their strides */
     int64_t x_rows, x_row;
@@ -522,8 +523,9 @@ int kk_expert_product(kk_ctx* ctx, const kk_expert_product_args* args, void* str
  * may be `base` (same stride) and overlaps nothing otherwise. */
 typedef struct {
     int32_t type;           /* KK_BF16, KK_F16, KK_F32: y, base, out */
-    int32_t rows, top;      /* rows >= 0; top 1..KK_MOST_CHOICES */
-    int32_t values;         /* of a row, >= 1 */
+    int32_t rows;           /* >= 0, rows * top at most 2^28 */
+    int32_t top;            /* 1..KK_MOST_CHOICES */
+    int32_t values;         /* of a row, >= 1, at most 2^28 */
     const void* y;          /* [rows * top] rows */
     int64_t y_row;
     const int32_t* expert;  /* [rows][top] */
@@ -542,8 +544,8 @@ typedef struct {
     int32_t type;           /* KK_BF16 or KK_F16: x, w, a, b */
     int32_t out_type;       /* `type` or KK_F32: y */
     int32_t rows;           /* >= 0, at most 2^24 */
-    int32_t inputs;         /* a multiple of 8 */
-    int32_t outputs;        /* >= 1 */
+    int32_t inputs;         /* a multiple of 8, at most 2^28 */
+    int32_t outputs;        /* >= 1, at most 2^28 */
     const void* x;          /* 16-byte aligned, as are w, a, b and their strides */
     int64_t x_row;
     const void* w;
