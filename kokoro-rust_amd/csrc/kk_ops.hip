@@ -175,7 +175,7 @@ int kk_expert_join(kk_ctx* ctx, const kk_expert_join_args* args, void* stream, c
         const std::string e = expert_join_error(args);
         if (!e.empty()) return refuse(err, errlen, KK_ERR_INVALID, e);
         if (!ctx) return refuse(err, errlen, KK_ERR_INVALID, "null context");
-        if ((int64_t)args->rows * ((args->values + 63) / 64) > kMostThreads / 64) return refuse(err, errlen, KK_ERR_INVALID, kTooLarge);
+        if (join_waves(*args) > kMostThreads / 256 * 4) return refuse(err, errlen, KK_ERR_INVALID, kTooLarge);
         return entry(ctx, err, errlen, [&] { return args->rows ? launch_join(*args, (hipStream_t)stream) : hipSuccess; });
     });
 }

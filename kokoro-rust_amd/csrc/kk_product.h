@@ -37,6 +37,7 @@ hipError_t launch_expert_product(const kk_expert_product_args& a, const ProductP
 hipError_t launch_adapter_product(const kk_adapter_product_args& a, const AdapterPlan& p, hipStream_t s);
 int64_t route_workspace(const kk_expert_route_args& a);
 hipError_t launch_route(const kk_expert_route_args& a, hipStream_t s);
+int64_t join_waves(const kk_expert_join_args& a);  // of 64 threads
 hipError_t launch_join(const kk_expert_join_args& a, hipStream_t s);
 
 }  // namespace kk

@@ -359,12 +359,18 @@ __global__ void __launch_bounds__(256) join_kernel(JoinDev a) {
 }
 
 template <int T>
-hipError_t run_join(JoinDev d, bool vec, int64_t rows, hipStream_t s) {
-    constexpr int V = T == KK_F32 ? 4 : 8;
-    d.per_row = (int)ceil_div(d.values, vec ? 64 * V : 64);
-    d.waves = (int)(rows * d.per_row);
+hipError_t run_join(const JoinDev& d, bool vec, hipStream_t s) {
     const dim3 grid((unsigned)ceil_div(d.waves, 4)), block(256);
-    return vec ? launch(join_kernel<T, V>, grid, block, 0, s, d) : launch(join_kernel<T, 1>, grid, block, 0, s, d);
+    return vec ? launch(join_kernel<T, T == KK_F32 ? 4 : 8>, grid, block, 0, s, d) : launch(join_kernel<T, 1>, grid, block, 0, s, d);
+}
+
+bool join_vec(const kk_expert_join_args& a) {
+    const int e = a.type == KK_F32 ? 4 : 2;
+    auto whole = [&](const void* p, int64_t row) { return !p || ((uintptr_t)p % 16 == 0 && row * e % 16 == 0); };
+    return a.values * (int64_t)e % 16 == 0 && whole(a.y, a.y_row) && whole(a.base, a.base_row) && whole(a.out, a.out_row);
+}
+int64_t join_per_row(const kk_expert_join_args& a) {
+    return ceil_div(a.values, !join_vec(a) ? 64 : a.type == KK_F32 ? 256 : 512);
 }
 
 // Rows that a block chooses for, and blocks: few enough that adding up their counts stays short.
@@ -411,16 +417,17 @@ hipError_t launch_route(const kk_expert_route_args& a, hipStream_t s) {
     return launch(place_kernel, dim3(d.blocks), dim3(kRouteThreads), lds, s, d);
 }
 
+int64_t join_waves(const kk_expert_join_args& a) { return a.rows * join_per_row(a); }
+
 hipError_t launch_join(const kk_expert_join_args& a, hipStream_t s) {
     JoinDev d{};
     d.y = a.y, d.base = a.base, d.out = a.out, d.y_row = a.y_row, d.base_row = a.base_row, d.out_row = a.out_row;
     d.expert = a.expert, d.weight = a.weight, d.top = a.top, d.values = a.values;
-    const int e = a.type == KK_F32 ? 4 : 2;
-    auto whole = [&](const void* p, int64_t row) { return !p || ((uintptr_t)p % 16 == 0 && row * e % 16 == 0); };
-    const bool vec = a.values * (int64_t)e % 16 == 0 && whole(a.y, a.y_row) && whole(a.base, a.base_row) && whole(a.out, a.out_row);
-    if (a.type == KK_BF16) return run_join<KK_BF16>(d, vec, a.rows, s);
-    if (a.type == KK_F16) return run_join<KK_F16>(d, vec, a.rows, s);
-    return run_join<KK_F32>(d, vec, a.rows, s);
+    d.per_row = (int)join_per_row(a), d.waves = (int)join_waves(a);
+    const bool vec = join_vec(a);
+    if (a.type == KK_BF16) return run_join<KK_BF16>(d, vec, s);
+    if (a.type == KK_F16) return run_join<KK_F16>(d, vec, s);
+    return run_join<KK_F32>(d, vec, s);
 }
 
 }  // namespace kk
