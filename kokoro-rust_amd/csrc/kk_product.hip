@@ -365,7 +365,8 @@ __device__ __forceinline__ void shrink_few(const ProductDev& p, int block, float
 }
 
 // Of many rows: of a row tile, of every slots-th of its adapters, as tiles of the products are.  12,661 rows of 4,096 inputs and rank 64
-// 36-38 us: x (104 MB) is read once for all ranks up to 64, at 2.8 TB/s; two blocks a CU allow the inputs to be split in two at most.
+// 36-38 us in 990 blocks (99 row tiles, two blocks for the adapters of each, the inputs in five parts): x (104 MB) is read once for all ranks up to
+// 64, at 2.8 TB/s; the parts' sums (16 MB) are written here and added up by halves_kernel.
 template <int T, class C>
 __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) shrink_kernel(ProductDev p) {
     constexpr int K = C::K;
@@ -427,7 +428,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerCu * C::kWaves / 4) shrink
 
 // ------------------------------------------------------------------ the products
 
-// The groups' tiles summed up, in LDS: sums[g] of the groups before g, and starts[g].  The block's first wave makes it.
+// The groups' tiles summed up, in LDS: sums[g] of the groups before g, and starts[g].  The block's first wave makes it.  Beside more than some 890
+// groups' eight bytes each, one block of 128 x 64 tiles fits a CU in place of two.
 struct Groups {
     const int *sums, *starts;
     int tiles;

@@ -103,13 +103,19 @@ inline AdapterPlan adapter_plan(const kk_adapter_product_args& a, int n_cu) {
     ProductPlan& p = r.main;
     p.splits = 1, p.k_split = a.inputs;
     auto tiles = [&](int64_t rows, int tile) { return ceil_div(rows, kTiles[tile].M) * ceil_div(a.outputs, kTiles[tile].N); };
+    // us here and below, of 4,096 inputs and outputs where no other are named, both sides measured.  Tiles of 128 rows where they take three
+    // quarters of the CUs: 1,024 rows (half of the CUs) 56, with tiles of 64 51; 1,280 61, 74 (with ten adapters of rank 32 75, 83); 1,600 59, 85;
+    // 1,900 65, 96.
     p.tile = tiles(a.rows, k128Wide) * 4 >= 3 * n_cu ? k128Wide : k64;
     // Parts only where even the smaller tiles leave CUs idle: 1,500 rows of 4,096 x 4,096 69 us without, 111 with them
     r.joined = tiles(a.rows, k64) < n_cu;
     int64_t rows = a.rows;
     if (r.joined) {
+        // tiles of 64 rows and of 128, 6,144 outputs: 32 rows 17, 21; 64: 20, 23; 96: 25.6, 25.4; 128: 27.4, 27.3; 256 rows 26.6, 27.0
         p.tile = a.rows <= 64 ? k64 : k128;
-        // a block for each CU where that splits the inputs, else two: 96 tiles in 2 parts take as long as in 5, with less to sum up
+        // A block for each CU where that splits the inputs, else two: 96 tiles in 2 parts take as long as in 5, with less to sum up.  Parts of 512
+        // inputs or more (of 256, of 1,024): one row 12.1 (12.0, 13.2); 16 rows of 2,048 x 1,024 9.1 (8.5, 10.5); 64 rows of 768 x 768 11.2 (9.4,
+        // 11.2); 200 rows of 2,048 x 2,048 13.3 (13.5, 14.1).
         const int64_t one = tiles(a.rows, p.tile), room = n_cu / one > 1 ? n_cu : 2 * n_cu;
         p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(room / one, a.inputs / 512));
         p.k_split = (int)ceil_div(ceil_div(a.inputs, p.splits), 64) * 64;
@@ -129,10 +135,15 @@ inline AdapterPlan adapter_plan(const kk_adapter_product_args& a, int n_cu) {
     }
     if (a.adapters) {
         const int64_t of_rows = ceil_div(a.rows, r.joined ? 16 : kTiles[k128].M), of_ranks = ceil_div(a.rank, r.joined ? 32 : kTiles[k128].N);
-        // blocks that take 1,024 inputs each; in many rows as few as two a CU allow
+        // A block takes 1,024 inputs (512, 2,048): one row with rank 16 13.7 (14.1, 14.8), 16 rows of 8 adapters 16.6 (16.3, 19.2), 96 rows of 40
+        // with rank 32 into 6,144 33.5 (36.9, 34.1).  In many rows 512 or more (256, 1,024), two row tiles' blocks a CU at most, each with `slots`
+        // blocks of its own: 700 rows of 2,048 inputs, ten adapters 40.5 (38.9, 45.6), 12,661 rows 477 (476, 472).
         const int64_t most = std::max<int64_t>(1, r.joined ? a.inputs / 1024 : std::min<int64_t>(a.inputs / 512, 2 * n_cu / (of_rows * of_ranks)));
         r.h_k = (int)ceil_div(ceil_div(a.inputs, most), 64) * 64;
         r.h_splits = (int)ceil_div(a.inputs, r.h_k);
+        // 16 blocks share a row tile's adapters (4, 2): 16 rows of 8 adapters 16.6 (19.7, 24.9), 96 of 40 into 6,144 33.5 (39.2, 45.4), but 400 of 64
+        // 77 (70, 76).  In many rows 2 (4, 16), made for tiles that hold few requests: 12,661 rows of ten 477 (477, 484), 700 of ten 40.5 (37.4, 38.1).
+        // Where each row is a request's, a tile holds many: 512 rows of 64 adapters 188 (144, 115), 96 rows of 40 into 28,672 182 (147, 124).
         r.slots = (int)std::min<int64_t>(a.adapters, r.joined && a.rows <= 512 ? 16 : 2);
         p.shrink = of_rows * of_ranks * r.slots * r.h_splits;
     }
