@@ -28,7 +28,7 @@ struct ProductDev {
     int h_rows;      // of the whole call, where a launch takes some
     float* h;        // [h_splits][h_rows][rank], times the adapter's scale
     uint16_t* h2;    // [rows][parts * rank]: each 8 values' first 16 bits, what these leave, and so on, in units of h_unit[row]
-    float* h_unit;   // [rows]
+    float* h_unit;   // [rows], NaN where h is
     float* part;     // [splits][entries][outputs]
     int splits, k_split;
 };

@@ -53,3 +53,24 @@ def test_adapter_product_infinite_b(ctx, kind, rows, n, k, rank, order):
         got = y[at].float()
         assert torch.equal(torch.isnan(got), torch.isnan(says))
         assert torch.equal(got[~torch.isnan(says)], says[~torch.isnan(says)])
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("rows, n", [(40, 100), (3000, 1000), (4200, 4096)])
+def test_adapter_product_rows_of_nan(ctx, kind, rows, n):
+    """Rows of NaN (a padded batch's) beside infinities in one adapter's b: those rows are NaN, every other one is what the formula says."""
+    k, rank = 72, 24
+    x, w = _randn((rows, k), 1, kind).abs() + 0.5, _randn((n, k), 2, kind, k ** -0.5)
+    a, b = _randn((3, rank, k), 3, kind, k ** -1).abs() + 0.5 / k, _randn((3, n, rank), 4, kind, rank ** -0.5)
+    scale, ids = torch.ones(3, device="cuda"), (torch.arange(rows, device="cuda") // 5 % 4 - 1).int()
+    want, bound = R.adapter_ref(x, w, None, a, b, scale, ids)
+    none = torch.arange(rows, device="cuda") % 13 == 7
+    x[none], x[none, 3:] = torch.nan, 1.0
+    b[1, ::9, 7] = torch.inf
+    y = torch.empty(rows, n, dtype=R.TYPES[kind], device="cuda")
+    R.adapter_run(ctx, R.adapter_args(x, w, y, None, a, b, scale, ids))
+    far = torch.zeros(rows, n, dtype=torch.bool, device="cuda")
+    far[:, ::9] = (ids == 1)[:, None]
+    assert torch.isnan(y[none]).all() and (y[far & ~none[:, None]] == torch.inf).all()
+    good = ~far & ~none[:, None]
+    R.close(y[good], want[good], bound[good])
